@@ -83,6 +83,30 @@ class AdamWArgs(C.Structure):
                 ("max_norm", C.c_double), ("step", C.c_int), ("decoupled", C.c_int)]
 
 
+class ResidualNormArgs(C.Structure):
+    _fields_ = [("M", C.c_int), ("D", C.c_int), ("dtype", C.c_int), ("stream_dtype", C.c_int), ("gate_dtype", C.c_int),
+                ("post_norm", C.c_int), ("pre_norm", C.c_int), ("gate_rows", C.c_int), ("h", c_fp), ("ldh", C.c_longlong),
+                ("x", c_fp), ("ldx", C.c_longlong), ("gate", c_fp), ("ldg", C.c_longlong), ("post_weight", c_fp), ("post_bias", c_fp),
+                ("pre_weight", c_fp), ("pre_bias", c_fp), ("residual_scale", C.c_float), ("eps", C.c_float), ("x_new", c_fp),
+                ("ldx_new", C.c_longlong), ("y", c_fp), ("ldy", C.c_longlong), ("stats", c_fp)]
+
+
+class ResidualNormGrads(C.Structure):
+    _fields_ = [("d_x_new", c_fp), ("ld_d_x_new", C.c_longlong), ("d_y", c_fp), ("ld_d_y", C.c_longlong), ("h", c_fp), ("ld_h", C.c_longlong),
+                ("x", c_fp), ("ld_x", C.c_longlong), ("gate", c_fp), ("ld_gate", C.c_longlong), ("post_weight", c_fp), ("post_bias", c_fp),
+                ("pre_weight", c_fp), ("pre_bias", c_fp)]
+
+
+class GradTensor(C.Structure):
+    _fields_ = [("grad", c_fp), ("out", c_fp), ("numel", C.c_longlong), ("dtype", C.c_int), ("out_dtype", C.c_int)]
+
+
+class GemmI8Args(C.Structure):
+    _fields_ = [("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("a", c_fp), ("lda", C.c_longlong), ("w", c_fp), ("ldw", C.c_longlong),
+                ("a_scale", c_fp), ("w_scale", c_fp), ("bias", c_fp), ("residual", c_fp), ("ldr", C.c_longlong), ("act", C.c_int),
+                ("out_dtype", C.c_int), ("out", c_fp), ("ldo", C.c_longlong)]
+
+
 OPT_CHUNK = 4096
 OPT_NOALLOC_MAX_CHUNKS = 65536
 KIND_GEMM_F32, KIND_GEMM_BF16, KIND_GROUPNORM, KIND_UPDATE, KIND_GEMM_BF16_T256, KIND_OTHER, KIND_GEMM_BF16_W256 = 0, 1, 2, 3, 4, 5, 6
@@ -125,6 +149,16 @@ SIGNATURES = {
     "adcdiff_clip_adamw_workspace_bytes": (C.c_size_t, [C.c_longlong]),
     "adcdiff_clip_adamw_step": (C.c_int, [c_fp, C.c_int, C.c_longlong, C.POINTER(AdamWArgs), c_fp, c_fp, C.c_size_t, c_fp]),
     "adcdiff_clip_adamw_step_noalloc": (C.c_int, [c_fp, C.c_int, C.c_longlong, C.POINTER(AdamWArgs), c_fp, c_fp]),
+    "adcdiff_residual_norm": (C.c_int, [C.POINTER(ResidualNormArgs), c_fp]),
+    "adcdiff_residual_norm_backward_workspace_bytes": (C.c_size_t, [C.POINTER(ResidualNormArgs), C.POINTER(ResidualNormGrads)]),
+    "adcdiff_residual_norm_backward": (C.c_int, [C.POINTER(ResidualNormArgs), C.POINTER(ResidualNormGrads), c_fp, C.c_size_t, c_fp]),
+    "adcdiff_grad_norm_workspace_bytes": (C.c_size_t, [c_fp, C.c_int]),
+    "adcdiff_grad_norm": (C.c_int, [c_fp, C.c_int, C.c_int, c_fp, c_fp, C.c_size_t, c_fp]),
+    "adcdiff_clip_grad_norm": (C.c_int, [c_fp, C.c_int, C.c_int, C.c_double, c_fp, c_fp, C.c_size_t, c_fp]),
+    "adcdiff_quantize_rows": (C.c_int, [c_fp, C.c_longlong, C.c_int, C.c_int, C.c_int, c_fp, C.c_longlong, c_fp, c_fp]),
+    "adcdiff_gemm_i8_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "adcdiff_gemm_i8": (C.c_int, [C.POINTER(GemmI8Args), c_fp, C.c_size_t, c_fp]),
+    "adcdiff_pitch_rows_i8": (C.c_int, [c_fp, C.c_longlong, C.c_int, C.c_int, c_fp, C.c_longlong, c_fp]),
     "adcdiff_debug_set": (C.c_int, [C.c_char_p, C.c_longlong]),
     "adcdiff_debug_get": (C.c_int, [C.c_char_p, C.POINTER(C.c_longlong)]),
     "adcdiff_timing_begin": (C.c_int, [C.c_int]),

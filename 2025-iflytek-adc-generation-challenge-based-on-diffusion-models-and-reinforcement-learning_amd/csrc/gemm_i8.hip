@@ -1,0 +1,315 @@
+// The 8-bit integer layer: codes of rows with a scale each (activations by row, weights by channel), and their product
+//   out[m, n] = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n] + residual[m, n]).
+// The sum runs on v_mfma_i32_16x16x64_i8 and is exact; what follows is float32 and rounded once.
+#include <algorithm>
+
+#include "row_access.h"
+
+namespace adcdiff {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------ codes of rows
+// A code is rne(x * 127 / top), exactly: t = x * (127 / top) in float32 is off by at most 127 * 2^-23 < 1.6e-5 (one division, one
+// product), so its rounding can only differ from the quotient's where t lies within that of a half; there the quotient is formed
+// in float64, where x * 127 is exact and the division's error is far below the distance of any quotient of two float32 numbers from a
+// half (>= 2^-26).  Below 1e-30, where 127 / top nears overflow, every element takes that path.
+__device__ __forceinline__ int code_of(float x, float top, float inv, bool tiny) {
+    const float t = x * inv, r = rintf(t);
+    if (tiny || fabsf(fabsf(t - r) - 0.5f) < 3.1e-5f) return (int)rint((double)x * 127.0 / (double)top);
+    return (int)r;
+}
+
+struct RowScale {
+    float top, inv, scale;
+    bool poison, tiny, zero;
+    __device__ __forceinline__ explicit RowScale(uint32_t top_bits) {
+        top = __builtin_bit_cast(float, top_bits);
+        poison = top_bits >= 0x7f800000u;   // infinity or NaN (NaN's bits are the larger)
+        zero = top_bits == 0u;
+        tiny = top < 1e-30f;
+        inv = 127.0f / top;
+        scale = poison ? __builtin_nanf("") : top / 127.0f;
+    }
+    __device__ __forceinline__ int code(float x) const { return poison || zero ? 0 : code_of(x, top, inv, tiny); }
+};
+
+template <int TPR>
+__device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red, int tid) {
+#pragma unroll
+    for (int m = (TPR < 64 ? TPR : 64) / 2; m > 0; m >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m));
+    if constexpr (TPR > 64) {
+        if ((tid & 63) == 0) red[tid >> 6] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < TPR / 64; ++w) v = max(v, red[w]);
+        __syncthreads();   // the next row writes red again
+    }
+    return v;
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+
+// one row per team, held in registers between the maximum and the codes
+template <typename T, bool VEC, int TPR, int V>
+__global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int8_t* __restrict__ q,
+                                                                 long long ldq, float* __restrict__ scale) {
+    constexpr int E = 8 * V, TEAMS = kThreads / TPR;
+    __shared__ uint32_t red[kThreads / 64];
+    const int tid = threadIdx.x, t = tid % TPR;
+    // a team wider than a wave is alone in its workgroup, so the barriers of the maximum are met by every thread
+    for (long long row = (long long)blockIdx.x * TEAMS + tid / TPR; row < M; row += (long long)gridDim.x * TEAMS) {
+        float v[E];
+        load_row<T, VEC, TPR, E>(x + row * ldx, t, K, v);
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = max(top, abs_bits(v[e]));
+        const RowScale s(team_max<TPR>(top, red, tid));
+        int8_t* out = q + row * ldq;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int c = (j * TPR + t) * 8;
+                if (c < Kp) {
+                    uint32_t w[2] = {0, 0};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)s.code(v[j * 8 + i]) & 0xffu) << (8 * (i & 3));
+                    *reinterpret_cast<uint2*>(out + c) = uint2{w[0], w[1]};
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int c = e * TPR + t;
+                if (c < Kp) out[c] = (int8_t)s.code(v[e]);
+            }
+        }
+        if (t == 0) scale[row] = s.scale;
+    }
+}
+
+// rows of any length: the row is read twice, the second time out of the cache
+template <typename T>
+__global__ __launch_bounds__(1024) void quantize_long_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int8_t* __restrict__ q, long long ldq,
+                                                                  float* __restrict__ scale) {
+    __shared__ uint32_t red[16];
+    for (long long row = blockIdx.x; row < M; row += gridDim.x) {
+        const T* in = x + row * ldx;
+        uint32_t top = 0;
+        for (int c = threadIdx.x; c < K; c += 1024) top = max(top, abs_bits(to_f(in[c])));
+        const RowScale s(team_max<1024>(top, red, threadIdx.x));
+        int8_t* out = q + row * ldq;
+        for (int c = threadIdx.x; c < Kp; c += 1024) out[c] = c < K ? (int8_t)s.code(to_f(in[c])) : (int8_t)0;
+        if (threadIdx.x == 0) scale[row] = s.scale;
+    }
+}
+
+template <typename T, bool VEC, int TPR, int V>
+void launch_quantize(const void* x, long long ldx, int M, int K, int Kp, int8_t* q, long long ldq, float* scale, hipStream_t stream) {
+    constexpr int teams = kThreads / TPR;
+    hipLaunchKernelGGL((quantize_rows_kernel<T, VEC, TPR, V>), dim3((unsigned)std::min(((long long)M + teams - 1) / teams, 1LL << 20)), dim3(kThreads), 0, stream,
+                       static_cast<const T*>(x), ldx, M, K, Kp, q, ldq, scale);
+}
+
+template <typename T, bool VEC>
+void quantize_by_width(const void* x, long long ldx, int M, int K, int Kp, int8_t* q, long long ldq, float* scale, hipStream_t stream) {
+    if (Kp <= 128) launch_quantize<T, VEC, 16, 1>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+    else if (Kp <= 512) launch_quantize<T, VEC, 64, 1>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+    else if (Kp <= 2048) launch_quantize<T, VEC, 256, 1>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+    else if (Kp <= 4096) launch_quantize<T, VEC, 256, 2>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+    else if (Kp <= 8192) launch_quantize<T, VEC, 256, 4>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+    else hipLaunchKernelGGL((quantize_long_rows_kernel<T>), dim3(std::min(M, 1 << 20)), dim3(1024), 0, stream, static_cast<const T*>(x), ldx, M, K, Kp, q, ldq, scale);
+}
+
+__global__ __launch_bounds__(256) void pitch_rows_kernel(const int8_t* __restrict__ src, long long ld_src, int M, int K, int8_t* __restrict__ dst, long long ld_dst) {
+    // sixteen columns per thread: byte loads at any alignment, one 16-byte store
+    const long long per_row = ld_dst / 16;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= per_row * M) return;
+    const long long row = i / per_row, c = (i - row * per_row) * 16;
+    const int8_t* s = src + row * ld_src + c;
+    const int n = (int)min(16LL, max(0LL, (long long)K - c));
+    u32x4 w = {0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < 16; ++b)
+        if (b < n) w[b >> 2] |= (uint32_t)(uint8_t)s[b] << (8 * (b & 3));
+    *reinterpret_cast<u32x4*>(dst + row * ld_dst + c) = w;
+}
+
+// ------------------------------------------------------------------ product
+struct I8Params {
+    const int8_t *a, *w;
+    const float *a_scale, *w_scale, *bias;
+    const void* residual;
+    void* out;
+    long long lda, ldw, ldr, ldo;
+    int M, N, K, act;
+};
+
+// 16 bytes of a row from column k on, with the bytes at columns >= K cleared.  Rows start on 16-byte boundaries, so a chunk that holds a
+// valid byte never leaves the page of that byte: the bytes behind K may be read, and count for nothing.
+__device__ __forceinline__ i32x4 load_chunk(const int8_t* __restrict__ row, int k, int K) {
+    if (k >= K) return i32x4{0, 0, 0, 0};
+    i32x4 v = *reinterpret_cast<const i32x4*>(row + k);
+    const int keep = K - k;
+    if (keep < 16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int b = keep - 4 * i;
+            v[i] = b >= 4 ? v[i] : b <= 0 ? 0 : v[i] & (int)((1u << (8 * b)) - 1u);
+        }
+    }
+    return v;
+}
+
+template <typename Out>
+__device__ __forceinline__ void finish(const I8Params& p, int m, int n, const i32x4& acc, float sa) {
+    // four consecutive outputs of a row
+    if (m >= p.M) return;
+    const Out* res = static_cast<const Out*>(p.residual) + (long long)m * p.ldr;
+    Out* out = static_cast<Out*>(p.out) + (long long)m * p.ldo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (n + i >= p.N) break;
+        float v = ((float)acc[i] * sa) * p.w_scale[n + i];
+        if (p.bias) v += p.bias[n + i];
+        if (p.residual) v += (float)res[n + i];
+        if (p.act) v = silu_f(v);
+        out[n + i] = (Out)v;
+    }
+}
+
+// BM x BN tile, 4 waves in WM x WN, K in steps of 128 through two LDS stages filled from registers.  LDS rows of 128 bytes, the
+// 16-byte chunk c of a row at position c ^ ((row >> 1) & 7): fragment reads are free of bank conflicts.  The weights are the MFMA's
+// first operand, so a lane's four results are four consecutive outputs of one row.
+template <typename Out, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(256) void gemm_i8_kernel(const I8Params p) {
+    constexpr int TM = BM / WM / 16, TN = BN / WN / 16, CHUNKS = (BM + BN) * 8 / 256;
+    __shared__ __attribute__((aligned(16))) char smem[2][(BM + BN) * 128];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave / WN, wn = wave % WN;
+    const int ntn = (p.N + BN - 1) / BN;
+    const int m0 = blockIdx.x / ntn * BM, n0 = blockIdx.x % ntn * BN;
+    const int8_t* src[CHUNKS];
+    int dst[CHUNKS];
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+        const int id = tid + 256 * j, r = id >> 3, c = id & 7;
+        src[j] = (r < BM ? p.a + (long long)min(m0 + r, p.M - 1) * p.lda : p.w + (long long)min(n0 + r - BM, p.N - 1) * p.ldw);
+        dst[j] = r * 128 + ((c ^ ((r >> 1) & 7)) << 4);
+    }
+    i32x4 acc[TM][TN] = {};
+    i32x4 next[CHUNKS];
+    const int kc = (tid & 7) * 16;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) next[j] = load_chunk(src[j], kc, p.K);
+    const int tiles = (p.K + 127) / 128;
+    for (int t = 0; t < tiles; ++t) {
+        char* st = smem[t & 1];
+#pragma unroll
+        for (int j = 0; j < CHUNKS; ++j) *reinterpret_cast<i32x4*>(st + dst[j]) = next[j];
+        if (t + 1 < tiles) {
+#pragma unroll
+            for (int j = 0; j < CHUNKS; ++j) next[j] = load_chunk(src[j], (t + 1) * 128 + kc, p.K);
+        }
+        __syncthreads();   // one per tile: a stage is written again only after the barrier of the tile in between
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            i32x4 fa[TM], fw[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const int r = wm * TM * 16 + i * 16 + (lane & 15);
+                fa[i] = *reinterpret_cast<const i32x4*>(st + r * 128 + (((4 * h + (lane >> 4)) ^ ((r >> 1) & 7)) << 4));
+            }
+#pragma unroll
+            for (int i = 0; i < TN; ++i) {
+                const int r = BM + wn * TN * 16 + i * 16 + (lane & 15);
+                fw[i] = *reinterpret_cast<const i32x4*>(st + r * 128 + (((4 * h + (lane >> 4)) ^ ((r >> 1) & 7)) << 4));
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fa[i], acc[i][j], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int m = m0 + wm * TM * 16 + i * 16 + (lane & 15);
+        const float sa = m < p.M ? p.a_scale[m] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) finish<Out>(p, m, n0 + wn * TN * 16 + j * 16 + 4 * (lane >> 4), acc[i][j], sa);
+    }
+}
+
+template <typename Out, int BM, int BN>
+int launch_tiles(const I8Params& p, hipStream_t stream) {
+    const long long tiles = (((long long)p.M + BM - 1) / BM) * (((long long)p.N + BN - 1) / BN);
+    if (tiles > 0xffffff) return fail(ADCDIFF_E_BADARG, "gemm_i8: %d x %d outputs are too many for one call", p.M, p.N);
+    hipLaunchKernelGGL((gemm_i8_kernel<Out, BM, BN, 2, 2>), dim3((unsigned)tiles), dim3(256), 0, stream, p);
+    return check_launch("gemm_i8");
+}
+
+template <typename Out>
+int launch_gemm(const I8Params& p, hipStream_t stream) {
+    return p.M <= 32 ? launch_tiles<Out, 32, 32>(p, stream) : launch_tiles<Out, 128, 128>(p, stream);
+}
+
+constexpr int kMaxK = 131071;   // 128 * 128 * K stays below 2^31
+
+}  // namespace
+}  // namespace adcdiff
+
+extern "C" int adcdiff_quantize_rows(const void* x, long long ldx, int dtype, int M, int K, int8_t* q, long long ldq, float* scale, adcdiff_stream_t stream_) {
+    using namespace adcdiff;
+    if (M < 0 || K < 1) return fail(ADCDIFF_E_BADARG, "quantize_rows: %d rows of %d columns", M, K);
+    if (!type_ok(dtype)) return fail(ADCDIFF_E_BADARG, "quantize_rows: type %d", dtype);
+    if (M == 0) return ADCDIFF_OK;
+    if (!x || !q || !scale) return fail(ADCDIFF_E_BADARG, "quantize_rows: null pointer");
+    if (ldx < K || ldq < K) return fail(ADCDIFF_E_BADARG, "quantize_rows: a row pitch below %d columns", K);
+    hipStream_t stream = as_stream(stream_);
+    const int Kp = (int)std::min<long long>(ldq, ((long long)K + 15) / 16 * 16);
+    TimingScope timing(ADCDIFF_KIND_OTHER, M, K, 0, 0.0, (double)M * K * (type_size(dtype) + 1), stream);
+    const bool vec = K % 8 == 0 && Kp % 8 == 0 && vector_rows(x, ldx, type_size(dtype)) && reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
+    if (dtype == ADCDIFF_BF16) {
+        if (vec) quantize_by_width<bf16_t, true>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+        else quantize_by_width<bf16_t, false>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+    } else {
+        if (vec) quantize_by_width<float, true>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+        else quantize_by_width<float, false>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+    }
+    return check_launch("quantize_rows");
+}
+
+extern "C" int adcdiff_pitch_rows_i8(const int8_t* src, long long ld_src, int M, int K, int8_t* dst, long long ld_dst, adcdiff_stream_t stream_) {
+    using namespace adcdiff;
+    if (M < 0 || K < 1 || ld_src < K || ld_dst < K || ld_dst % 16 != 0) return fail(ADCDIFF_E_BADARG, "pitch_rows_i8: %d rows of %d columns, pitches %lld -> %lld", M, K, ld_src, ld_dst);
+    if (M == 0) return ADCDIFF_OK;
+    if (!src || !dst || !aligned16(dst)) return fail(ADCDIFF_E_BADARG, "pitch_rows_i8: null pointer, or a destination off its 16-byte boundary");
+    const long long threads = ld_dst / 16 * M;
+    if (threads > 0x7fffffffLL * 128) return fail(ADCDIFF_E_BADARG, "pitch_rows_i8: too many rows");
+    hipStream_t stream = as_stream(stream_);
+    TimingScope timing(ADCDIFF_KIND_OTHER, M, K, 0, 0.0, 2.0 * M * K, stream);
+    hipLaunchKernelGGL(pitch_rows_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, src, ld_src, M, K, dst, ld_dst);
+    return check_launch("pitch_rows_i8");
+}
+
+extern "C" size_t adcdiff_gemm_i8_workspace_bytes(int, int, int) { return 0; }
+
+extern "C" int adcdiff_gemm_i8(const adcdiff_gemm_i8_args* a, void*, size_t, adcdiff_stream_t stream_) {
+    using namespace adcdiff;
+    if (!a) return fail(ADCDIFF_E_BADARG, "gemm_i8: null args");
+    if (a->M < 0 || a->N < 1 || a->K < 1 || a->K > kMaxK) return fail(ADCDIFF_E_BADARG, "gemm_i8: M %d, N %d, K %d (1..%d)", a->M, a->N, a->K, kMaxK);
+    if (!type_ok(a->out_dtype) || (a->act != 0 && a->act != 1)) return fail(ADCDIFF_E_BADARG, "gemm_i8: type %d, act %d", a->out_dtype, a->act);
+    if (a->M == 0) return ADCDIFF_OK;
+    if (!a->a || !a->w || !a->a_scale || !a->w_scale || !a->out) return fail(ADCDIFF_E_BADARG, "gemm_i8: null pointer");
+    if (!aligned16(a->a) || !aligned16(a->w) || a->lda % 16 != 0 || a->ldw % 16 != 0 || a->lda < a->K || a->ldw < a->K)
+        return fail(ADCDIFF_E_BADARG, "gemm_i8: the rows of a and w start on 16-byte boundaries and hold %d columns (pitches %lld, %lld)", a->K, a->lda, a->ldw);
+    if (a->ldo < a->N || (a->residual && a->ldr < a->N)) return fail(ADCDIFF_E_BADARG, "gemm_i8: a row pitch below %d columns", a->N);
+    hipStream_t stream = as_stream(stream_);
+    I8Params p{a->a, a->w, a->a_scale, a->w_scale, a->bias, a->residual, a->out, a->lda, a->ldw, a->ldr, a->ldo, a->M, a->N, a->K, a->act};
+    const int so = type_size(a->out_dtype);
+    TimingScope timing(ADCDIFF_KIND_OTHER, a->M, a->N, a->K, 2.0 * a->M * a->N * a->K,
+                       (double)a->M * a->K + (double)a->N * a->K + (double)a->M * a->N * so * (a->residual ? 2 : 1), stream);
+    return a->out_dtype == ADCDIFF_BF16 ? launch_gemm<bf16_t>(p, stream) : launch_gemm<float>(p, stream);
+}

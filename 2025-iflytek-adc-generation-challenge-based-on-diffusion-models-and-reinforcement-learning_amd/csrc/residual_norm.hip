@@ -1,0 +1,533 @@
+// The norms before and after a residual block, fused with the block's gate and the residual scale, and their gradients:
+//   x' = residual_scale * x + gate . N_post(h),   y = N_pre(x'),   N(v) = (v - [mean]) / sqrt(mean((v - [mean])^2) + eps) . weight + bias
+// The bracketed mean belongs to the layer norm; the rms norm has none.  All arithmetic is float32; h, y share one type, x, x' another,
+// the gate has its own, and each output is rounded once.  y is formed from the unrounded x'.
+//
+// A team of TPR threads owns a row and holds it in registers (V vectors of 8 columns per thread), so every pass over the row after the
+// first load is free; both kernels are bound by HBM.  Statistics are two-pass (mean, then centred squares) on those registers.
+#include <algorithm>
+
+#include "row_access.h"
+
+namespace adcdiff {
+namespace {
+
+struct ResNormParams {
+    const void *h, *x, *gate;
+    const float *post_w, *post_b, *pre_w, *pre_b;
+    void *xn, *y;
+    float* stats;                 // [M, 4]: post mean, 1 / post deviation, pre mean, 1 / pre deviation
+    long long ldh, ldx, ldg, ldxn, ldy;
+    int M, D, post, pre, gate_bf16, gate_share;   // gate_share: rows per gate row
+    float scale, eps, inv_d;
+};
+
+struct ResNormGradParams {
+    ResNormParams f;
+    const void *d_xn, *d_y;
+    void *d_h, *d_x, *d_gate;
+    long long ld_dxn, ld_dy, ld_dh, ld_dx, ld_dg;
+    float* partial;               // [workgroups][vectors][D] weight and bias gradients of a workgroup's rows
+    float* gate_partial;          // [chunks][D] gate gradients, where several chunks share a gate row
+    int slot_post_w, slot_post_b, slot_pre_w, slot_pre_b, vectors;   // row of each vector in a workgroup's partials, or -1
+    int chunks, chunk_rows, chunks_per_gate;
+    int group_rows;               // rows of one gate row (M where the gate's gradient is not summed over rows)
+};
+
+template <bool VEC, int TPR, int E>
+__device__ __forceinline__ void load_gate(const void* gate, int bf16, long long offset, int t, int D, float (&v)[E]) {
+    if (bf16) load_row<bf16_t, VEC, TPR, E>(static_cast<const bf16_t*>(gate) + offset, t, D, v);
+    else load_row<float, VEC, TPR, E>(static_cast<const float*>(gate) + offset, t, D, v);
+}
+
+// mean and 1 / sqrt(variance + eps) of the row in v (mean = 0 for the rms norm); what stands in columns >= D is left out
+template <bool VEC, int TPR, int E, typename Sum>
+__device__ __forceinline__ void row_stats(const float (&v)[E], int kind, int t, int tid, int D, float inv_d, float eps, Sum& sum, float& mean, float& inv) {
+    float s[1] = {0.0f};
+    mean = 0.0f;
+    if (kind == 2) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[0] += column<VEC, TPR>(t, e) < D ? v[e] : 0.0f;
+        sum(s, tid);
+        mean = s[0] * inv_d;
+        s[0] = 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float c = column<VEC, TPR>(t, e) < D ? v[e] - mean : 0.0f;
+        s[0] = fmaf(c, c, s[0]);
+    }
+    sum(s, tid);
+    inv = 1.0f / sqrtf(fmaf(s[0], inv_d, eps));
+}
+
+template <typename T, typename R, bool VEC, int TPR, int V>
+__global__ __launch_bounds__(kThreads) void residual_norm_kernel(const ResNormParams p) {
+    constexpr int E = 8 * V, TEAMS = kThreads / TPR;
+    __shared__ float red[2 * (kThreads / 64)];
+    const int tid = threadIdx.x, t = tid % TPR, D = p.D;
+    TeamSum<TPR, 1> sum(red);
+    // Teams wider than a wave are one per workgroup, so the barriers inside the sums are met by every thread.
+    for (long long row = (long long)blockIdx.x * TEAMS + tid / TPR; row < p.M; row += (long long)gridDim.x * TEAMS) {
+        float v[E], w[E];
+        float post_mean = 0.0f, post_inv = 1.0f, pre_mean = 0.0f, pre_inv = 1.0f;
+        load_row<R, VEC, TPR, E>(static_cast<const R*>(p.x) + row * p.ldx, t, D, v);
+        if (p.h) {
+            float u[E];
+            load_row<T, VEC, TPR, E>(static_cast<const T*>(p.h) + row * p.ldh, t, D, u);
+            if (p.post) {
+                row_stats<VEC, TPR, E>(u, p.post, t, tid, D, p.inv_d, p.eps, sum, post_mean, post_inv);
+#pragma unroll
+                for (int e = 0; e < E; ++e) u[e] = (u[e] - post_mean) * post_inv;
+                if (p.post_w) {
+                    load_row<float, VEC, TPR, E>(p.post_w, t, D, w);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) u[e] *= w[e];
+                }
+                if (p.post_b) {
+                    load_row<float, VEC, TPR, E>(p.post_b, t, D, w);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) u[e] += w[e];
+                }
+            }
+            if (p.gate) {
+                load_gate<VEC, TPR, E>(p.gate, p.gate_bf16, (p.gate_share == 1 ? row : row / p.gate_share) * p.ldg, t, D, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) u[e] *= w[e];
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = fmaf(p.scale, v[e], u[e]);
+        }
+        if (p.xn) store_row<R, VEC, TPR, E>(static_cast<R*>(p.xn) + row * p.ldxn, t, D, v);
+        if (p.pre) {
+            row_stats<VEC, TPR, E>(v, p.pre, t, tid, D, p.inv_d, p.eps, sum, pre_mean, pre_inv);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = (v[e] - pre_mean) * pre_inv;
+            if (p.pre_w) {
+                load_row<float, VEC, TPR, E>(p.pre_w, t, D, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] *= w[e];
+            }
+            if (p.pre_b) {
+                load_row<float, VEC, TPR, E>(p.pre_b, t, D, w);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] += w[e];
+            }
+            store_row<T, VEC, TPR, E>(static_cast<T*>(p.y) + row * p.ldy, t, D, v);
+        }
+        if (p.stats && t == 0) *reinterpret_cast<f32x4*>(p.stats + row * 4) = f32x4{post_mean, post_inv, pre_mean, pre_inv};
+    }
+}
+
+// Gradients.  With u = N_post(h), xhat / uhat the normalised rows, g the gradient of a norm's output times its weight:
+//   d = d_x' + (g - [mean g] - xhat mean(g xhat)) / deviation      (g = d_y . pre_weight)
+//   d_x = residual_scale d,   d_gate = d . u,   d_h = N_post's gradient of d . gate,   d_weight = sum over rows of d_y . xhat, ...
+// x' and u are formed again from h and x in float32 (the rounded x' would cost the same traffic as x and lose bits); the statistics
+// come from the forward pass.  The rows are cut into chunks of consecutive rows that share a gate row; a team runs over chunks with
+// its column sums in registers, so weights cost one partial row per workgroup and the gate one row per chunk.  The partial rows are
+// added in a fixed order by column_sum_kernel: no atomics, results do not change from run to run.
+template <typename T, typename R, bool VEC, int TPR>
+__global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads) void residual_norm_grad_kernel(const ResNormGradParams q) {
+    constexpr int E = 8, THREADS = TPR > kThreads ? TPR : kThreads, TEAMS = THREADS / TPR;
+    __shared__ float red[4 * (THREADS / 64)];
+    __shared__ float joined[TEAMS > 1 ? THREADS * E : 1];
+    const ResNormParams& p = q.f;
+    const int tid = threadIdx.x, t = tid % TPR, team = tid / TPR, D = p.D;
+    TeamSum<TPR, 2> sum(red);
+    float a_pre_w[E] = {}, a_pre_b[E] = {}, a_post_w[E] = {}, a_post_b[E] = {};
+    const int teams = gridDim.x * TEAMS;
+    // Every team of a workgroup makes the same number of turns (barriers inside the sums); turns without a row do nothing.
+    for (int c0 = blockIdx.x * TEAMS; c0 < q.chunks; c0 += teams) {
+        const int c = c0 + team;
+        const int group = c / q.chunks_per_gate;
+        const long long first = (long long)group * q.group_rows + (long long)(c % q.chunks_per_gate) * q.chunk_rows;
+        const long long last = c < q.chunks ? min(first + q.chunk_rows, (long long)(group + 1) * q.group_rows) : first;
+        float a_gate[E] = {};
+        for (int r = 0; r < q.chunk_rows; ++r) {
+            const long long row = first + r;
+            const bool live = row < last;
+            float d[E], v[E], u[E], w[E], s[2];
+            f32x4 st = {0.0f, 1.0f, 0.0f, 1.0f};
+#pragma unroll
+            for (int e = 0; e < E; ++e) d[e] = v[e] = u[e] = 0.0f;
+            if (live) {
+                if (p.post || p.pre) st = *reinterpret_cast<const f32x4*>(p.stats + row * 4);
+                if (q.d_xn) load_row<R, VEC, TPR, E>(static_cast<const R*>(q.d_xn) + row * q.ld_dxn, t, D, d);
+                if (p.pre) load_row<R, VEC, TPR, E>(static_cast<const R*>(p.x) + row * p.ldx, t, D, v);
+                if (p.h) load_row<T, VEC, TPR, E>(static_cast<const T*>(p.h) + row * p.ldh, t, D, u);
+            }
+            float uhat[E], gate[E];
+            if (p.h) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) gate[e] = 1.0f;
+                if (p.gate && live) load_gate<VEC, TPR, E>(p.gate, p.gate_bf16, (row / p.gate_share) * p.ldg, t, D, gate);
+#pragma unroll
+                for (int e = 0; e < E; ++e) uhat[e] = u[e];
+                if (p.post) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) uhat[e] = u[e] = (u[e] - st[0]) * st[1];
+                    if (p.post_w) {
+                        load_row<float, VEC, TPR, E>(p.post_w, t, D, w);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) u[e] *= w[e];
+                    }
+                    if (p.post_b) {
+                        load_row<float, VEC, TPR, E>(p.post_b, t, D, w);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) u[e] += w[e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = fmaf(p.scale, v[e], gate[e] * u[e]);
+            }
+            if (p.pre) {
+                float g[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) g[e] = 0.0f;
+                if (live && q.d_y) load_row<T, VEC, TPR, E>(static_cast<const T*>(q.d_y) + row * q.ld_dy, t, D, g);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    v[e] = (v[e] - st[2]) * st[3];
+                    if (live) {
+                        a_pre_w[e] = fmaf(g[e], v[e], a_pre_w[e]);
+                        a_pre_b[e] += g[e];
+                    }
+                }
+                if (p.pre_w) {
+                    load_row<float, VEC, TPR, E>(p.pre_w, t, D, w);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) g[e] *= w[e];
+                }
+                s[0] = s[1] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (column<VEC, TPR>(t, e) < D) { s[0] += g[e]; s[1] = fmaf(g[e], v[e], s[1]); }
+                sum(s, tid);
+                const float m0 = p.pre == 2 ? s[0] * p.inv_d : 0.0f, m1 = s[1] * p.inv_d;
+#pragma unroll
+                for (int e = 0; e < E; ++e) d[e] = fmaf(g[e] - m0 - v[e] * m1, st[3], d[e]);
+            }
+            if (q.d_x && live) {
+                float o[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = p.scale * d[e];
+                store_row<R, VEC, TPR, E>(static_cast<R*>(q.d_x) + row * q.ld_dx, t, D, o);
+            }
+            if (p.h) {
+                if (q.d_gate) {
+                    if (p.gate_share == 1) {
+                        if (live) {
+                            float o[E];
+#pragma unroll
+                            for (int e = 0; e < E; ++e) o[e] = d[e] * u[e];
+                            if (p.gate_bf16) store_row<bf16_t, VEC, TPR, E>(static_cast<bf16_t*>(q.d_gate) + row * q.ld_dg, t, D, o);
+                            else store_row<float, VEC, TPR, E>(static_cast<float*>(q.d_gate) + row * q.ld_dg, t, D, o);
+                        }
+                    } else if (live) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) a_gate[e] = fmaf(d[e], u[e], a_gate[e]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) d[e] *= gate[e];
+                if (p.post) {
+                    if (live) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) { a_post_w[e] = fmaf(d[e], uhat[e], a_post_w[e]); a_post_b[e] += d[e]; }
+                    }
+                    if (p.post_w) {
+                        load_row<float, VEC, TPR, E>(p.post_w, t, D, w);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) d[e] *= w[e];
+                    }
+                    s[0] = s[1] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (column<VEC, TPR>(t, e) < D) { s[0] += d[e]; s[1] = fmaf(d[e], uhat[e], s[1]); }
+                    sum(s, tid);
+                    const float m0 = p.post == 2 ? s[0] * p.inv_d : 0.0f, m1 = s[1] * p.inv_d;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) d[e] = (d[e] - m0 - uhat[e] * m1) * st[1];
+                }
+                if (q.d_h && live) store_row<T, VEC, TPR, E>(static_cast<T*>(q.d_h) + row * q.ld_dh, t, D, d);
+            }
+        }
+        if (q.d_gate && p.gate_share != 1 && c < q.chunks) {
+            if (q.chunks_per_gate > 1) store_row<float, VEC, TPR, E>(q.gate_partial + (long long)c * D, t, D, a_gate);
+            else if (p.gate_bf16) store_row<bf16_t, VEC, TPR, E>(static_cast<bf16_t*>(q.d_gate) + group * q.ld_dg, t, D, a_gate);
+            else store_row<float, VEC, TPR, E>(static_cast<float*>(q.d_gate) + group * q.ld_dg, t, D, a_gate);
+        }
+    }
+    float* out = q.partial + (long long)blockIdx.x * q.vectors * D;
+    auto flush = [&](float (&a)[E], int slot) {
+        if (slot < 0) return;
+        if constexpr (TEAMS > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; ++e) joined[e * THREADS + tid] = a[e];
+            __syncthreads();
+            if (team == 0) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    for (int k = 1; k < TEAMS; ++k) a[e] += joined[e * THREADS + k * TPR + t];
+            }
+        }
+        if (team == 0) store_row<float, VEC, TPR, E>(out + (long long)slot * D, t, D, a);
+    };
+    flush(a_pre_w, q.slot_pre_w);
+    flush(a_pre_b, q.slot_pre_b);
+    flush(a_post_w, q.slot_post_w);
+    flush(a_post_b, q.slot_post_b);
+}
+
+// out[seg][col] = sum over i < count of part[seg * seg_stride + i * row_stride + col], in a fixed order: 32 columns x 32 row groups
+// per workgroup, each thread a strided share of the rows, then a tree over the groups.  Segments 0 .. vectors - 1 are the weight and
+// bias gradients, the others the gate rows.
+struct ColumnSumParams {
+    const float *partial, *gate_partial;
+    float* out[4];
+    void* d_gate;
+    long long ld_dg;
+    int D, vectors, segments, workgroups, chunks_per_gate, gate_bf16;
+};
+
+__global__ __launch_bounds__(1024) void column_sum_kernel(const ColumnSumParams p) {
+    __shared__ float part[32][33];
+    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
+    const int col = blockIdx.x * 32 + cx;
+    for (int seg = blockIdx.y; seg < p.segments; seg += gridDim.y) {
+        const bool weight = seg < p.vectors;
+        const float* src = weight ? p.partial + (long long)seg * p.D : p.gate_partial + (long long)(seg - p.vectors) * p.chunks_per_gate * p.D;
+        const long long step = weight ? (long long)p.vectors * p.D : p.D;
+        const int count = weight ? p.workgroups : p.chunks_per_gate;
+        float s = 0.0f;
+        if (col < p.D) {
+#pragma unroll 4
+            for (int i = ry; i < count; i += 32) s += src[i * step + col];
+        }
+        part[ry][cx] = s;
+        __syncthreads();
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) {
+            if (ry < m) part[ry][cx] += part[ry + m][cx];
+            __syncthreads();
+        }
+        if (ry == 0 && col < p.D) {
+            if (weight) p.out[seg][col] = part[0][cx];
+            else if (p.gate_bf16) static_cast<bf16_t*>(p.d_gate)[(long long)(seg - p.vectors) * p.ld_dg + col] = (bf16_t)part[0][cx];
+            else static_cast<float*>(p.d_gate)[(long long)(seg - p.vectors) * p.ld_dg + col] = part[0][cx];
+        }
+        __syncthreads();
+    }
+}
+
+bool norm_kind(int k) { return k >= 0 && k <= 2; }
+
+constexpr int kMaxD = 8192;
+
+int check_args(const char* who, const adcdiff_residual_norm_args* a) {
+    if (!a) return fail(ADCDIFF_E_BADARG, "%s: null args", who);
+    if (a->M < 0 || a->D < 1 || a->D > kMaxD) return fail(ADCDIFF_E_BADARG, "%s: %d rows of %d columns (1..%d)", who, a->M, a->D, kMaxD);
+    if (!type_ok(a->dtype) || !type_ok(a->stream_dtype) || (a->gate && !type_ok(a->gate_dtype)))
+        return fail(ADCDIFF_E_BADARG, "%s: types %d, %d, %d are not ADCDIFF_F32 / ADCDIFF_BF16", who, a->dtype, a->stream_dtype, a->gate_dtype);
+    if (!norm_kind(a->post_norm) || !norm_kind(a->pre_norm)) return fail(ADCDIFF_E_BADARG, "%s: norms %d, %d", who, a->post_norm, a->pre_norm);
+    if (!(a->eps >= 0.0f)) return fail(ADCDIFF_E_BADARG, "%s: eps %g", who, (double)a->eps);
+    if (a->M > 0 && !a->x) return fail(ADCDIFF_E_BADARG, "%s: null x", who);
+    if (a->M > 0 && !a->h && (a->gate || a->post_norm || a->residual_scale != 1.0f))
+        return fail(ADCDIFF_E_BADARG, "%s: a gate, a post norm or a residual scale without h", who);
+    if ((!a->post_norm && (a->post_weight || a->post_bias)) || (!a->pre_norm && (a->pre_weight || a->pre_bias)))
+        return fail(ADCDIFF_E_BADARG, "%s: a weight or bias without its norm", who);
+    if (a->gate && (a->gate_rows < 1 || a->M % a->gate_rows != 0) && a->M > 0)
+        return fail(ADCDIFF_E_BADARG, "%s: %d gate rows do not divide %d rows", who, a->gate_rows, a->M);
+    if ((a->h && a->ldh < a->D) || (a->x && a->ldx < a->D) || (a->gate && a->gate_rows > 1 && a->ldg != 0 && a->ldg < a->D))
+        return fail(ADCDIFF_E_BADARG, "%s: a row pitch below %d columns", who, a->D);
+    return ADCDIFF_OK;
+}
+
+ResNormParams forward_params(const adcdiff_residual_norm_args& a) {
+    ResNormParams p{};
+    p.h = a.h; p.x = a.x; p.gate = a.gate;
+    p.post_w = a.post_weight; p.post_b = a.post_bias; p.pre_w = a.pre_weight; p.pre_b = a.pre_bias;
+    p.xn = a.x_new; p.y = a.y; p.stats = a.stats;
+    p.ldh = a.ldh; p.ldx = a.ldx; p.ldg = a.ldg; p.ldxn = a.ldx_new; p.ldy = a.ldy;
+    p.M = a.M; p.D = a.D; p.post = a.h ? a.post_norm : 0; p.pre = a.pre_norm;
+    p.gate_bf16 = a.gate_dtype == ADCDIFF_BF16;
+    p.gate_share = a.gate && a.M > 0 ? a.M / a.gate_rows : 1;
+    p.scale = a.residual_scale; p.eps = a.eps; p.inv_d = 1.0f / (float)a.D;
+    return p;
+}
+
+bool vector_inputs(const adcdiff_residual_norm_args& a) {
+    const int st = type_size(a.dtype), sr = type_size(a.stream_dtype), sg = type_size(a.gate_dtype);
+    return a.D % 8 == 0 && vector_rows(a.h, a.ldh, st) && vector_rows(a.x, a.ldx, sr) && vector_rows(a.gate, a.ldg, sg) &&
+           vector_rows(a.post_weight, 0, 4) && vector_rows(a.post_bias, 0, 4) && vector_rows(a.pre_weight, 0, 4) && vector_rows(a.pre_bias, 0, 4);
+}
+
+template <typename T, typename R, bool VEC, int TPR, int V>
+void launch_forward(const ResNormParams& p, hipStream_t stream) {
+    constexpr int teams = kThreads / TPR;
+    const long long groups = ((long long)p.M + teams - 1) / teams;
+    hipLaunchKernelGGL((residual_norm_kernel<T, R, VEC, TPR, V>), dim3((unsigned)std::min<long long>(groups, 1 << 20)), dim3(kThreads), 0, stream, p);
+}
+
+// The narrowest team that holds the row
+template <typename T, typename R, bool VEC>
+void forward_by_width(const ResNormParams& p, hipStream_t stream) {
+    if (p.D <= 128) launch_forward<T, R, VEC, 16, 1>(p, stream);
+    else if (p.D <= 512) launch_forward<T, R, VEC, 64, 1>(p, stream);
+    else if (p.D <= 1024) launch_forward<T, R, VEC, 64, 2>(p, stream);
+    else if (p.D <= 2048) launch_forward<T, R, VEC, 64, 4>(p, stream);
+    else if (p.D <= 4096) launch_forward<T, R, VEC, 256, 2>(p, stream);
+    else launch_forward<T, R, VEC, 256, 4>(p, stream);
+}
+
+template <bool VEC>
+void forward_by_type(const ResNormParams& p, int dtype, int stream_dtype, hipStream_t stream) {
+    if (dtype == ADCDIFF_BF16) {
+        if (stream_dtype == ADCDIFF_BF16) forward_by_width<bf16_t, bf16_t, VEC>(p, stream);
+        else forward_by_width<bf16_t, float, VEC>(p, stream);
+    } else {
+        if (stream_dtype == ADCDIFF_BF16) forward_by_width<float, bf16_t, VEC>(p, stream);
+        else forward_by_width<float, float, VEC>(p, stream);
+    }
+}
+
+// How a backward pass cuts its rows.  A chunk lies inside one gate row's rows; a workgroup runs over several chunks.
+struct Cut {
+    int tpr, teams, workgroups, chunk_rows, chunks_per_gate, chunks, group_rows, vectors;
+    bool gate_sum;      // the gate's gradient is a sum over rows
+};
+
+int team_width(int D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
+
+Cut cut_rows(int M, int D, int gate_rows, bool gate_grad, int vectors) {
+    Cut c{};
+    c.tpr = team_width(D);
+    c.teams = std::max(kThreads, c.tpr) / c.tpr;
+    c.vectors = vectors;
+    c.gate_sum = gate_grad && gate_rows > 0 && M / std::max(gate_rows, 1) != 1;
+    const int groups = c.gate_sum ? gate_rows : 1;
+    c.group_rows = M / groups;
+    if (M == 0) { c.chunks_per_gate = 1; c.chunk_rows = 1; return c; }
+    // about 1024 workgroups' worth of teams, and chunks of at least 8 rows
+    const int workers = 1024 * c.teams;
+    const int want = std::max(1, (workers + groups - 1) / groups);
+    c.chunk_rows = std::max(std::min(c.group_rows, 8), (c.group_rows + want - 1) / want);
+    c.chunks_per_gate = (c.group_rows + c.chunk_rows - 1) / c.chunk_rows;
+    c.chunks = groups * c.chunks_per_gate;
+    c.workgroups = std::min(1024, (c.chunks + c.teams - 1) / c.teams);
+    return c;
+}
+
+size_t workspace_floats(const Cut& c, int D) {
+    size_t n = (size_t)c.workgroups * c.vectors * D;
+    if (c.gate_sum && c.chunks_per_gate > 1) n += (size_t)c.chunks * D;
+    return n;
+}
+
+template <typename T, typename R, bool VEC>
+void backward_by_width(const ResNormGradParams& q, const Cut& c, hipStream_t stream) {
+    const dim3 grid(c.workgroups);
+    switch (c.tpr) {
+        case 16: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 16>), grid, dim3(kThreads), 0, stream, q); break;
+        case 64: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 64>), grid, dim3(kThreads), 0, stream, q); break;
+        case 128: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 128>), grid, dim3(kThreads), 0, stream, q); break;
+        case 256: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 256>), grid, dim3(kThreads), 0, stream, q); break;
+        case 512: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 512>), grid, dim3(512), 0, stream, q); break;
+        default: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 1024>), grid, dim3(1024), 0, stream, q); break;
+    }
+}
+
+template <bool VEC>
+void backward_by_type(const ResNormGradParams& q, const Cut& c, int dtype, int stream_dtype, hipStream_t stream) {
+    if (dtype == ADCDIFF_BF16) {
+        if (stream_dtype == ADCDIFF_BF16) backward_by_width<bf16_t, bf16_t, VEC>(q, c, stream);
+        else backward_by_width<bf16_t, float, VEC>(q, c, stream);
+    } else {
+        if (stream_dtype == ADCDIFF_BF16) backward_by_width<float, bf16_t, VEC>(q, c, stream);
+        else backward_by_width<float, float, VEC>(q, c, stream);
+    }
+}
+
+int vector_count(const adcdiff_residual_norm_grads& g) { return !!g.post_weight + !!g.post_bias + !!g.pre_weight + !!g.pre_bias; }
+
+}  // namespace
+}  // namespace adcdiff
+
+extern "C" int adcdiff_residual_norm(const adcdiff_residual_norm_args* a, adcdiff_stream_t stream_) {
+    using namespace adcdiff;
+    int rc = check_args("residual_norm", a);
+    if (rc != ADCDIFF_OK) return rc;
+    if (a->M == 0) return ADCDIFF_OK;
+    if ((a->pre_norm != 0) != (a->y != nullptr)) return fail(ADCDIFF_E_BADARG, "residual_norm: y goes with a pre norm and only with one");
+    if (!a->y && !a->x_new) return fail(ADCDIFF_E_BADARG, "residual_norm: no output");
+    if ((a->x_new && a->ldx_new < a->D) || (a->y && a->ldy < a->D)) return fail(ADCDIFF_E_BADARG, "residual_norm: a row pitch below %d columns", a->D);
+    if (a->stats && !aligned16(a->stats)) return fail(ADCDIFF_E_BADARG, "residual_norm: stats are not on a 16-byte boundary");
+    hipStream_t stream = as_stream(stream_);
+    const ResNormParams p = forward_params(*a);
+    const int st = type_size(a->dtype), sr = type_size(a->stream_dtype);
+    TimingScope timing(ADCDIFF_KIND_OTHER, a->M, a->D, 0, 0.0, (double)a->M * a->D * ((a->h ? st : 0) + (a->y ? st : 0) + sr + (a->x_new ? sr : 0)), stream);
+    if (vector_inputs(*a) && vector_rows(a->x_new, a->ldx_new, sr) && vector_rows(a->y, a->ldy, st)) forward_by_type<true>(p, a->dtype, a->stream_dtype, stream);
+    else forward_by_type<false>(p, a->dtype, a->stream_dtype, stream);
+    return check_launch("residual_norm");
+}
+
+extern "C" size_t adcdiff_residual_norm_backward_workspace_bytes(const adcdiff_residual_norm_args* a, const adcdiff_residual_norm_grads* g) {
+    using namespace adcdiff;
+    if (check_args("residual_norm_backward", a) != ADCDIFF_OK || !g) return 0;
+    return std::max<size_t>(16, workspace_floats(cut_rows(a->M, a->D, a->gate ? a->gate_rows : 0, g->gate != nullptr, vector_count(*g)), a->D) * 4);
+}
+
+extern "C" int adcdiff_residual_norm_backward(const adcdiff_residual_norm_args* a, const adcdiff_residual_norm_grads* g, void* workspace,
+                                              size_t workspace_bytes, adcdiff_stream_t stream_) {
+    using namespace adcdiff;
+    int rc = check_args("residual_norm_backward", a);
+    if (rc != ADCDIFF_OK) return rc;
+    if (!g) return fail(ADCDIFF_E_BADARG, "residual_norm_backward: null gradients");
+    if (a->M > 0 && !g->d_x_new && !g->d_y) return fail(ADCDIFF_E_BADARG, "residual_norm_backward: no incoming gradient");
+    if (g->d_y && !a->pre_norm) return fail(ADCDIFF_E_BADARG, "residual_norm_backward: d_y without a pre norm");
+    if (a->M > 0 && (a->post_norm || a->pre_norm) && (!a->stats || !aligned16(a->stats)))
+        return fail(ADCDIFF_E_BADARG, "residual_norm_backward: the statistics of the forward pass are missing or not on a 16-byte boundary");
+    const bool has_h = a->h || a->M == 0;   // the address of no rows may be null
+    if ((g->h && !has_h) || (g->gate && !a->gate) || ((g->post_weight || g->post_bias) && !(has_h && a->post_norm)) || ((g->pre_weight || g->pre_bias) && !a->pre_norm))
+        return fail(ADCDIFF_E_BADARG, "residual_norm_backward: a gradient of what the forward pass did not have");
+    if ((g->d_x_new && g->ld_d_x_new < a->D) || (g->d_y && g->ld_d_y < a->D) || (g->h && g->ld_h < a->D) || (g->x && g->ld_x < a->D) ||
+        (g->gate && a->gate_rows > 1 && g->ld_gate < a->D))
+        return fail(ADCDIFF_E_BADARG, "residual_norm_backward: a row pitch below %d columns", a->D);
+    const Cut c = cut_rows(a->M, a->D, a->gate ? a->gate_rows : 0, g->gate != nullptr, vector_count(*g));
+    const size_t need = std::max<size_t>(16, workspace_floats(c, a->D) * 4);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+        return fail(ADCDIFF_E_WORKSPACE, "residual_norm_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    hipStream_t stream = as_stream(stream_);
+    const int st = type_size(a->dtype), sr = type_size(a->stream_dtype), sg = type_size(a->gate_dtype);
+    ResNormGradParams q{};
+    q.f = forward_params(*a);
+    q.d_xn = g->d_x_new; q.d_y = g->d_y; q.d_h = g->h; q.d_x = g->x; q.d_gate = g->gate;
+    q.ld_dxn = g->ld_d_x_new; q.ld_dy = g->ld_d_y; q.ld_dh = g->ld_h; q.ld_dx = g->ld_x; q.ld_dg = g->ld_gate;
+    q.chunks = c.chunks; q.chunk_rows = c.chunk_rows; q.chunks_per_gate = c.chunks_per_gate; q.group_rows = c.group_rows;
+    q.vectors = c.vectors;
+    q.partial = static_cast<float*>(workspace);
+    q.gate_partial = q.partial + (size_t)c.workgroups * c.vectors * a->D;
+    ColumnSumParams s{};
+    int slot = 0;
+    auto place = [&](float* out) { if (!out) return -1; s.out[slot] = out; return slot++; };
+    q.slot_pre_w = place(g->pre_weight); q.slot_pre_b = place(g->pre_bias); q.slot_post_w = place(g->post_weight); q.slot_post_b = place(g->post_bias);
+    if (a->M > 0) {
+        TimingScope timing(ADCDIFF_KIND_OTHER, a->M, a->D, 0, 0.0, (double)a->M * a->D * ((a->h ? 2.0 : 0.0) * st + (g->d_y ? st : 0) + 2.0 * sr + (g->d_x_new ? sr : 0)), stream);
+        const bool vec = vector_inputs(*a) && vector_rows(g->d_x_new, g->ld_d_x_new, sr) && vector_rows(g->d_y, g->ld_d_y, st) &&
+                         vector_rows(g->h, g->ld_h, st) && vector_rows(g->x, g->ld_x, sr) && vector_rows(g->gate, a->gate_rows > 1 ? g->ld_gate : 0, sg);
+        if (vec) backward_by_type<true>(q, c, a->dtype, a->stream_dtype, stream);
+        else backward_by_type<false>(q, c, a->dtype, a->stream_dtype, stream);
+        rc = check_launch("residual_norm_backward");
+        if (rc != ADCDIFF_OK) return rc;
+    }
+    const int gate_segments = g->gate && (a->M == 0 || (c.gate_sum && c.chunks_per_gate > 1)) ? a->gate_rows : 0;
+    const int segments = c.vectors + gate_segments;
+    s.partial = q.partial; s.gate_partial = q.gate_partial; s.d_gate = g->gate; s.ld_dg = g->ld_gate;
+    s.D = a->D; s.vectors = c.vectors; s.segments = segments; s.workgroups = a->M > 0 ? c.workgroups : 0;
+    s.chunks_per_gate = a->M > 0 ? c.chunks_per_gate : 0; s.gate_bf16 = a->gate_dtype == ADCDIFF_BF16;
+    if (segments == 0) return ADCDIFF_OK;
+    TimingScope timing(ADCDIFF_KIND_OTHER, segments, a->D, 0, 0.0, 4.0 * workspace_floats(c, a->D), stream);
+    hipLaunchKernelGGL(column_sum_kernel, dim3((a->D + 31) / 32, std::min(segments, 65535)), dim3(1024), 0, stream, s);
+    return check_launch("residual_norm_backward: column sums");
+}

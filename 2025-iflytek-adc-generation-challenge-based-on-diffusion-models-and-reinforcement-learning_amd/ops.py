@@ -219,6 +219,289 @@ def _raw_latent_summary(x):
     return out
 
 
+# ---- gated residual norms, gradient norm, 8-bit integer layer --------------------------------------------------------
+_CODES = {torch.float32: F32, torch.bfloat16: BF16}
+_TYPES = {F32: torch.float32, BF16: torch.bfloat16}
+_NORMS = {None: 0, "rms": 1, "layer": 2}
+
+
+def _device_of(*tensors):
+    """The index of the one GPU that holds all the tensors."""
+    dev = -2
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _need_gpu(t)
+        i = t.get_device()
+        if dev not in (-2, i):
+            raise ValueError("tensors on different devices: cuda:%d and cuda:%d" % (dev, i))
+        dev = i
+    return dev
+
+
+class _on:
+    """Makes the tensors' device the current one for a call where it is not; the stream is that device's current stream."""
+    __slots__ = ("dev", "before")
+
+    def __init__(self, dev):
+        self.dev = dev
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.dev:
+            torch.cuda.set_device(self.dev)
+        return torch._C._cuda_getCurrentRawStream(self.dev)
+
+    def __exit__(self, *exc):
+        if self.before != self.dev:
+            torch.cuda.set_device(self.before)
+        return False
+
+
+def _code(t, what):
+    code = _CODES.get(t.dtype)
+    if code is None:
+        raise ValueError("%s must be float32 or bfloat16, got %s" % (what, t.dtype))
+    return code
+
+
+def _pitch(t, what):
+    """Row pitch in elements of a 2-D tensor whose rows are contiguous."""
+    if t.dim() != 2:
+        raise ValueError("%s must be two-dimensional, got shape %s" % (what, tuple(t.shape)))
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError("the rows of %s must be contiguous, got strides %s" % (what, t.stride()))
+    if rows <= 1:
+        return cols
+    if t.stride(0) < cols:
+        raise ValueError("the rows of %s overlap: strides %s" % (what, t.stride()))
+    return t.stride(0)
+
+
+def _vector(t, n, what):
+    """Address of an optional contiguous float32 vector."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous float32 vector of %d elements, got %s %s" % (what, n, t.dtype, tuple(t.shape)))
+    return t.data_ptr()
+
+
+def _rows_or_copy(t):
+    """t, or a copy of it, with contiguous rows that do not overlap (incoming gradients may be expanded)."""
+    if t is None or ((t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])):
+        return t
+    return t.contiguous()
+
+
+def _residual_norm_args(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps):
+    a = _lib.ResidualNormArgs()
+    a.x, a.ldx, a.stream_dtype = x.data_ptr(), _pitch(x, "x"), _code(x, "x")
+    M, D = x.shape
+    a.M, a.D = M, D
+    a.dtype = a.stream_dtype
+    if h is not None:
+        if h.shape != x.shape:
+            raise ValueError("h %s and x %s differ in shape" % (tuple(h.shape), tuple(x.shape)))
+        a.h, a.ldh, a.dtype = h.data_ptr(), _pitch(h, "h"), _code(h, "h")
+    elif gate is not None or post_norm or residual_scale != 1.0:
+        raise ValueError("a gate, a post norm or a residual scale needs h")
+    if gate is not None:
+        if gate.dim() != 2 or gate.shape[1] != D or (M > 0 and (gate.shape[0] < 1 or M % gate.shape[0] != 0)):
+            raise ValueError("gate must be [G, %d] with G dividing %d rows, got %s" % (D, M, tuple(gate.shape)))
+        a.gate, a.gate_rows, a.gate_dtype = gate.data_ptr(), gate.shape[0], _code(gate, "gate")
+        if gate.shape[0] > 1 and gate.stride(0) == 0 and (D <= 1 or gate.stride(1) == 1):
+            a.ldg = 0                    # one row expanded over the groups
+        else:
+            a.ldg = _pitch(gate, "gate")
+    if not post_norm and (post_weight is not None or post_bias is not None):
+        raise ValueError("post_weight / post_bias without a post norm")
+    if not pre_norm and (pre_weight is not None or pre_bias is not None):
+        raise ValueError("pre_weight / pre_bias without a pre norm")
+    a.post_norm, a.pre_norm = post_norm, pre_norm
+    a.post_weight, a.post_bias = _vector(post_weight, D, "post_weight"), _vector(post_bias, D, "post_bias")
+    a.pre_weight, a.pre_bias = _vector(pre_weight, D, "pre_weight"), _vector(pre_bias, D, "pre_bias")
+    a.residual_scale, a.eps = residual_scale, eps
+    return a
+
+
+def _raw_residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x, with_stats):
+    """adcdiff_residual_norm: [x_new where with_x] + [y where pre_norm] + [stats [M, 4] where with_stats]."""
+    dev = _device_of(h, x, gate, post_weight, post_bias, pre_weight, pre_bias)
+    a = _residual_norm_args(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps)
+    outs = []
+    if with_x:
+        o = torch.empty((a.M, a.D), device=x.device, dtype=x.dtype)
+        a.x_new, a.ldx_new = o.data_ptr(), a.D
+        outs.append(o)
+    if pre_norm:
+        o = torch.empty((a.M, a.D), device=x.device, dtype=_TYPES[a.dtype])
+        a.y, a.ldy = o.data_ptr(), a.D
+        outs.append(o)
+    if with_stats:
+        o = torch.empty((a.M, 4), device=x.device, dtype=torch.float32)
+        a.stats = o.data_ptr()
+        outs.append(o)
+    with _on(dev) as stream:
+        check(_lib.load().adcdiff_residual_norm(C.byref(a), stream))
+    return outs
+
+
+def _raw_residual_norm_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y, post_norm, pre_norm, residual_scale,
+                                eps, need):
+    """adcdiff_residual_norm_backward: the gradients of (h, x, gate, post_weight, post_bias, pre_weight, pre_bias) that `need` asks for."""
+    dev = _device_of(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y)
+    a = _residual_norm_args(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps)
+    given = (h, x, gate, post_weight, post_bias, pre_weight, pre_bias)
+    if len(need) != 7 or any(n and t is None for n, t in zip(need, given)):
+        raise ValueError("need asks for the gradient of an input that is not there")
+    if post_norm or pre_norm:
+        if stats is None or stats.dtype != torch.float32 or stats.shape != (a.M, 4) or not stats.is_contiguous():
+            raise ValueError("stats must be the contiguous float32 [%d, 4] tensor of the forward pass" % a.M)
+        a.stats = stats.data_ptr()
+    g = _lib.ResidualNormGrads()
+    for t, like, name in ((d_x_new, x.dtype, "d_x_new"), (d_y, _TYPES[a.dtype], "d_y")):
+        if t is not None and (t.shape != x.shape or t.dtype != like):
+            raise ValueError("%s must be %s %s, got %s %s" % (name, like, tuple(x.shape), t.dtype, tuple(t.shape)))
+    d_x_new, d_y = _rows_or_copy(d_x_new), _rows_or_copy(d_y)
+    if d_x_new is not None:
+        g.d_x_new, g.ld_d_x_new = d_x_new.data_ptr(), _pitch(d_x_new, "d_x_new")
+    if d_y is not None:
+        g.d_y, g.ld_d_y = d_y.data_ptr(), _pitch(d_y, "d_y")
+    outs = []
+    for i, name in enumerate(("h", "x", "gate")):
+        if need[i]:
+            o = torch.empty(given[i].shape, device=x.device, dtype=given[i].dtype)
+            setattr(g, name, o.data_ptr())
+            setattr(g, "ld_" + name, a.D)
+            outs.append(o)
+    for i, name in enumerate(("post_weight", "post_bias", "pre_weight", "pre_bias")):
+        if need[3 + i]:
+            o = torch.empty((a.D,), device=x.device, dtype=torch.float32)
+            setattr(g, name, o.data_ptr())
+            outs.append(o)
+    lib = _lib.load()
+    with _on(dev) as stream:
+        ws = torch.empty(lib.adcdiff_residual_norm_backward_workspace_bytes(C.byref(a), C.byref(g)), device=x.device, dtype=torch.uint8)
+        check(lib.adcdiff_residual_norm_backward(C.byref(a), C.byref(g), ws.data_ptr(), ws.numel(), stream))
+    return outs
+
+
+def _dense(t):
+    """Whether the elements of t fill one block of memory, in any order."""
+    if t.layout != torch.strided:
+        return False
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _grad_table(grads, out):
+    """(device, host array of adcdiff_grad_tensor)"""
+    dev, rows = -2, []
+    for i, g in enumerate(grads):
+        o = g if out is None else out[i]
+        if not g.is_cuda or not o.is_cuda:
+            _need_gpu(g, o)
+        if g.get_device() != dev:
+            if dev != -2:
+                raise ValueError("gradients on different devices")
+            dev = g.get_device()
+        if not g.is_contiguous() and not _dense(g):
+            raise ValueError("gradient %d has gaps or overlaps in memory: shape %s, strides %s" % (i, tuple(g.shape), g.stride()))
+        code = _code(g, "gradients")
+        if o is not g:
+            if o.get_device() != dev or o.shape != g.shape or o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
+                raise ValueError("output %d must be like its gradient in device, shape and strides" % i)
+            rows += (g.data_ptr(), o.data_ptr(), g.numel(), code | _code(o, "outputs") << 32)
+        else:
+            p = g.data_ptr()
+            rows += (p, p, g.numel(), code | code << 32)
+    return dev, (C.c_longlong * max(len(rows), 1))(*rows)
+
+
+def _raw_grad_norm(grads, norm_type, max_norm=None, out=None):
+    """adcdiff_grad_norm, or adcdiff_clip_grad_norm with a max_norm: the norm, a float32 scalar on the gradients' device."""
+    dev, table = _grad_table(grads, out)
+    lib = _lib.load()
+    n = len(grads)
+    need = lib.adcdiff_grad_norm_workspace_bytes(table, n)
+    device = torch.device("cuda", dev)
+    norm = torch.empty((), device=device, dtype=torch.float32)
+    ws = torch.empty(need, device=device, dtype=torch.uint8)
+    with _on(dev) as stream:
+        if max_norm is None:
+            check(lib.adcdiff_grad_norm(table, n, norm_type, norm.data_ptr(), ws.data_ptr(), need, stream))
+        else:
+            check(lib.adcdiff_clip_grad_norm(table, n, norm_type, max_norm, norm.data_ptr(), ws.data_ptr(), need, stream))
+            # the library wrote the tensors behind torch's back
+            torch.autograd.graph.increment_version(grads if out is None else out)
+    return norm
+
+
+def _raw_quantize_rows(x):
+    dev = _device_of(x)
+    code, ldx = _code(x, "x"), _pitch(x, "x")
+    M, K = x.shape
+    if K < 1:
+        raise ValueError("rows of no columns have no scale")
+    pitch = (K + 15) // 16 * 16
+    q = torch.empty((M, pitch), device=x.device, dtype=torch.int8)
+    scale = torch.empty((M,), device=x.device, dtype=torch.float32)
+    with _on(dev) as stream:
+        check(_lib.load().adcdiff_quantize_rows(x.data_ptr(), ldx, code, M, K, q.data_ptr(), pitch, scale.data_ptr(), stream))
+    return (q if pitch == K else q[:, :K]), scale
+
+
+def _i8_rows(t, what, stream):
+    """(tensor, pitch) of 8-bit codes with rows on 16-byte boundaries: t itself, or a copy with that layout."""
+    ld = _pitch(t, what)
+    M, K = t.shape
+    pitch = (K + 15) // 16 * 16
+    if t.data_ptr() % 16 == 0 and (ld % 16 == 0 or M <= 1):
+        return t, (ld if M > 1 else pitch)
+    o = torch.empty((M, pitch), device=t.device, dtype=torch.int8)
+    check(_lib.load().adcdiff_pitch_rows_i8(t.data_ptr(), ld, M, K, o.data_ptr(), pitch, stream))
+    return o, pitch
+
+
+def _raw_gemm_int8(a, a_scale, w, w_scale, bias, residual, act, out_dtype):
+    dev = _device_of(a, a_scale, w, w_scale, bias, residual)
+    if a.dtype != torch.int8 or w.dtype != torch.int8:
+        raise ValueError("a and w must be int8, got %s and %s" % (a.dtype, w.dtype))
+    if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
+        raise ValueError("a [M, K] and w [N, K] do not fit: %s, %s" % (tuple(a.shape), tuple(w.shape)))
+    M, K = a.shape
+    N = w.shape[0]
+    if K < 1 or N < 1:
+        raise ValueError("no columns: a %s, w %s" % (tuple(a.shape), tuple(w.shape)))
+    out = torch.empty((M, N), device=a.device, dtype=_TYPES[out_dtype])
+    p = _lib.GemmI8Args()
+    p.M, p.N, p.K, p.act, p.out_dtype = M, N, K, act, out_dtype
+    p.a_scale, p.w_scale, p.bias = _vector(a_scale, M, "a_scale"), _vector(w_scale, N, "w_scale"), _vector(bias, N, "bias")
+    if residual is not None:
+        if residual.shape != (M, N) or residual.dtype != out.dtype:
+            raise ValueError("residual must be %s %s, got %s %s" % (out.dtype, (M, N), residual.dtype, tuple(residual.shape)))
+        p.residual, p.ldr = residual.data_ptr(), _pitch(residual, "residual")
+    p.out, p.ldo = out.data_ptr(), N
+    lib = _lib.load()
+    with _on(dev) as stream:
+        a, p.lda = _i8_rows(a, "a", stream)
+        w, p.ldw = _i8_rows(w, "w", stream)
+        p.a, p.w = a.data_ptr(), w.data_ptr()
+        need = lib.adcdiff_gemm_i8_workspace_bytes(M, N, K)
+        ws = torch.empty(need, device=out.device, dtype=torch.uint8) if need else None
+        check(lib.adcdiff_gemm_i8(C.byref(p), ws.data_ptr() if need else None, need, stream))
+    return out
+
+
 class timing:
     """Context manager over adcdiff_timing_begin/_end: ``with ops.timing(4096) as t: ...; t.records``."""
 
@@ -292,3 +575,149 @@ def latent_summary(x):
     if x.dtype != torch.float32 or x.dim() != 2 or x.stride(1) != 1:
         raise ValueError("latent_summary expects a [B, D] float32 tensor with contiguous rows")
     return torch.ops.adcdiff.latent_summary(x)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """Autograd link of residual_norm / row_norm over torch.ops.adcdiff.residual_norm and residual_norm_backward."""
+
+    @staticmethod
+    def forward(ctx, h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x):
+        outs = torch.ops.adcdiff.residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps,
+                                               with_x, True)
+        ctx.save_for_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, outs[-1])
+        ctx.args = (post_norm, pre_norm, residual_scale, eps)
+        ctx.set_materialize_grads(False)
+        return (outs[0] if with_x else None), (outs[-2] if pre_norm else None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_x_new, d_y):
+        need = list(ctx.needs_input_grad[:7])
+        if (d_x_new is None and d_y is None) or not any(need):
+            return (None,) * 12
+        outs = iter(torch.ops.adcdiff.residual_norm_backward(*ctx.saved_tensors, d_x_new, d_y, *ctx.args, need))
+        return tuple(next(outs) if n else None for n in need) + (None,) * 5
+
+
+def _norm_code(norm, what):
+    if norm not in _NORMS:
+        raise ValueError("%s must be None, 'rms' or 'layer', got %r" % (what, norm))
+    return _NORMS[norm]
+
+
+def _residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x):
+    from . import torch_ops  # noqa: F401
+    _need_gpu(h, x, gate, post_weight, post_bias, pre_weight, pre_bias)
+    args = (h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, float(residual_scale), float(eps), with_x)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:7]):
+        return _ResidualNorm.apply(*args)
+    outs = torch.ops.adcdiff.residual_norm(*args, False)
+    return (outs[0] if with_x else None), (outs[-1] if pre_norm else None)
+
+
+def residual_norm(h, x, gate=None, post_norm=None, post_weight=None, post_bias=None, pre_norm=None, pre_weight=None, pre_bias=None,
+                  residual_scale=1.0, eps=1e-6):
+    """The seam between two residual blocks in one pass: (x_new, y) with
+
+        x_new = residual_scale * x + gate * N_post(h),    y = N_pre(x_new)    (y is None without a pre norm)
+
+    h [M, D]: what the block computed; x [M, D]: the residual stream, which may have another type (float32 under bfloat16 blocks).
+    post_norm / pre_norm: None, "rms" (v / sqrt(mean(v^2) + eps)) or "layer" (of v - mean(v)), each with an optional float32 weight
+    and bias [D].  gate: [D] or [G, D] with G dividing M: row r reads gate row r // (M / G) (one gate for all rows, one for each
+    group of consecutive rows, one for each row).  Types float32 and bfloat16; x_new has x's type, y has h's; float32 inside, one
+    rounding per output.  Any row pitch and any D from 1 to 8192.
+
+    Differentiable once in every tensor; gradients of a shared gate and of the weights are summed in a fixed order.  Works under
+    graph capture; where a backward pass is captured, no other graph of the same leaves may be alive on another stream (autograd's
+    accumulation belongs to the stream of a leaf's first use), or torch.ops.adcdiff.residual_norm_backward is called directly."""
+    if gate is not None and gate.dim() == 1:
+        gate = gate.unsqueeze(0)
+    return _residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, _norm_code(post_norm, "post_norm"),
+                          _norm_code(pre_norm, "pre_norm"), residual_scale, eps, True)
+
+
+def row_norm(x, norm="rms", weight=None, bias=None, eps=1e-6):
+    """The norm in front of a first block: "rms" or "layer" of the rows of x [M, D], in x's type.  Differentiable like residual_norm."""
+    if norm is None:
+        raise ValueError("norm must be 'rms' or 'layer'")
+    return _residual_norm(None, x, None, None, None, weight, bias, 0, _norm_code(norm, "norm"), 1.0, eps, False)[1]
+
+
+def _norm_type(norm_type):
+    if norm_type in (2, 2.0):
+        return 2
+    if norm_type in (float("inf"), "inf"):
+        return 0
+    raise ValueError("norm_type must be 2 or inf, got %r" % (norm_type,))
+
+
+def _as_list(tensors):
+    tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
+    for t in tensors:
+        if not torch.is_tensor(t):
+            raise TypeError("gradients must be tensors, got %s" % type(t).__name__)
+    return tensors
+
+
+def grad_norm(grads, norm_type=2.0):
+    """The norm over all elements of all gradient tensors (float32 and bfloat16, any shapes without gaps in memory): a float32 scalar on
+    their device.  norm_type 2 (squares summed in float64, so nothing overflows on the way) or inf (largest magnitude).  No
+    synchronisation, the same bits every run; NaN if any element is.  An empty list has norm 0, on the CPU."""
+    from . import torch_ops  # noqa: F401
+    grads, code = _as_list(grads), _norm_type(norm_type)
+    _need_gpu(*grads)
+    return torch.ops.adcdiff.grad_norm(grads, code) if grads else torch.zeros(())
+
+
+def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, out=None):
+    """Scales the gradient tensors by min(1, max_norm / (norm + 1e-6)) and returns their norm before that (see grad_norm).
+
+    In place; with `out`, a list of tensors of the same shapes (float32 or bfloat16, such as views of an optimizer's float32 arena),
+    the scaled gradients go there and `grads` stay.  Tensors that are written must not overlap one another or another gradient.
+    A norm that is not finite is handled as torch.nn.utils.clip_grad_norm_ does: NaN gradients from a NaN norm, zeros (and NaN for the
+    infinite elements) from an infinite one; error_if_nonfinite raises before anything is written, at the price of a synchronisation."""
+    from . import torch_ops  # noqa: F401
+    grads, code, max_norm = _as_list(grads), _norm_type(norm_type), float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError("max_norm must not be negative or NaN, got %r" % max_norm)
+    if out is not None:
+        out = _as_list(out)
+        if len(out) != len(grads):
+            raise ValueError("%d outputs for %d gradients" % (len(out), len(grads)))
+    if not grads:
+        return torch.zeros(())
+    _need_gpu(*grads)
+    if error_if_nonfinite and not bool(torch.isfinite(grad_norm(grads, norm_type))):
+        raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
+    if out is None:
+        return torch.ops.adcdiff.clip_grad_norm_(grads, max_norm, code)
+    return torch.ops.adcdiff.clip_grad_norm_out(grads, max_norm, code, out)
+
+
+def quantize_rows(x):
+    """(codes int8 [M, K], scale float32 [M]) of the rows of x [M, K] (float32 or bfloat16): scale = max|row| / 127, codes =
+    row / scale rounded half to even, exactly.  For activations (a scale per token) and weights [N, K] (a scale per output channel)
+    alike.  The codes' rows start on 16-byte boundaries, as gemm_int8 reads them.  A row of zeros has scale 0; a row with a NaN or an
+    infinity has scale NaN, so that every product with it is NaN."""
+    from . import torch_ops  # noqa: F401
+    _need_gpu(x)
+    return torch.ops.adcdiff.quantize_rows(x)
+
+
+def gemm_int8(a, a_scale, w, w_scale, bias=None, residual=None, act=0, out_dtype="bf16"):
+    """act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n] + residual[m, n]) for int8 a [M, K] and w [N, K], float32 scales and
+    bias, residual [M, N] in out_dtype; act 0 none, 1 SiLU.  The sum is exact (K up to 131071).  Codes whose rows do not start on
+    16-byte boundaries are copied to such rows on every call: keep weights as quantize_rows returns them."""
+    from . import torch_ops  # noqa: F401
+    code = dtype_code(out_dtype)
+    _need_gpu(a, a_scale, w, w_scale, bias, residual)
+    return torch.ops.adcdiff.gemm_int8(a, a_scale, w, w_scale, bias, residual, int(act), code)
+
+
+def linear_int8(x, w, w_scale, bias=None, residual=None, act=0, out_dtype="bf16"):
+    """The 8-bit integer form of a linear layer: the rows of x [M, K] (float32 or bfloat16) are quantised as by quantize_rows and
+    multiplied with the codes w [N, K] (see gemm_int8).  For inference: it has no gradient."""
+    from . import torch_ops  # noqa: F401
+    code = dtype_code(out_dtype)
+    _need_gpu(x, w, w_scale, bias, residual)
+    return torch.ops.adcdiff.linear_int8(x, w, w_scale, bias, residual, int(act), code)

@@ -86,3 +86,12 @@ class FusedClipAdamW:
             torch.autograd.graph.increment_version(params)
             torch.autograd.graph.increment_version([s["exp_avg"] for s in states] + [s["exp_avg_sq"] for s in states])
         return self.grad_norm
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ (diffusion_model.py:434-436) on its own, for any optimizer and any number of parameter groups under
+    one norm: scales the .grad of the parameters (float32 or bfloat16) in place and returns their norm (ops.clip_grad_norm_)."""
+    from . import ops
+    parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    return ops.clip_grad_norm_([p.grad for p in parameters if p.grad is not None], max_norm, norm_type, error_if_nonfinite)

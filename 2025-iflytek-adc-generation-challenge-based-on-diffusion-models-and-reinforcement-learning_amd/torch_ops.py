@@ -7,6 +7,8 @@ take and return tensors, ints and floats only:
 
 * single kernels: ``gemm``, ``groupnorm_silu``, ``philox_normal``, ``ddpm_step``, ``ddim_step``, ``q_sample``,
   ``latent_summary``;
+* the operators around a residual block: ``residual_norm``, ``residual_norm_backward``, ``grad_norm``, ``clip_grad_norm_``,
+  ``clip_grad_norm_out``, ``quantize_rows``, ``gemm_int8``, ``linear_int8``;
 * the denoiser through a native plan handle (an int: the ``adcdiff_unet*`` of ``_Engine``): ``condition_embed``,
   ``unet_forward``, ``ddpm_sample_loop``, ``ddim_sample_loop``, ``unet_train_forward``, ``mse_loss_grad``,
   ``unet_backward``.  ``ws`` is the engine's workspace (a uint8 tensor the operator scribbles in: declared as mutated).
@@ -244,6 +246,67 @@ def unet_backward(handle: int, d_eps: Tensor, grad_pointers: Tensor, grad_arena:
     p, n = _ws(ws)
     check(_lib.load().adcdiff_unet_backward(_h(handle), ops._ptr(d_eps), d_eps.stride(0),
                                             C.cast(C.c_void_p(grad_pointers.data_ptr()), C.POINTER(_lib.UnetGrads)), p, n, ops._stream()))
+
+
+# ------------------------------------------------- gated residual norms, gradient norm, 8-bit integer layer
+# Defined on the dispatcher directly: torch.library.custom_op wraps every call in checks that take 15 us on the host, which is
+# several times what these kernels take at small sizes.
+_fragment = torch.library.Library("adcdiff", "FRAGMENT")
+
+
+def _define(schema, impl, fake):
+    name = schema[:schema.index("(")]
+    _fragment.define(schema, tags=(torch.Tag.pt2_compliant_tag,))
+    _fragment.impl(name, impl, "CUDA")
+    torch.library.register_fake("adcdiff::" + name, fake, lib=_fragment)
+    getattr(torch.ops.adcdiff, name)     # listed by names()
+
+
+def _fake_residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x, with_stats):
+    outs = [x.new_empty(x.shape)] if with_x else []
+    if pre_norm:
+        outs.append((x if h is None else h).new_empty(x.shape))
+    if with_stats:
+        outs.append(x.new_empty((x.shape[0], 4), dtype=torch.float32))
+    return outs
+
+
+def _fake_residual_norm_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y, post_norm, pre_norm,
+                                 residual_scale, eps, need):
+    given = (h, x, gate, post_weight, post_bias, pre_weight, pre_bias)
+    return [t.new_empty(t.shape) for t, n in zip(given, need) if n]
+
+
+def _fake_quantize_rows(x):
+    M, K = x.shape
+    return x.new_empty((M, (K + 15) // 16 * 16), dtype=torch.int8)[:, :K], x.new_empty((M,), dtype=torch.float32)
+
+
+_NORM_INPUTS = "Tensor? h, Tensor x, Tensor? gate, Tensor? post_weight, Tensor? post_bias, Tensor? pre_weight, Tensor? pre_bias"
+_define("residual_norm(" + _NORM_INPUTS + ", int post_norm, int pre_norm, float residual_scale, float eps, bool with_x, bool with_stats) -> Tensor[]",
+        ops._raw_residual_norm, _fake_residual_norm)
+_define("residual_norm_backward(" + _NORM_INPUTS + ", Tensor? stats, Tensor? d_x_new, Tensor? d_y, int post_norm, int pre_norm, "
+        "float residual_scale, float eps, bool[] need) -> Tensor[]", ops._raw_residual_norm_backward, _fake_residual_norm_backward)
+_define("grad_norm(Tensor[] grads, int norm_type) -> Tensor", ops._raw_grad_norm,
+        lambda grads, norm_type: grads[0].new_empty((), dtype=torch.float32))
+_define("clip_grad_norm_(Tensor(a!)[] grads, float max_norm, int norm_type) -> Tensor",
+        lambda grads, max_norm, norm_type: ops._raw_grad_norm(grads, norm_type, max_norm),
+        lambda grads, max_norm, norm_type: grads[0].new_empty((), dtype=torch.float32))
+_define("clip_grad_norm_out(Tensor[] grads, float max_norm, int norm_type, Tensor(a!)[] out) -> Tensor",
+        lambda grads, max_norm, norm_type, out: ops._raw_grad_norm(grads, norm_type, max_norm, out),
+        lambda grads, max_norm, norm_type, out: grads[0].new_empty((), dtype=torch.float32))
+_define("quantize_rows(Tensor x) -> (Tensor, Tensor)", ops._raw_quantize_rows, _fake_quantize_rows)
+_define("gemm_int8(Tensor a, Tensor a_scale, Tensor w, Tensor w_scale, Tensor? bias, Tensor? residual, int act, int out_dtype) -> Tensor",
+        ops._raw_gemm_int8, lambda a, a_scale, w, w_scale, bias, residual, act, out_dtype: a.new_empty((a.shape[0], w.shape[0]), dtype=_td(out_dtype)))
+
+
+def _linear_int8(x, w, w_scale, bias, residual, act, out_dtype):
+    a, a_scale = ops._raw_quantize_rows(x)
+    return ops._raw_gemm_int8(a, a_scale, w, w_scale, bias, residual, act, out_dtype)
+
+
+_define("linear_int8(Tensor x, Tensor w, Tensor w_scale, Tensor? bias, Tensor? residual, int act, int out_dtype) -> Tensor", _linear_int8,
+        lambda x, w, w_scale, bias, residual, act, out_dtype: x.new_empty((x.shape[0], w.shape[0]), dtype=_td(out_dtype)))
 
 
 def names():

@@ -343,6 +343,119 @@ int adcdiff_clip_adamw_step(const adcdiff_opt_tensor* tensors, int n_tensors, lo
 int adcdiff_clip_adamw_step_noalloc(const adcdiff_opt_tensor* tensors, int n_tensors, long long total_chunks,
                                     const adcdiff_adamw_args* args, float* grad_norm, adcdiff_stream_t stream);
 
+/* ------------------------------------------------------------------ gated residual norms -- */
+
+/* The norms before and after a residual block, fused with the block's gate and the residual scale (the seam between two blocks of a
+ * conditioned denoiser; no counterpart in the reference, whose blocks add h + residual bare, diffusion_model.py:907):
+ *   x_new = residual_scale * x + gate . N_post(h),   y = N_pre(x_new),   N(v) = (v - [mean]) / sqrt(mean((v - [mean])^2) + eps) . weight + bias
+ * norm kinds: 0 none (N(v) = v), 1 rms (no [mean]), 2 layer.  Arithmetic in float32, one rounding per output; y is formed from the
+ * unrounded x_new.
+ *   h, y           [M, ld >= D] in dtype;  h NULL: x_new = x, only y = N_pre(x) is formed (no gate, no post norm, residual_scale 1)
+ *   x, x_new       [M, ld >= D] in stream_dtype; x_new NULL: not written.  x_new may alias x, and y may alias h
+ *   gate           [gate_rows, ldg] in gate_dtype, or NULL; gate_rows divides M and row r reads gate row r / (M / gate_rows); ldg = 0
+ *                  repeats one row
+ *   weights, biases [D] float32, each optional
+ *   stats          [M, 4] float32 on a 16-byte boundary, or NULL: the row statistics that the backward pass reads
+ * D <= 8192, any D and any pitch; rows on 16-byte boundaries with D % 8 == 0 take the vector path. */
+enum { ADCDIFF_NORM_NONE = 0, ADCDIFF_NORM_RMS = 1, ADCDIFF_NORM_LAYER = 2 };
+typedef struct adcdiff_residual_norm_args {
+    int M, D;
+    int dtype, stream_dtype, gate_dtype;   /* ADCDIFF_F32 / ADCDIFF_BF16 */
+    int post_norm, pre_norm;
+    int gate_rows;
+    const void* h;
+    long long ldh;
+    const void* x;
+    long long ldx;
+    const void* gate;
+    long long ldg;
+    const float *post_weight, *post_bias, *pre_weight, *pre_bias;
+    float residual_scale, eps;
+    void* x_new;
+    long long ldx_new;
+    void* y;
+    long long ldy;
+    float* stats;
+} adcdiff_residual_norm_args;
+int adcdiff_residual_norm(const adcdiff_residual_norm_args* args, adcdiff_stream_t stream);
+
+/* Its gradients, from the forward pass's inputs and stats (x_new and y of the arguments are not read): d_x_new in stream_dtype and d_y in
+ * dtype are the incoming ones (either may be NULL = zero), the others are written where not NULL: h, x, gate in their input's type (gate
+ * [gate_rows, ld_gate], summed over the rows that share a gate row), weights and biases [D] float32.  Column sums are added in a
+ * fixed order; nothing is accumulated into what the outputs held.  No output may alias an input. */
+typedef struct adcdiff_residual_norm_grads {
+    const void* d_x_new;
+    long long ld_d_x_new;
+    const void* d_y;
+    long long ld_d_y;
+    void* h;
+    long long ld_h;
+    void* x;
+    long long ld_x;
+    void* gate;
+    long long ld_gate;
+    float *post_weight, *post_bias, *pre_weight, *pre_bias;
+} adcdiff_residual_norm_grads;
+size_t adcdiff_residual_norm_backward_workspace_bytes(const adcdiff_residual_norm_args* args, const adcdiff_residual_norm_grads* grads);
+int adcdiff_residual_norm_backward(const adcdiff_residual_norm_args* args, const adcdiff_residual_norm_grads* grads, void* workspace,
+                                   size_t workspace_bytes, adcdiff_stream_t stream);
+
+/* ------------------------------------------------------------------ gradient norm --------- */
+
+/* The global norm over many gradient tensors and the clipping by it (torch.nn.utils.clip_grad_norm_, diffusion_model.py:434-436, on its
+ * own: any optimizer, several parameter groups under one norm, bf16 gradients, clipped copies):
+ *   norm_type 2: sqrt(sum g^2);  norm_type 0: max |g|           (over every element of every tensor; NaN if any is NaN)
+ *   factor = min(1, max_norm / (norm + 1e-6));  out = g * factor, in float32, rounded once
+ * Squares are summed in float64 in a fixed order: no overflow or underflow for any float32 gradient, the same bits every run.
+ * `tensors` is a HOST array (read before the call returns); numel elements at grad are contiguous, in dtype.  out / out_dtype (clip only):
+ * where the clipped gradient goes; out == grad with the same dtype clips in place, and then a factor of exactly 1 writes nothing.
+ * Outputs must not overlap each other or another tensor's gradient (rejected); gradients that are only read may.
+ * norm: device float32 scalar.  No host synchronisation; workspace of adcdiff_grad_norm_workspace_bytes. */
+typedef struct adcdiff_grad_tensor {
+    const void* grad;
+    void* out;
+    long long numel;
+    int dtype, out_dtype;
+} adcdiff_grad_tensor;
+size_t adcdiff_grad_norm_workspace_bytes(const adcdiff_grad_tensor* tensors, int n_tensors);
+int adcdiff_grad_norm(const adcdiff_grad_tensor* tensors, int n_tensors, int norm_type, float* norm, void* workspace, size_t workspace_bytes,
+                      adcdiff_stream_t stream);
+int adcdiff_clip_grad_norm(const adcdiff_grad_tensor* tensors, int n_tensors, int norm_type, double max_norm, float* norm, void* workspace,
+                           size_t workspace_bytes, adcdiff_stream_t stream);
+
+/* ------------------------------------------------------------------ 8-bit integer layer --- */
+
+/* Codes of the rows of x [M, K] (dtype): scale[r] = max_k |x[r, k]| / 127 and q[r, k] = x[r, k] * 127 / max|x[r]| rounded half to even,
+ * exactly (no second rounding near a tie).  A row of zeros has scale 0 and codes 0; a row with a NaN or an infinity has scale NaN and codes
+ * 0, so that what it stands for, and every product with it, is NaN.  q has a pitch of ldq >= K bytes; columns K .. min(ldq, K rounded up to
+ * 16) - 1 are written as 0.  Serves activations (a scale for each token) and weights [N, K] (a scale for each channel) alike. */
+int adcdiff_quantize_rows(const void* x, long long ldx, int dtype, int M, int K, int8_t* q, long long ldq, float* scale, adcdiff_stream_t stream);
+
+/* out[m, n] = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n] + residual[m, n]) on v_mfma_i32_16x16x64_i8: the sum is exact
+ * (int32, K <= 131071), the rest float32 with one rounding to out_dtype.  act: 0 none, 1 SiLU.
+ *   a [M, lda], w [N, ldw] int8 with rows on 16-byte boundaries (pointer and pitch; bytes behind K may hold anything), a_scale [M],
+ *   w_scale [N] float32; bias [N] float32 or NULL; residual [M, ldr] in out_dtype or NULL (may alias out); out [M, ldo].
+ * workspace: adcdiff_gemm_i8_workspace_bytes(M, N, K) bytes on a 16-byte boundary (0: none needed), not shared by calls that overlap. */
+typedef struct adcdiff_gemm_i8_args {
+    int M, N, K;
+    const int8_t* a;
+    long long lda;
+    const int8_t* w;
+    long long ldw;
+    const float *a_scale, *w_scale, *bias;
+    const void* residual;
+    long long ldr;
+    int act, out_dtype;
+    void* out;
+    long long ldo;
+} adcdiff_gemm_i8_args;
+size_t adcdiff_gemm_i8_workspace_bytes(int M, int N, int K);
+int adcdiff_gemm_i8(const adcdiff_gemm_i8_args* args, void* workspace, size_t workspace_bytes, adcdiff_stream_t stream);
+
+/* Codes copied to rows on 16-byte boundaries: dst [M, ld_dst] (ld_dst a multiple of 16, >= K) from src [M, ld_src] at any alignment; the
+ * columns behind K are written as 0. */
+int adcdiff_pitch_rows_i8(const int8_t* src, long long ld_src, int M, int K, int8_t* dst, long long ld_dst, adcdiff_stream_t stream);
+
 /* ------------------------------------------------------------------ measurement ------ */
 
 /* Measurement and test switches; no counterpart in the reference.  With no call of adcdiff_debug_set the library reads no
