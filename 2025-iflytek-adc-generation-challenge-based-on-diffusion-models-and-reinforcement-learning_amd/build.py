@@ -32,7 +32,10 @@ def build_library(force=False, verbose=False):
     gen, inc = os.path.join(CSRC, "gen_w4_mainloop.py"), os.path.join(CSRC, "w4_mainloop.inc")
     if force or _stale(inc, [gen]):
         subprocess.run([sys.executable, gen, inc], check=True)
-    headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "row_access.h"), os.path.join(CSRC, "unet_plan.h"), inc, os.path.join(os.path.dirname(HERE), "include", "adcdiff.h")]
+    inc_i8 = os.path.join(CSRC, "w4_mainloop_i8.inc")
+    if force or _stale(inc_i8, [gen]):
+        subprocess.run([sys.executable, gen, "--i8", inc_i8], check=True)
+    headers = [inc_i8, os.path.join(CSRC, "common.h"), os.path.join(CSRC, "row_access.h"), os.path.join(CSRC, "unet_plan.h"), inc, os.path.join(os.path.dirname(HERE), "include", "adcdiff.h")]
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
     objs, cmds = [], []

@@ -147,6 +147,12 @@ struct I8Params {
     int M, N, K, act;
 };
 
+// v * sigmoid(v) on the hardware's exp2 and reciprocal (each within one unit in the last place): the argument's rounding adds |v| * 2^-24 relative,
+// which the sigmoid's own slope keeps below 2^-23 of |v|; the exact division costs four times the instructions.
+__device__ __forceinline__ float silu_fast(float v) {
+    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896f));
+}
+
 // 16 bytes of a row from column k on, with the bytes at columns >= K cleared.  Rows start on 16-byte boundaries, so a chunk that holds a
 // valid byte never leaves the page of that byte: the bytes behind K may be read, and count for nothing.
 __device__ __forceinline__ i32x4 load_chunk(const int8_t* __restrict__ row, int k, int K) {
@@ -175,7 +181,7 @@ __device__ __forceinline__ void finish(const I8Params& p, int m, int n, const i3
         float v = ((float)acc[i] * sa) * p.w_scale[n + i];
         if (p.bias) v += p.bias[n + i];
         if (p.residual) v += (float)res[n + i];
-        if (p.act) v = silu_f(v);
+        if (p.act) v = silu_fast(v);
         out[n + i] = (Out)v;
     }
 }
@@ -242,6 +248,262 @@ __global__ __launch_bounds__(256) void gemm_i8_kernel(const I8Params p) {
     }
 }
 
+// ---- few rows: the waves of a workgroup share its BM x BN tile and split K ---------------------------------------------------
+// A unit is 128 columns (a cache line of a row, two MFMA steps).  Wave w takes units w, w + WAVES, ..; its fragments go from memory to
+// registers (no LDS stage, no barrier), DEPTH units in flight.  The partial sums meet in LDS; integer sums do not depend on their
+// order.  Bound by the latency of one or two rounds of loads; the tile is kept small so that enough workgroups share the weights' bytes.
+template <typename Out, int BM, int BN, int WAVES, int DEPTH>
+__global__ __launch_bounds__(64 * WAVES) void gemm_i8_split_kernel(const I8Params p) {
+    constexpr int TM = BM / 16, TN = BN / 16, PITCH = BN + 4;
+    __shared__ __attribute__((aligned(16))) int part[WAVES][BM * PITCH];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ntn = (p.N + BN - 1) / BN;
+    const int m0 = blockIdx.x / ntn * BM, n0 = blockIdx.x % ntn * BN;
+    const int8_t *ra[TM], *rw[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) ra[i] = p.a + (long long)min(m0 + 16 * i + (lane & 15), p.M - 1) * p.lda;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) rw[j] = p.w + (long long)min(n0 + 16 * j + (lane & 15), p.N - 1) * p.ldw;
+    const int kl = (lane >> 4) * 16;
+    const int units = (p.K + 127) / 128;
+    const bool ragged = (p.K & 15) != 0;
+    i32x4 acc[TM][TN] = {};
+    i32x4 fa[DEPTH][2][TM], fw[DEPTH][2][TN];
+    // Only the weights are cleared behind K; the rows' codes there meet zeros.
+    auto load = [&](int d, int u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = u * 128 + h * 64 + kl;
+            const bool in = k < p.K;
+            const int ka = in ? k : 0;
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                fw[d][h][j] = *reinterpret_cast<const i32x4*>(rw[j] + ka);
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) fa[d][h][i] = *reinterpret_cast<const i32x4*>(ra[i] + ka);
+        }
+    };
+    auto multiply = [&](int d, int u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (u + 1 == units) {   // the last unit: clear what lies behind K
+                const int keep = p.K - (u * 128 + h * 64 + kl);
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int b = keep - 4 * i;
+                        fw[d][h][j][i] = b >= 4 ? fw[d][h][j][i] : b <= 0 || !ragged ? 0 : fw[d][h][j][i] & (int)((1u << (8 * (b & 3))) - 1u);
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[d][h][j], fa[d][h][i], acc[i][j], 0, 0, 0);
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (wave + d * WAVES < units) load(d, wave + d * WAVES);
+    for (int u = wave; u < units; u += DEPTH * WAVES) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const int v = u + d * WAVES;
+            if (v < units) {
+                multiply(d, v);
+                if (v + DEPTH * WAVES < units) load(d, v + DEPTH * WAVES);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            *reinterpret_cast<i32x4*>(&part[wave][(16 * i + (lane & 15)) * PITCH + 16 * j + 4 * (lane >> 4)]) = acc[i][j];
+    __syncthreads();
+    for (int e = tid; e < BM * BN / 4; e += 64 * WAVES) {
+        const int r = e / (BN / 4), c = e % (BN / 4) * 4;
+        i32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) sum += *reinterpret_cast<const i32x4*>(&part[w][r * PITCH + c]);
+        if (m0 + r < p.M) finish<Out>(p, m0 + r, n0 + c, sum, p.a_scale[m0 + r]);
+    }
+}
+
+// ---- many rows: 256 x 256 tile, 4 waves (2 x 2, 128 x 128 each), one wave per SIMD --------------------------------------------
+// The main loop is the hand-allocated assembly of the bf16 product (gen_w4_mainloop.py, which documents registers, LDS image and
+// protocol) with the 8-bit MFMA: a K tile is the same 128 bytes of a row, now 128 codes.  It runs over the whole K tiles; columns
+// behind them are added by a short tail on fragments loaded straight from memory.  A tile at the lower or right edge is moved back inside
+// the matrix (every load in range) and stores only the rows and columns that no other tile stores.
+#include "w4_mainloop_i8.inc"
+
+// SIDE: bit 0 residual, bit 1 SiLU, known at compile time so that loads and stores are counted exactly and no wait covers the stores; -1: asked
+// for at run time, together with single-element accesses (outputs whose rows are not on 16-byte boundaries).
+template <typename Out, int SIDE>
+__global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(const I8Params p) {
+    constexpr bool VEC = SIDE >= 0;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
+    // consecutive tiles (the columns of one tile row first) run on one XCD, whose L2 they share; workgroup b runs on XCD b mod 8
+    const int nwg = gridDim.x, ntn = (p.N + 255) >> 8;
+    const int xcd = blockIdx.x & 7, share_of = nwg >> 3, more = nwg & 7;
+    const int bid = xcd * share_of + min(xcd, more) + (blockIdx.x >> 3);
+    const int nidx = bid % ntn;
+    const int m_lo = bid / ntn * 256, n_lo = nidx * 256;
+    const int m0 = min(m_lo, p.M - 256), n0 = min(n_lo, p.N - 256);
+    const int kt = p.K >> 7;
+
+    const bool loads_a = wave < 2;
+    const int half = wave & 1;
+    const unsigned ld = (unsigned)(loads_a ? p.lda : p.ldw);
+    const unsigned long long base = loads_a ? (unsigned long long)p.a + (unsigned long long)(m0 + half * 128) * p.lda
+                                            : (unsigned long long)p.w + (unsigned long long)(n0 + half * 128) * p.ldw;
+    const int seg_lo = __builtin_amdgcn_readfirstlane((int)(unsigned)base);
+    const int seg_hi = __builtin_amdgcn_readfirstlane((int)((unsigned)(base >> 32) & 0xffffu));
+    const int seg_ld = __builtin_amdgcn_readfirstlane((int)ld);
+    const int seg_kt = __builtin_amdgcn_readfirstlane(kt);
+    const int seg_nrec = __builtin_amdgcn_readfirstlane((int)(127u * ld + (unsigned)kt * 128u));
+    const int zero = __builtin_amdgcn_readfirstlane(0);
+    const int s_dst = __builtin_amdgcn_readfirstlane((int)(lds0 + (loads_a ? 0u : 32768u) + (unsigned)half * 16384u));
+    const int frow = lane & 15, fchunk = lane >> 4, fx = (frow >> 1) & 7;
+    const int v_aoff0 = (int)lds0 + (wm * 128 + frow) * 128 + ((fchunk ^ fx) << 4);
+    const int v_aoff1 = (int)lds0 + (wm * 128 + frow) * 128 + (((4 + fchunk) ^ fx) << 4);
+    const int v_boff0 = (int)lds0 + 32768 + (wn * 128 + frow) * 128 + ((fchunk ^ fx) << 4);
+    const int v_boff1 = (int)lds0 + 32768 + (wn * 128 + frow) * 128 + (((4 + fchunk) ^ fx) << 4);
+    const int v_src0 = (int)((unsigned)(lane >> 3) * ld + (unsigned)(((lane & 7) ^ (lane >> 4)) * 16));
+    const int v_src1 = (int)((unsigned)(lane >> 3) * ld + (unsigned)(((lane & 7) ^ (4 + (lane >> 4))) * 16));
+    // L2 prefetch: the workgroups of a tile row share its A rows and split the touching of them (a share of at most 64 rows each)
+    const int share = ntn >= 4 ? max(1, 256 / ntn) : 64;
+    const int prow0 = ntn >= 4 ? min(nidx * share, 256 - share) : half * 128 + (ntn == 2 ? nidx * 64 : 0);
+    const bool pf_wave = loads_a && (prow0 >> 7) == half;
+    const int pf_row = min((prow0 & 127) + lane % share, 127);
+    const int v_pf = pf_wave ? (int)((unsigned)pf_row * ld + (unsigned)(lane / share) * 128u) : 0;
+
+    i32x4 acc[8][8];
+    asm volatile(ADCDIFF_W4I8_MAINLOOP_ASM
+                 : ADCDIFF_W4_OUTS(acc)
+                 : "{s40}"(seg_lo), "{s41}"(seg_hi), "{s42}"(seg_ld), "{s43}"(seg_kt), "{s44}"(seg_nrec), "{s45}"(zero), "{s46}"(zero), "{s47}"(zero),
+                   "{s48}"(zero), "{s49}"(zero), "{s50}"(zero), "{s51}"(zero), "{s52}"(zero), "{s53}"(zero), "{s54}"(zero), "{s55}"(seg_kt), "{s56}"(s_dst),
+                   "{v130}"(v_aoff0), "{v131}"(v_boff0), "{v132}"(v_aoff1), "{v133}"(v_boff1), "{v136}"(v_src0), "{v137}"(v_src1), "{v138}"(v_src0),
+                   "{v139}"(v_src1), "{v140}"(v_src0), "{v141}"(v_src1), "{v144}"(v_pf), "{v145}"(v_pf), "{v146}"(v_pf)
+                 : ADCDIFF_W4_CLOBBERS);
+    const int mw = m0 + wm * 128, nw = n0 + wn * 128;
+    for (int k0 = kt * 128; k0 < p.K; k0 += 64) {   // the columns behind the whole K tiles
+        const int k = k0 + fchunk * 16;
+        const int8_t* rw = p.w + (long long)(nw + frow) * p.ldw;
+        const int8_t* ra = p.a + (long long)(mw + frow) * p.lda;
+#pragma unroll
+        for (int jh = 0; jh < 8; jh += 4) {
+            i32x4 fw[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) fw[j] = load_chunk(rw + (long long)(16 * (jh + j)) * p.ldw, k, p.K);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const i32x4 fa = load_chunk(ra + (long long)(16 * i) * p.lda, k, p.K);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][jh + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fa, acc[i][jh + j], 0, 0, 0);
+            }
+        }
+    }
+    // A lane holds outputs 4 g .. 4 g + 3 (g = lane / 16) of row lane % 16 in every 16 x 16 block.  Exchanging odd lane rows of block 2 j with even
+    // ones of block 2 j + 1 leaves it eight consecutive outputs: columns 0..7 (g 0, 1) or 8..15 (g 2, 3) of block 2 j (g even) or 2 j + 1.
+    const int nl = nw + 16 * (fchunk & 1) + 8 * (fchunk >> 1);
+    // Scales, biases and the first rows' residual are loaded before the first store, and each further residual one step ahead of its use:
+    // a load behind a store to memory that it might share waits a whole round trip (measured: 13 of 27 us outside the K loop).
+    float w[4][8], b[4][8], sa[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            w[j][c] = p.w_scale[nl + 32 * j + c];
+            b[j][c] = p.bias ? p.bias[nl + 32 * j + c] : 0.0f;
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sa[i] = p.a_scale[mw + 16 * i + frow];
+    typedef Out Side __attribute__((ext_vector_type(8)));
+    typedef Side SideAny __attribute__((aligned(VEC ? 16 : sizeof(Out))));
+    const bool residual = SIDE >= 0 ? (SIDE & 1) != 0 : p.residual != nullptr, act = SIDE >= 0 ? (SIDE & 2) != 0 : p.act != 0;
+    const Out* const res = static_cast<const Out*>(p.residual) + (long long)(mw + frow) * p.ldr + nl;
+    Side side[2][4];
+    auto fetch = [&](int i) __attribute__((always_inline)) {
+        if (residual) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) side[i & 1][j] = *reinterpret_cast<const SideAny*>(res + (long long)(16 * i) * p.ldr + 32 * j);
+        }
+    };
+    fetch(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long m = mw + 16 * i + frow;
+        if (i < 7) fetch(i + 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float v[8];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const auto s = __builtin_amdgcn_permlane16_swap((unsigned)acc[i][2 * j][c], (unsigned)acc[i][2 * j + 1][c], false, false);
+                v[c] = fmaf((float)(int)s[0] * sa[i], w[j][c], b[j][c]);
+                v[4 + c] = fmaf((float)(int)s[1] * sa[i], w[j][4 + c], b[j][4 + c]);
+            }
+            if (residual) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[c] += (float)side[i & 1][j][c];
+            }
+            if (act) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[c] = silu_fast(v[c]);
+            }
+            const int n = nl + 32 * j;
+            Out* out = static_cast<Out*>(p.out) + m * p.ldo + n;
+            Side o;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) o[c] = (Out)v[c];
+            if (m >= m_lo) {
+                if (n >= n_lo) {
+                    *reinterpret_cast<SideAny*>(out) = o;
+                } else if constexpr (!VEC) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        if (n + c >= n_lo) out[c] = o[c];
+                }
+            }
+        }
+    }
+}
+
+template <typename Out, int SIDE>
+int launch_w4(const I8Params& p, hipStream_t stream) {
+    constexpr int smem = 2 * 65536;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_i8_w4_kernel<Out, SIDE>), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (attr != hipSuccess) return fail(ADCDIFF_E_LAUNCH, "gemm_i8: hipFuncSetAttribute: %s", hipGetErrorString(attr));
+    const long long tiles = (((long long)p.M + 255) / 256) * (((long long)p.N + 255) / 256);
+    if (tiles > 0xffffff) return fail(ADCDIFF_E_BADARG, "gemm_i8: %d x %d outputs are too many for one call", p.M, p.N);
+    hipLaunchKernelGGL((gemm_i8_w4_kernel<Out, SIDE>), dim3((unsigned)tiles), dim3(256), smem, stream, p);
+    return check_launch("gemm_i8");
+}
+
+template <typename Out>
+int launch_w4_side(const I8Params& p, hipStream_t stream) {
+    constexpr int per16 = 16 / sizeof(Out);
+    const bool vec = p.N % 8 == 0 && aligned16(p.out) && p.ldo % per16 == 0 && (!p.residual || (aligned16(p.residual) && p.ldr % per16 == 0));
+    if (!vec) return launch_w4<Out, -1>(p, stream);
+    if (p.act) return p.residual ? launch_w4<Out, 3>(p, stream) : launch_w4<Out, 2>(p, stream);
+    return p.residual ? launch_w4<Out, 1>(p, stream) : launch_w4<Out, 0>(p, stream);
+}
+
+template <typename Out, int BM, int BN, int WAVES, int DEPTH>
+int launch_split(const I8Params& p, hipStream_t stream) {
+    const long long tiles = (((long long)p.M + BM - 1) / BM) * (((long long)p.N + BN - 1) / BN);
+    if (tiles * WAVES * 64 > 0xffffffffLL) return fail(ADCDIFF_E_BADARG, "gemm_i8: %d x %d outputs are too many for one call", p.M, p.N);
+    hipLaunchKernelGGL((gemm_i8_split_kernel<Out, BM, BN, WAVES, DEPTH>), dim3((unsigned)tiles), dim3(64 * WAVES), 0, stream, p);
+    return check_launch("gemm_i8");
+}
+
 template <typename Out, int BM, int BN>
 int launch_tiles(const I8Params& p, hipStream_t stream) {
     const long long tiles = (((long long)p.M + BM - 1) / BM) * (((long long)p.N + BN - 1) / BN);
@@ -252,7 +514,15 @@ int launch_tiles(const I8Params& p, hipStream_t stream) {
 
 template <typename Out>
 int launch_gemm(const I8Params& p, hipStream_t stream) {
-    return p.M <= 32 ? launch_tiles<Out, 32, 32>(p, stream) : launch_tiles<Out, 128, 128>(p, stream);
+    const long long tiles256 = (((long long)p.M + 255) / 256) * (((long long)p.N + 255) / 256);
+    if (p.M >= 256 && p.N >= 256 && p.K >= 256 && tiles256 >= 96 && p.lda < (1 << 23) && p.ldw < (1 << 23)) {
+        return launch_w4_side<Out>(p, stream);
+    }
+    if (p.M <= 16) return launch_split<Out, 16, 16, 16, 2>(p, stream);
+    if (p.M <= 32) return launch_split<Out, 32, 16, 8, 4>(p, stream);
+    if (p.M <= 128) return launch_split<Out, 64, 32, 8, 2>(p, stream);
+    if ((long long)((p.M + 63) / 64) * ((p.N + 63) / 64) <= 1024) return launch_split<Out, 64, 64, 4, 2>(p, stream);
+    return launch_tiles<Out, 128, 128>(p, stream);
 }
 
 constexpr int kMaxK = 131071;   // 128 * 128 * K stays below 2^31

@@ -53,6 +53,8 @@ W_SET = [0, 64]
 STAGE = 0x10000
 PF = 4           # prefetch distance in K tiles beyond the tile being staged
 L = []
+INT8 = False     # --i8: the loop of the 8-bit integer product (gemm_i8.hip): the same bytes, 128 codes per K tile, v_mfma_i32_16x16x64_i8 with the
+                 # weights as first operand, so that a lane's four results are four consecutive outputs of one row
 ABLATE = set()   # lab only: "nodma", "noread", "nobar", "nowait", "dmafirsthalf", "nopf"; "stamps": the measurement build's loop
 
 
@@ -64,6 +66,9 @@ def mfma(i, j, s):
     acc = 4 * (8 * i + j)
     a = A_SET[s] + 4 * i
     w = W_SET[s] + 4 * j
+    if INT8:
+        e(f"v_mfma_i32_16x16x64_i8 a[{acc}:{acc + 3}], v[{w}:{w + 3}], v[{a}:{a + 3}], a[{acc}:{acc + 3}]")
+        return
     e(f"v_mfma_f32_16x16x32_bf16 a[{acc}:{acc + 3}], v[{a}:{a + 3}], v[{w}:{w + 3}], a[{acc}:{acc + 3}]")
 
 
@@ -320,6 +325,7 @@ def emit(f, name):
 
 def main():
     # gen_w4_mainloop.py [out]                      the product's loop
+    # gen_w4_mainloop.py --i8 out                   the loop of the 8-bit integer product
     # gen_w4_mainloop.py --lab out name=flag+flag.. ablated variants for the main-loop laboratory
     if len(sys.argv) > 1 and sys.argv[1] == "--lab":
         with open(sys.argv[2], "w") as f:
@@ -342,6 +348,15 @@ def main():
         with open(sys.argv[2], "w") as f:
             f.write("// Generated by gen_w4_mainloop.py --stamps -- do not edit.\n")
             emit(f, "ADCDIFF_W4S_MAINLOOP_ASM")
+        return
+    global INT8
+    if len(sys.argv) > 2 and sys.argv[1] == "--i8":
+        INT8 = True
+        generate()
+        with open(sys.argv[2], "w") as f:
+            f.write("// Generated by gen_w4_mainloop.py --i8 -- do not edit.  Register map and protocol: see the generator.\n")
+            emit_constraints(f)
+            emit(f, "ADCDIFF_W4I8_MAINLOOP_ASM")
         return
     import os
     ABLATE.update(x for x in os.environ.get("W4_ABLATE", "").split("+") if x)   # experiments: W4_ABLATE=dmafirsthalf+readlate
