@@ -138,6 +138,8 @@ __global__ __launch_bounds__(256) void pitch_rows_kernel(const int8_t* __restric
 }
 
 // ------------------------------------------------------------------ product
+typedef f32x4 f32x4_any __attribute__((aligned(4)));   // vectors of scales and biases start at any element
+
 struct I8Params {
     const int8_t *a, *w;
     const float *a_scale, *w_scale, *bias;
@@ -145,6 +147,7 @@ struct I8Params {
     void* out;
     long long lda, ldw, ldr, ldo;
     int M, N, K, act;
+    bool vec;
 };
 
 // v * sigmoid(v) on the hardware's exp2 and reciprocal (each within one unit in the last place): the argument's rounding adds |v| * 2^-24 relative,
@@ -169,82 +172,134 @@ __device__ __forceinline__ i32x4 load_chunk(const int8_t* __restrict__ row, int 
     return v;
 }
 
+// Eight consecutive outputs of row m from column n on (fewer at the right edge)
 template <typename Out>
-__device__ __forceinline__ void finish(const I8Params& p, int m, int n, const i32x4& acc, float sa) {
-    // four consecutive outputs of a row
-    if (m >= p.M) return;
-    const Out* res = static_cast<const Out*>(p.residual) + (long long)m * p.ldr;
-    Out* out = static_cast<Out*>(p.out) + (long long)m * p.ldo;
+__device__ __forceinline__ void finish8(const I8Params& p, int m, int n, const i32x4& lo, const i32x4& hi) {
+    const float sa = p.a_scale[m];
+    const Out* res = static_cast<const Out*>(p.residual) + (long long)m * p.ldr + n;
+    Out* out = static_cast<Out*>(p.out) + (long long)m * p.ldo + n;
+    typedef Out Eight __attribute__((ext_vector_type(8)));
+    typedef Eight EightAt16 __attribute__((aligned(16)));
+    if (p.vec) {   // N is a multiple of 8 and rows of out and residual lie on 16-byte boundaries
+        float w[8], b[8] = {};
+        Eight r, o;
+        const f32x4_any* pw = reinterpret_cast<const f32x4_any*>(p.w_scale + n);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (n + i >= p.N) break;
-        float v = ((float)acc[i] * sa) * p.w_scale[n + i];
-        if (p.bias) v += p.bias[n + i];
-        if (p.residual) v += (float)res[n + i];
-        if (p.act) v = silu_fast(v);
-        out[n + i] = (Out)v;
+        for (int c = 0; c < 4; ++c) { w[c] = pw[0][c]; w[4 + c] = pw[1][c]; }
+        if (p.bias) {
+            const f32x4_any* pb = reinterpret_cast<const f32x4_any*>(p.bias + n);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) { b[c] = pb[0][c]; b[4 + c] = pb[1][c]; }
+        }
+        if (p.residual) r = *reinterpret_cast<const EightAt16*>(res);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            float v = fmaf((float)(c < 4 ? lo[c & 3] : hi[c & 3]) * sa, w[c], b[c]);
+            if (p.residual) v += (float)r[c];
+            if (p.act) v = silu_fast(v);
+            o[c] = (Out)v;
+        }
+        *reinterpret_cast<EightAt16*>(out) = o;
+    } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (n + c >= p.N) break;
+            float v = fmaf((float)(c < 4 ? lo[c & 3] : hi[c & 3]) * sa, p.w_scale[n + c], p.bias ? p.bias[n + c] : 0.0f);
+            if (p.residual) v += (float)res[c];
+            if (p.act) v = silu_fast(v);
+            out[c] = (Out)v;
+        }
     }
 }
 
-// BM x BN tile, 4 waves in WM x WN, K in steps of 128 through two LDS stages filled from registers.  LDS rows of 128 bytes, the
-// 16-byte chunk c of a row at position c ^ ((row >> 1) & 7): fragment reads are free of bank conflicts.  The weights are the MFMA's
-// first operand, so a lane's four results are four consecutive outputs of one row.
-template <typename Out, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(256) void gemm_i8_kernel(const I8Params p) {
-    constexpr int TM = BM / WM / 16, TN = BN / WN / 16, CHUNKS = (BM + BN) * 8 / 256;
-    __shared__ __attribute__((aligned(16))) char smem[2][(BM + BN) * 128];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = wave / WN, wn = wave % WN;
-    const int ntn = (p.N + BN - 1) / BN;
-    const int m0 = blockIdx.x / ntn * BM, n0 = blockIdx.x % ntn * BN;
-    const int8_t* src[CHUNKS];
-    int dst[CHUNKS];
+// ---- BM x BN tile through a ring of LDS stages ------------------------------------------------------------------------------------
+// Eight waves (2 x 4); a stage is 128 columns of the tile's rows, filled by LDS-DMA (64 lanes x 16 bytes = eight rows of 128 bytes per
+// instruction).  The chunk c of a row lies at position c ^ ((row >> 1) & 7), applied to the source address, so fragment reads are free of bank
+// conflicts.  STAGES - 1 tiles are under way; a stage is refilled behind the barrier that follows the last wait for its reads.  The loop is
+// bound by the LDS-DMA (one instruction of 1 KiB per CU every 21 ns), hence the deep ring and, for the same output, the larger tile; two waves per
+// SIMD cover each other's LDS reads.  The weights are the MFMA's first operand: a lane's four results are consecutive outputs of a row.
+template <typename Out, int BM, int BN, int STAGES>
+__global__ __launch_bounds__(512) void gemm_i8_ring_kernel(const I8Params p) {
+    constexpr int TM = BM / 32, TN = BN / 64, PIECES = (BM + BN) / 64, STAGE = (BM + BN) * 128, PITCH = BN + 4;
+    static_assert(PIECES * 64 == BM + BN && TN >= 1, "a wave loads PIECES pieces of eight rows");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 2, wn = wave & 3;
+    // consecutive tiles on one XCD (workgroup b runs on XCD b mod 8): they share rows in its L2
+    const int ntn = (p.N + BN - 1) / BN, xcd = blockIdx.x & 7;
+    const int bid = xcd * (gridDim.x >> 3) + min(xcd, (int)(gridDim.x & 7)) + (blockIdx.x >> 3);
+    const int m0 = bid / ntn * BM, n0 = bid % ntn * BN;
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
+    const int8_t* src[PIECES];
 #pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) {
-        const int id = tid + 256 * j, r = id >> 3, c = id & 7;
-        src[j] = (r < BM ? p.a + (long long)min(m0 + r, p.M - 1) * p.lda : p.w + (long long)min(n0 + r - BM, p.N - 1) * p.ldw);
-        dst[j] = r * 128 + ((c ^ ((r >> 1) & 7)) << 4);
+    for (int j = 0; j < PIECES; ++j) {   // rows past the edge repeat the last one; what they give is not stored
+        const int r = (wave * PIECES + j) * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+        src[j] = (r < BM ? p.a + (long long)min(m0 + r, p.M - 1) * p.lda : p.w + (long long)min(n0 + r - BM, p.N - 1) * p.ldw) + 16 * c;
     }
+    const unsigned dst = lds0 + (unsigned)(wave * PIECES) * 1024u;
+    auto issue = [&](int t, int stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) glds16_untracked(src[j] + (long long)t * 128, dst + (unsigned)stage * STAGE + 1024u * j);
+    };
     i32x4 acc[TM][TN] = {};
-    i32x4 next[CHUNKS];
-    const int kc = (tid & 7) * 16;
-#pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) next[j] = load_chunk(src[j], kc, p.K);
-    const int tiles = (p.K + 127) / 128;
-    for (int t = 0; t < tiles; ++t) {
-        char* st = smem[t & 1];
-#pragma unroll
-        for (int j = 0; j < CHUNKS; ++j) *reinterpret_cast<i32x4*>(st + dst[j]) = next[j];
-        if (t + 1 < tiles) {
-#pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) next[j] = load_chunk(src[j], (t + 1) * 128 + kc, p.K);
-        }
-        __syncthreads();   // one per tile: a stage is written again only after the barrier of the tile in between
+    auto multiply = [&](const char* st) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             i32x4 fa[TM], fw[TN];
 #pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const int r = wm * TM * 16 + i * 16 + (lane & 15);
-                fa[i] = *reinterpret_cast<const i32x4*>(st + r * 128 + (((4 * h + (lane >> 4)) ^ ((r >> 1) & 7)) << 4));
+            for (int j = 0; j < TN; ++j) {
+                const int r = BM + (wn * TN + j) * 16 + (lane & 15);
+                fw[j] = *reinterpret_cast<const i32x4*>(st + r * 128 + (((4 * h + (lane >> 4)) ^ ((r >> 1) & 7)) << 4));
             }
 #pragma unroll
-            for (int i = 0; i < TN; ++i) {
-                const int r = BM + wn * TN * 16 + i * 16 + (lane & 15);
-                fw[i] = *reinterpret_cast<const i32x4*>(st + r * 128 + (((4 * h + (lane >> 4)) ^ ((r >> 1) & 7)) << 4));
+            for (int i = 0; i < TM; ++i) {
+                const int r = (wm * TM + i) * 16 + (lane & 15);
+                fa[i] = *reinterpret_cast<const i32x4*>(st + r * 128 + (((4 * h + (lane >> 4)) ^ ((r >> 1) & 7)) << 4));
             }
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fa[i], acc[i][j], 0, 0, 0);
         }
+    };
+    const int kt = p.K >> 7;
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t)
+        if (t < kt) issue(t, t);
+    int stage = 0;
+    for (int t = 0; t < kt; ++t) {
+        // tiles t + 1 .. t + STAGES - 2 may stay in flight; then every wave's pieces of tile t are there, and stage t - 1 has been read
+        wait_tiles_in_flight<PIECES>(min(STAGES - 2, kt - 1 - t));
+        asm volatile("s_barrier" ::: "memory");
+        if (t + STAGES - 1 < kt) issue(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+        multiply(smem + stage * STAGE);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this wave's reads are done before it meets the next barrier
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
+    if (p.K & 127) {   // the columns behind the whole tiles, through registers, cleared behind K
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int m = m0 + wm * TM * 16 + i * 16 + (lane & 15);
-        const float sa = m < p.M ? p.a_scale[m] : 0.0f;
+        for (int j = 0; j < PIECES; ++j) {
+            const int r = (wave * PIECES + j) * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+            *reinterpret_cast<i32x4*>(smem + (wave * PIECES + j) * 1024 + lane * 16) = load_chunk(src[j] - 16 * c, kt * 128 + 16 * c, p.K);
+        }
+        __syncthreads();
+        multiply(smem);
+    }
+    __syncthreads();
+    int* const sums = reinterpret_cast<int*>(smem);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) finish<Out>(p, m, n0 + wn * TN * 16 + j * 16 + 4 * (lane >> 4), acc[i][j], sa);
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            *reinterpret_cast<i32x4*>(sums + ((wm * TM + i) * 16 + (lane & 15)) * PITCH + (wn * TN + j) * 16 + 4 * (lane >> 4)) = acc[i][j];
+    __syncthreads();
+#pragma unroll
+    for (int e = tid; e < BM * BN / 8; e += 512) {
+        const int r = e / (BN / 8), c = e % (BN / 8) * 8;
+        if (m0 + r < p.M && n0 + c < p.N)
+            finish8<Out>(p, m0 + r, n0 + c, *reinterpret_cast<const i32x4*>(sums + r * PITCH + c), *reinterpret_cast<const i32x4*>(sums + r * PITCH + c + 4));
     }
 }
 
@@ -323,12 +378,16 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_i8_split_kernel(const I8Param
         for (int j = 0; j < TN; ++j)
             *reinterpret_cast<i32x4*>(&part[wave][(16 * i + (lane & 15)) * PITCH + 16 * j + 4 * (lane >> 4)]) = acc[i][j];
     __syncthreads();
-    for (int e = tid; e < BM * BN / 4; e += 64 * WAVES) {
-        const int r = e / (BN / 4), c = e % (BN / 4) * 4;
-        i32x4 sum = {0, 0, 0, 0};
+    for (int e = tid; e < BM * BN / 8; e += 64 * WAVES) {
+        const int r = e / (BN / 8), c = e % (BN / 8) * 8;
+        if (m0 + r >= p.M || n0 + c >= p.N) continue;
+        i32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) sum += *reinterpret_cast<const i32x4*>(&part[w][r * PITCH + c]);
-        if (m0 + r < p.M) finish<Out>(p, m0 + r, n0 + c, sum, p.a_scale[m0 + r]);
+        for (int w = 0; w < WAVES; ++w) {
+            lo += *reinterpret_cast<const i32x4*>(&part[w][r * PITCH + c]);
+            hi += *reinterpret_cast<const i32x4*>(&part[w][r * PITCH + c + 4]);
+        }
+        finish8<Out>(p, m0 + r, n0 + c, lo, hi);
     }
 }
 
@@ -489,9 +548,7 @@ int launch_w4(const I8Params& p, hipStream_t stream) {
 
 template <typename Out>
 int launch_w4_side(const I8Params& p, hipStream_t stream) {
-    constexpr int per16 = 16 / sizeof(Out);
-    const bool vec = p.N % 8 == 0 && aligned16(p.out) && p.ldo % per16 == 0 && (!p.residual || (aligned16(p.residual) && p.ldr % per16 == 0));
-    if (!vec) return launch_w4<Out, -1>(p, stream);
+    if (!p.vec) return launch_w4<Out, -1>(p, stream);
     if (p.act) return p.residual ? launch_w4<Out, 3>(p, stream) : launch_w4<Out, 2>(p, stream);
     return p.residual ? launch_w4<Out, 1>(p, stream) : launch_w4<Out, 0>(p, stream);
 }
@@ -504,25 +561,40 @@ int launch_split(const I8Params& p, hipStream_t stream) {
     return check_launch("gemm_i8");
 }
 
-template <typename Out, int BM, int BN>
-int launch_tiles(const I8Params& p, hipStream_t stream) {
+template <typename Out, int BM, int BN, int STAGES>
+int launch_ring(const I8Params& p, hipStream_t stream) {
+    constexpr int smem = std::max((BM + BN) * 128 * STAGES, BM * (BN + 4) * 4);
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_i8_ring_kernel<Out, BM, BN, STAGES>), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (attr != hipSuccess) return fail(ADCDIFF_E_LAUNCH, "gemm_i8: hipFuncSetAttribute: %s", hipGetErrorString(attr));
     const long long tiles = (((long long)p.M + BM - 1) / BM) * (((long long)p.N + BN - 1) / BN);
-    if (tiles > 0xffffff) return fail(ADCDIFF_E_BADARG, "gemm_i8: %d x %d outputs are too many for one call", p.M, p.N);
-    hipLaunchKernelGGL((gemm_i8_kernel<Out, BM, BN, 2, 2>), dim3((unsigned)tiles), dim3(256), 0, stream, p);
+    if (tiles > 0x7fffff) return fail(ADCDIFF_E_BADARG, "gemm_i8: %d x %d outputs are too many for one call", p.M, p.N);
+    hipLaunchKernelGGL((gemm_i8_ring_kernel<Out, BM, BN, STAGES>), dim3((unsigned)tiles), dim3(512), smem, stream, p);
     return check_launch("gemm_i8");
 }
 
+// Which kernel: measured on all of them over 1..65536 rows, 512..4096 outputs, 512..8192 columns (us, M x N x K).
+//   few rows: the smallest split tile that still gives at most one workgroup per CU
+//     32 x 2048 x 4096: 16 x 16 tile 7.1, 32 x 16 8.6, 32 x 32 10.2;  64 x 2048 x 2048: 6.9, 6.0, 6.7;  128 x 2048 x 2048: 11.4, 8.8, 7.2, 64 x 64 ring 7.9
+//   more: the least of these estimates, which are fits to the measured times (kt: K tiles of 128; one round: 256 workgroups)
+//     64 x 64 ring    2.5 + rounds (1.0 + 0.28 kt), two workgroups to a CU:  512 x 2048 x 2048 9.2 (128 x 128: 14.4), 1024 x 2048 x 2048 11.9 (15.7)
+//     128 x 128 ring  whole rounds (4.8 + 0.66 kt):  2048 x 2048 x 2048 17.3 (64 x 64: 22.1, 256 x 256: 27.7)
+//     256 x 256       whole rounds (10.7 + 1.5 kt), less where half the CUs stay free:  8192 x 2048 x 2048 34.3 (60.1), 65536 x 512 x 512 33.3 (59.7)
 template <typename Out>
 int launch_gemm(const I8Params& p, hipStream_t stream) {
-    const long long tiles256 = (((long long)p.M + 255) / 256) * (((long long)p.N + 255) / 256);
-    if (p.M >= 256 && p.N >= 256 && p.K >= 256 && tiles256 >= 96 && p.lda < (1 << 23) && p.ldw < (1 << 23)) {
-        return launch_w4_side<Out>(p, stream);
+    auto tiles = [&](int bm, int bn) { return (((long long)p.M + bm - 1) / bm) * (((long long)p.N + bn - 1) / bn); };
+    if (p.M <= 16 || tiles(16, 16) <= 256) return launch_split<Out, 16, 16, 8, 4>(p, stream);
+    if (tiles(32, 16) <= 256) return launch_split<Out, 32, 16, 8, 4>(p, stream);
+    if (tiles(32, 32) <= 256) return launch_split<Out, 32, 32, 8, 2>(p, stream);
+    const double kt = (p.K + 127) / 128;
+    auto rounds = [](long long n) { return (double)((n + 255) / 256); };
+    const double t64 = 2.5 + std::max(1.0, tiles(64, 64) / 256.0) * (1.0 + 0.28 * kt);
+    const double t128 = rounds(tiles(128, 128)) * (4.8 + 0.66 * kt);
+    // the 256 x 256 kernel needs whole tiles in every direction and 32-bit offsets inside them
+    if (p.M >= 256 && p.N >= 256 && p.K >= 256 && p.lda < (1 << 23) && p.ldw < (1 << 23)) {
+        const double t256 = rounds(tiles(256, 256)) * (10.7 + 1.5 * kt) * (tiles(256, 256) <= 128 ? 0.85 : 1.0);
+        if (t256 < std::min(t64, t128)) return launch_w4_side<Out>(p, stream);
     }
-    if (p.M <= 16) return launch_split<Out, 16, 16, 16, 2>(p, stream);
-    if (p.M <= 32) return launch_split<Out, 32, 16, 8, 4>(p, stream);
-    if (p.M <= 128) return launch_split<Out, 64, 32, 8, 2>(p, stream);
-    if ((long long)((p.M + 63) / 64) * ((p.N + 63) / 64) <= 1024) return launch_split<Out, 64, 64, 4, 2>(p, stream);
-    return launch_tiles<Out, 128, 128>(p, stream);
+    return t64 < t128 ? launch_ring<Out, 64, 64, 4>(p, stream) : launch_ring<Out, 128, 128, 4>(p, stream);
 }
 
 constexpr int kMaxK = 131071;   // 128 * 128 * K stays below 2^31
@@ -577,8 +649,9 @@ extern "C" int adcdiff_gemm_i8(const adcdiff_gemm_i8_args* a, void*, size_t, adc
         return fail(ADCDIFF_E_BADARG, "gemm_i8: the rows of a and w start on 16-byte boundaries and hold %d columns (pitches %lld, %lld)", a->K, a->lda, a->ldw);
     if (a->ldo < a->N || (a->residual && a->ldr < a->N)) return fail(ADCDIFF_E_BADARG, "gemm_i8: a row pitch below %d columns", a->N);
     hipStream_t stream = as_stream(stream_);
-    I8Params p{a->a, a->w, a->a_scale, a->w_scale, a->bias, a->residual, a->out, a->lda, a->ldw, a->ldr, a->ldo, a->M, a->N, a->K, a->act};
+    I8Params p{a->a, a->w, a->a_scale, a->w_scale, a->bias, a->residual, a->out, a->lda, a->ldw, a->ldr, a->ldo, a->M, a->N, a->K, a->act, false};
     const int so = type_size(a->out_dtype);
+    p.vec = a->N % 8 == 0 && vector_rows(a->out, a->ldo, so) && vector_rows(a->residual, a->ldr, so);
     TimingScope timing(ADCDIFF_KIND_OTHER, a->M, a->N, a->K, 2.0 * a->M * a->N * a->K,
                        (double)a->M * a->K + (double)a->N * a->K + (double)a->M * a->N * so * (a->residual ? 2 : 1), stream);
     return a->out_dtype == ADCDIFF_BF16 ? launch_gemm<bf16_t>(p, stream) : launch_gemm<float>(p, stream);

@@ -129,6 +129,33 @@ def test_epilogues(out, bias, residual, act):
         _check(M, N, K, out, bias, residual, act)
 
 
+@pytest.mark.parametrize("out", ["fp32", "bf16"])
+@pytest.mark.parametrize("residual, act", list(itertools.product((False, True), (0, 1))))
+@pytest.mark.parametrize("M, N, K", [(8200, 2056, 300), (8192, 2048, 256), (9001, 1800, 643), (16500, 1027, 400), (33000, 257, 513)])
+def test_large_products(M, N, K, out, residual, act):
+    """tiles that end past the last row and column, columns behind the whole K tiles, outputs on and off 16-byte boundaries"""
+    _check(M, N, K, out, True, residual, act)
+
+
+def test_residual_in_place():
+    """out may be the residual itself (C ABI): tiles at the edges overlap, and each element is still read before it is written once"""
+    import ctypes as C
+    from adcdiff import _lib
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    for M, N, K in ((8200, 2056, 300), (3000, 1000, 512), (600, 200, 128), (20, 300, 700)):
+        a, w = _codes(gen, M, (K + 15) // 16 * 16), _codes(gen, N, (K + 15) // 16 * 16)
+        sa, sw = torch.rand(M, generator=gen, device="cuda"), torch.rand(N, generator=gen, device="cuda")
+        res = torch.randn(M, N, generator=gen, device="cuda")
+        want = ops.gemm_int8(a[:, :K], sa, w[:, :K], sw, residual=res, out_dtype="fp32")
+        p = _lib.GemmI8Args()
+        p.M, p.N, p.K, p.out_dtype, p.lda, p.ldw, p.ldr, p.ldo = M, N, K, 0, a.stride(0), w.stride(0), N, N
+        p.a, p.w, p.a_scale, p.w_scale, p.residual, p.out = (t.data_ptr() for t in (a, w, sa, sw, res, res))
+        need = _lib.load().adcdiff_gemm_i8_workspace_bytes(M, N, K)
+        ws = torch.empty(max(16, need), dtype=torch.uint8, device="cuda")
+        _lib.check(_lib.load().adcdiff_gemm_i8(C.byref(p), ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(res, want)
+
+
 @pytest.mark.parametrize("M, N, K", [(1, 64, 1003), (50, 33, 77), (300, 1001, 515)])
 def test_packed_codes(M, N, K):
     """codes without padding between rows, and at odd addresses"""
