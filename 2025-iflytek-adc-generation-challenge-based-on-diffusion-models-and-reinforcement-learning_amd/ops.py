@@ -8,7 +8,10 @@ The public functions (gemm, groupnorm_silu, philox_normal, ddpm_step, ddim_step,
 the PyTorch dispatcher: they call the custom operators ``torch.ops.adcdiff.*`` registered in ``torch_ops.py``
 (torch.library.custom_op with fake-tensor rules), whose implementations are the ``_raw_*`` ctypes wrappers below.
 """
+import array
 import ctypes as C
+import operator
+import struct
 
 import torch
 
@@ -223,40 +226,30 @@ def _raw_latent_summary(x):
 _CODES = {torch.float32: F32, torch.bfloat16: BF16}
 _TYPES = {F32: torch.float32, BF16: torch.bfloat16}
 _NORMS = {None: 0, "rms": 1, "layer": 2}
+_dtype_of = operator.attrgetter("dtype")
+
+
+_current_device, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+# The C structs of include/adcdiff.h as one pack call each: filling a ctypes.Structure field by field takes several microseconds.
+_pack_norm_args = struct.Struct("8iQqQqQqQQQQffQqQqQ").pack       # adcdiff_residual_norm_args
+_pack_norm_grads = struct.Struct("QqQqQqQqQqQQQQ").pack           # adcdiff_residual_norm_grads
+_pack_gemm_i8 = struct.Struct("iii4xQqQqQQQQqiiQq").pack          # adcdiff_gemm_i8_args
 
 
 def _device_of(*tensors):
     """The index of the one GPU that holds all the tensors."""
     dev = -2
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            _need_gpu(t)
-        i = t.get_device()
-        if dev not in (-2, i):
-            raise ValueError("tensors on different devices: cuda:%d and cuda:%d" % (dev, i))
-        dev = i
+        if t is not None:
+            i = t.get_device()
+            if i != dev:
+                if i < 0:
+                    _need_gpu(t)
+                if dev != -2:
+                    raise ValueError("tensors on different devices: cuda:%d and cuda:%d" % (dev, i))
+                dev = i
     return dev
-
-
-class _on:
-    """Makes the tensors' device the current one for a call where it is not; the stream is that device's current stream."""
-    __slots__ = ("dev", "before")
-
-    def __init__(self, dev):
-        self.dev = dev
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.dev:
-            torch.cuda.set_device(self.dev)
-        return torch._C._cuda_getCurrentRawStream(self.dev)
-
-    def __exit__(self, *exc):
-        if self.before != self.dev:
-            torch.cuda.set_device(self.before)
-        return False
 
 
 def _code(t, what):
@@ -267,125 +260,133 @@ def _code(t, what):
 
 
 def _pitch(t, what):
-    """Row pitch in elements of a 2-D tensor whose rows are contiguous."""
-    if t.dim() != 2:
+    """Row pitch in elements of a 2-D tensor whose rows are contiguous and do not overlap."""
+    strides = t.stride()
+    if len(strides) != 2:
         raise ValueError("%s must be two-dimensional, got shape %s" % (what, tuple(t.shape)))
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
-        raise ValueError("the rows of %s must be contiguous, got strides %s" % (what, t.stride()))
+    if strides[1] != 1 and cols > 1:
+        raise ValueError("the rows of %s must be contiguous, got strides %s" % (what, strides))
     if rows <= 1:
         return cols
-    if t.stride(0) < cols:
-        raise ValueError("the rows of %s overlap: strides %s" % (what, t.stride()))
-    return t.stride(0)
+    if strides[0] < cols:
+        raise ValueError("the rows of %s overlap: strides %s" % (what, strides))
+    return strides[0]
 
 
 def _vector(t, n, what):
-    """Address of an optional contiguous float32 vector."""
+    """Address of an optional contiguous float32 vector, 0 for None."""
     if t is None:
-        return None
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        return 0
+    if t.dtype is not torch.float32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError("%s must be a contiguous float32 vector of %d elements, got %s %s" % (what, n, t.dtype, tuple(t.shape)))
     return t.data_ptr()
 
 
-def _rows_or_copy(t):
-    """t, or a copy of it, with contiguous rows that do not overlap (incoming gradients may be expanded)."""
-    if t is None or ((t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])):
-        return t
-    return t.contiguous()
+def _gradient_rows(t, like_shape, like_type, what):
+    """(tensor, pitch) of an optional incoming gradient: t itself, or a copy where its rows are not contiguous or overlap (expanded)."""
+    if t is None:
+        return None, 0
+    if t.shape != like_shape or t.dtype is not like_type:
+        raise ValueError("%s must be %s %s, got %s %s" % (what, like_type, tuple(like_shape), t.dtype, tuple(t.shape)))
+    (rows, cols), (s0, s1) = like_shape, t.stride()
+    if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1):
+        t = t.contiguous()
+        return t, cols
+    return t, (s0 if rows > 1 else cols)
 
 
-def _residual_norm_args(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps):
-    a = _lib.ResidualNormArgs()
-    a.x, a.ldx, a.stream_dtype = x.data_ptr(), _pitch(x, "x"), _code(x, "x")
-    M, D = x.shape
-    a.M, a.D = M, D
-    a.dtype = a.stream_dtype
+def _norm_inputs(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps):
+    """(M, D, type of y, the fields of adcdiff_residual_norm_args up to eps)"""
+    ldx, stream_code = _pitch(x, "x"), _code(x, "x")
+    M, D = shape = x.shape
     if h is not None:
-        if h.shape != x.shape:
-            raise ValueError("h %s and x %s differ in shape" % (tuple(h.shape), tuple(x.shape)))
-        a.h, a.ldh, a.dtype = h.data_ptr(), _pitch(h, "h"), _code(h, "h")
+        if h.shape != shape:
+            raise ValueError("h %s and x %s differ in shape" % (tuple(h.shape), tuple(shape)))
+        hp, ldh, code = h.data_ptr(), _pitch(h, "h"), _code(h, "h")
     elif gate is not None or post_norm or residual_scale != 1.0:
         raise ValueError("a gate, a post norm or a residual scale needs h")
+    else:
+        hp, ldh, code = 0, 0, stream_code
+    gp = ldg = gate_code = gate_rows = 0
     if gate is not None:
-        if gate.dim() != 2 or gate.shape[1] != D or (M > 0 and (gate.shape[0] < 1 or M % gate.shape[0] != 0)):
+        gate_rows = gate.shape[0]
+        if gate.dim() != 2 or gate.shape[1] != D or (M > 0 and (gate_rows < 1 or M % gate_rows != 0)):
             raise ValueError("gate must be [G, %d] with G dividing %d rows, got %s" % (D, M, tuple(gate.shape)))
-        a.gate, a.gate_rows, a.gate_dtype = gate.data_ptr(), gate.shape[0], _code(gate, "gate")
-        if gate.shape[0] > 1 and gate.stride(0) == 0 and (D <= 1 or gate.stride(1) == 1):
-            a.ldg = 0                    # one row expanded over the groups
+        gp, gate_code = gate.data_ptr(), _code(gate, "gate")
+        if gate_rows > 1 and gate.stride(0) == 0 and (D <= 1 or gate.stride(1) == 1):
+            ldg = 0                    # one row expanded over the groups
         else:
-            a.ldg = _pitch(gate, "gate")
+            ldg = _pitch(gate, "gate")
     if not post_norm and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight / post_bias without a post norm")
     if not pre_norm and (pre_weight is not None or pre_bias is not None):
         raise ValueError("pre_weight / pre_bias without a pre norm")
-    a.post_norm, a.pre_norm = post_norm, pre_norm
-    a.post_weight, a.post_bias = _vector(post_weight, D, "post_weight"), _vector(post_bias, D, "post_bias")
-    a.pre_weight, a.pre_bias = _vector(pre_weight, D, "pre_weight"), _vector(pre_bias, D, "pre_bias")
-    a.residual_scale, a.eps = residual_scale, eps
-    return a
+    return M, D, code, (M, D, code, stream_code, gate_code, post_norm, pre_norm, gate_rows, hp, ldh, x.data_ptr(), ldx, gp, ldg,
+                        _vector(post_weight, D, "post_weight"), _vector(post_bias, D, "post_bias"), _vector(pre_weight, D, "pre_weight"),
+                        _vector(pre_bias, D, "pre_bias"), residual_scale, eps)
 
 
 def _raw_residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x, with_stats):
     """adcdiff_residual_norm: [x_new where with_x] + [y where pre_norm] + [stats [M, 4] where with_stats]."""
-    dev = _device_of(h, x, gate, post_weight, post_bias, pre_weight, pre_bias)
-    a = _residual_norm_args(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps)
-    outs = []
+    dev = _device_of(x, h, gate, post_weight, post_bias, pre_weight, pre_bias)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _raw_residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x, with_stats)
+    M, D, _, fields = _norm_inputs(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps)
+    outs, xp, yp, sp = [], 0, 0, 0
     if with_x:
-        o = torch.empty((a.M, a.D), device=x.device, dtype=x.dtype)
-        a.x_new, a.ldx_new = o.data_ptr(), a.D
+        o = x.new_empty((M, D))
+        xp = o.data_ptr()
         outs.append(o)
     if pre_norm:
-        o = torch.empty((a.M, a.D), device=x.device, dtype=_TYPES[a.dtype])
-        a.y, a.ldy = o.data_ptr(), a.D
+        o = (x if h is None else h).new_empty((M, D))
+        yp = o.data_ptr()
         outs.append(o)
     if with_stats:
-        o = torch.empty((a.M, 4), device=x.device, dtype=torch.float32)
-        a.stats = o.data_ptr()
+        o = x.new_empty((M, 4), dtype=torch.float32)
+        sp = o.data_ptr()
         outs.append(o)
-    with _on(dev) as stream:
-        check(_lib.load().adcdiff_residual_norm(C.byref(a), stream))
+    check(_lib.load().adcdiff_residual_norm(_pack_norm_args(*fields, xp, D, yp, D, sp), _stream_of(dev)))
     return outs
 
 
 def _raw_residual_norm_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y, post_norm, pre_norm, residual_scale,
                                 eps, need):
     """adcdiff_residual_norm_backward: the gradients of (h, x, gate, post_weight, post_bias, pre_weight, pre_bias) that `need` asks for."""
-    dev = _device_of(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y)
-    a = _residual_norm_args(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps)
+    dev = _device_of(x, h, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _raw_residual_norm_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y, post_norm, pre_norm,
+                                               residual_scale, eps, need)
+    M, D, code, fields = _norm_inputs(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps)
     given = (h, x, gate, post_weight, post_bias, pre_weight, pre_bias)
-    if len(need) != 7 or any(n and t is None for n, t in zip(need, given)):
-        raise ValueError("need asks for the gradient of an input that is not there")
+    if len(need) != 7:
+        raise ValueError("need has one entry for each of the seven inputs")
+    sp = 0
     if post_norm or pre_norm:
-        if stats is None or stats.dtype != torch.float32 or stats.shape != (a.M, 4) or not stats.is_contiguous():
-            raise ValueError("stats must be the contiguous float32 [%d, 4] tensor of the forward pass" % a.M)
-        a.stats = stats.data_ptr()
-    g = _lib.ResidualNormGrads()
-    for t, like, name in ((d_x_new, x.dtype, "d_x_new"), (d_y, _TYPES[a.dtype], "d_y")):
-        if t is not None and (t.shape != x.shape or t.dtype != like):
-            raise ValueError("%s must be %s %s, got %s %s" % (name, like, tuple(x.shape), t.dtype, tuple(t.shape)))
-    d_x_new, d_y = _rows_or_copy(d_x_new), _rows_or_copy(d_y)
-    if d_x_new is not None:
-        g.d_x_new, g.ld_d_x_new = d_x_new.data_ptr(), _pitch(d_x_new, "d_x_new")
-    if d_y is not None:
-        g.d_y, g.ld_d_y = d_y.data_ptr(), _pitch(d_y, "d_y")
-    outs = []
-    for i, name in enumerate(("h", "x", "gate")):
-        if need[i]:
-            o = torch.empty(given[i].shape, device=x.device, dtype=given[i].dtype)
-            setattr(g, name, o.data_ptr())
-            setattr(g, "ld_" + name, a.D)
+        if stats is None or stats.dtype is not torch.float32 or stats.shape != (M, 4) or not stats.is_contiguous():
+            raise ValueError("stats must be the contiguous float32 [%d, 4] tensor of the forward pass" % M)
+        sp = stats.data_ptr()
+    d_x_new, ld_dx = _gradient_rows(d_x_new, x.shape, x.dtype, "d_x_new")
+    d_y, ld_dy = _gradient_rows(d_y, x.shape, _TYPES[code], "d_y")
+    outs, at = [], []
+    for t, n in zip(given, need):
+        if n:
+            if t is None:
+                raise ValueError("need asks for the gradient of an input that is not there")
+            o = t.new_empty(t.shape)
             outs.append(o)
-    for i, name in enumerate(("post_weight", "post_bias", "pre_weight", "pre_bias")):
-        if need[3 + i]:
-            o = torch.empty((a.D,), device=x.device, dtype=torch.float32)
-            setattr(g, name, o.data_ptr())
-            outs.append(o)
+            at.append(o.data_ptr())
+        else:
+            at.append(0)
+    args = _pack_norm_args(*fields, 0, D, 0, D, sp)
+    grads = _pack_norm_grads(0 if d_x_new is None else d_x_new.data_ptr(), ld_dx, 0 if d_y is None else d_y.data_ptr(), ld_dy, at[0], D, at[1], D, at[2], D,
+                             at[3], at[4], at[5], at[6])
     lib = _lib.load()
-    with _on(dev) as stream:
-        ws = torch.empty(lib.adcdiff_residual_norm_backward_workspace_bytes(C.byref(a), C.byref(g)), device=x.device, dtype=torch.uint8)
-        check(lib.adcdiff_residual_norm_backward(C.byref(a), C.byref(g), ws.data_ptr(), ws.numel(), stream))
+    need_bytes = lib.adcdiff_residual_norm_backward_workspace_bytes(args, grads)
+    ws = x.new_empty((need_bytes,), dtype=torch.uint8)
+    check(lib.adcdiff_residual_norm_backward(args, grads, ws.data_ptr(), need_bytes, _stream_of(dev)))
     return outs
 
 
@@ -403,60 +404,84 @@ def _dense(t):
     return True
 
 
+def _same_device(tensors):
+    devices = set(map(torch.Tensor.get_device, tensors))
+    if len(devices) != 1 or -1 in devices:
+        _need_gpu(*tensors)
+        raise ValueError("gradients on different devices")
+    return devices.pop()
+
+
+def _codes_of(tensors, what):
+    """Type codes of the tensors: one number where they are all alike, else a list."""
+    types = set(map(_dtype_of, tensors))
+    for t in types:
+        if t not in _CODES:
+            raise ValueError("%s must be float32 or bfloat16, got %s" % (what, t))
+    return _CODES[types.pop()] if len(types) == 1 else [_CODES[t.dtype] for t in tensors]
+
+
 def _grad_table(grads, out):
-    """(device, host array of adcdiff_grad_tensor)"""
-    dev, rows = -2, []
-    for i, g in enumerate(grads):
-        o = g if out is None else out[i]
-        if not g.is_cuda or not o.is_cuda:
-            _need_gpu(g, o)
-        if g.get_device() != dev:
-            if dev != -2:
-                raise ValueError("gradients on different devices")
-            dev = g.get_device()
-        if not g.is_contiguous() and not _dense(g):
-            raise ValueError("gradient %d has gaps or overlaps in memory: shape %s, strides %s" % (i, tuple(g.shape), g.stride()))
-        code = _code(g, "gradients")
-        if o is not g:
-            if o.get_device() != dev or o.shape != g.shape or o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
-                raise ValueError("output %d must be like its gradient in device, shape and strides" % i)
-            rows += (g.data_ptr(), o.data_ptr(), g.numel(), code | _code(o, "outputs") << 32)
-        else:
-            p = g.data_ptr()
-            rows += (p, p, g.numel(), code | code << 32)
-    return dev, (C.c_longlong * max(len(rows), 1))(*rows)
+    """(device, host array of adcdiff_grad_tensor): four 64-bit words for each tensor, the two types in the last"""
+    n = len(grads)
+    dev = _same_device(grads)
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        for i, g in enumerate(grads):
+            if not _dense(g):
+                raise ValueError("gradient %d has gaps or overlaps in memory: shape %s, strides %s" % (i, tuple(g.shape), g.stride()))
+    rows = array.array("q", bytes(32 * n))
+    pointers = array.array("q", map(torch.Tensor.data_ptr, grads))
+    codes = _codes_of(grads, "gradients")
+    rows[0::4], rows[2::4] = pointers, array.array("q", map(torch.Tensor.numel, grads))
+    if out is None:
+        rows[1::4], out_codes = pointers, codes
+    else:
+        if _same_device(out) != dev:
+            raise ValueError("gradients and outputs on different devices")
+        for i, (g, o) in enumerate(zip(grads, out)):
+            if o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
+                raise ValueError("output %d must be like its gradient in shape and strides" % i)
+        rows[1::4], out_codes = array.array("q", map(torch.Tensor.data_ptr, out)), _codes_of(out, "outputs")
+    if type(codes) is int and type(out_codes) is int:
+        rows[3::4] = array.array("q", [codes | out_codes << 32]) * n
+    else:
+        codes, out_codes = ([c] * n if type(c) is int else c for c in (codes, out_codes))
+        rows[3::4] = array.array("q", [c | o << 32 for c, o in zip(codes, out_codes)])
+    return dev, rows
 
 
 def _raw_grad_norm(grads, norm_type, max_norm=None, out=None):
     """adcdiff_grad_norm, or adcdiff_clip_grad_norm with a max_norm: the norm, a float32 scalar on the gradients' device."""
     dev, table = _grad_table(grads, out)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _raw_grad_norm(grads, norm_type, max_norm, out)
     lib = _lib.load()
-    n = len(grads)
-    need = lib.adcdiff_grad_norm_workspace_bytes(table, n)
-    device = torch.device("cuda", dev)
-    norm = torch.empty((), device=device, dtype=torch.float32)
-    ws = torch.empty(need, device=device, dtype=torch.uint8)
-    with _on(dev) as stream:
-        if max_norm is None:
-            check(lib.adcdiff_grad_norm(table, n, norm_type, norm.data_ptr(), ws.data_ptr(), need, stream))
-        else:
-            check(lib.adcdiff_clip_grad_norm(table, n, norm_type, max_norm, norm.data_ptr(), ws.data_ptr(), need, stream))
-            # the library wrote the tensors behind torch's back
-            torch.autograd.graph.increment_version(grads if out is None else out)
+    n, at = len(grads), table.buffer_info()[0]
+    need = lib.adcdiff_grad_norm_workspace_bytes(at, n)
+    norm = grads[0].new_empty((), dtype=torch.float32)
+    ws = grads[0].new_empty((need,), dtype=torch.uint8)
+    if max_norm is None:
+        check(lib.adcdiff_grad_norm(at, n, norm_type, norm.data_ptr(), ws.data_ptr(), need, _stream_of(dev)))
+    else:
+        check(lib.adcdiff_clip_grad_norm(at, n, norm_type, max_norm, norm.data_ptr(), ws.data_ptr(), need, _stream_of(dev)))
+        torch.autograd.graph.increment_version(grads if out is None else out)    # the library wrote the tensors behind torch's back
     return norm
 
 
 def _raw_quantize_rows(x):
     dev = _device_of(x)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _raw_quantize_rows(x)
     code, ldx = _code(x, "x"), _pitch(x, "x")
     M, K = x.shape
     if K < 1:
         raise ValueError("rows of no columns have no scale")
     pitch = (K + 15) // 16 * 16
-    q = torch.empty((M, pitch), device=x.device, dtype=torch.int8)
-    scale = torch.empty((M,), device=x.device, dtype=torch.float32)
-    with _on(dev) as stream:
-        check(_lib.load().adcdiff_quantize_rows(x.data_ptr(), ldx, code, M, K, q.data_ptr(), pitch, scale.data_ptr(), stream))
+    q = x.new_empty((M, pitch), dtype=torch.int8)
+    scale = x.new_empty((M,), dtype=torch.float32)
+    check(_lib.load().adcdiff_quantize_rows(x.data_ptr(), ldx, code, M, K, q.data_ptr(), pitch, scale.data_ptr(), _stream_of(dev)))
     return (q if pitch == K else q[:, :K]), scale
 
 
@@ -467,14 +492,17 @@ def _i8_rows(t, what, stream):
     pitch = (K + 15) // 16 * 16
     if t.data_ptr() % 16 == 0 and (ld % 16 == 0 or M <= 1):
         return t, (ld if M > 1 else pitch)
-    o = torch.empty((M, pitch), device=t.device, dtype=torch.int8)
+    o = t.new_empty((M, pitch))
     check(_lib.load().adcdiff_pitch_rows_i8(t.data_ptr(), ld, M, K, o.data_ptr(), pitch, stream))
     return o, pitch
 
 
 def _raw_gemm_int8(a, a_scale, w, w_scale, bias, residual, act, out_dtype):
     dev = _device_of(a, a_scale, w, w_scale, bias, residual)
-    if a.dtype != torch.int8 or w.dtype != torch.int8:
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _raw_gemm_int8(a, a_scale, w, w_scale, bias, residual, act, out_dtype)
+    if a.dtype is not torch.int8 or w.dtype is not torch.int8:
         raise ValueError("a and w must be int8, got %s and %s" % (a.dtype, w.dtype))
     if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
         raise ValueError("a [M, K] and w [N, K] do not fit: %s, %s" % (tuple(a.shape), tuple(w.shape)))
@@ -482,23 +510,21 @@ def _raw_gemm_int8(a, a_scale, w, w_scale, bias, residual, act, out_dtype):
     N = w.shape[0]
     if K < 1 or N < 1:
         raise ValueError("no columns: a %s, w %s" % (tuple(a.shape), tuple(w.shape)))
-    out = torch.empty((M, N), device=a.device, dtype=_TYPES[out_dtype])
-    p = _lib.GemmI8Args()
-    p.M, p.N, p.K, p.act, p.out_dtype = M, N, K, act, out_dtype
-    p.a_scale, p.w_scale, p.bias = _vector(a_scale, M, "a_scale"), _vector(w_scale, N, "w_scale"), _vector(bias, N, "bias")
+    scales = _vector(a_scale, M, "a_scale"), _vector(w_scale, N, "w_scale"), _vector(bias, N, "bias")
+    out = a_scale.new_empty((M, N), dtype=_TYPES[out_dtype])
+    res, ldr = 0, 0
     if residual is not None:
-        if residual.shape != (M, N) or residual.dtype != out.dtype:
+        if residual.shape != (M, N) or residual.dtype is not out.dtype:
             raise ValueError("residual must be %s %s, got %s %s" % (out.dtype, (M, N), residual.dtype, tuple(residual.shape)))
-        p.residual, p.ldr = residual.data_ptr(), _pitch(residual, "residual")
-    p.out, p.ldo = out.data_ptr(), N
+        res, ldr = residual.data_ptr(), _pitch(residual, "residual")
+    stream = _stream_of(dev)
+    a, lda = _i8_rows(a, "a", stream)
+    w, ldw = _i8_rows(w, "w", stream)
     lib = _lib.load()
-    with _on(dev) as stream:
-        a, p.lda = _i8_rows(a, "a", stream)
-        w, p.ldw = _i8_rows(w, "w", stream)
-        p.a, p.w = a.data_ptr(), w.data_ptr()
-        need = lib.adcdiff_gemm_i8_workspace_bytes(M, N, K)
-        ws = torch.empty(need, device=out.device, dtype=torch.uint8) if need else None
-        check(lib.adcdiff_gemm_i8(C.byref(p), ws.data_ptr() if need else None, need, stream))
+    need = lib.adcdiff_gemm_i8_workspace_bytes(M, N, K)
+    ws = a.new_empty((need,)) if need else None
+    check(lib.adcdiff_gemm_i8(_pack_gemm_i8(M, N, K, a.data_ptr(), lda, w.data_ptr(), ldw, *scales, res, ldr, act, out_dtype, out.data_ptr(), N),
+                              ws.data_ptr() if need else 0, need, stream))
     return out
 
 
@@ -606,8 +632,6 @@ def _norm_code(norm, what):
 
 
 def _residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x):
-    from . import torch_ops  # noqa: F401
-    _need_gpu(h, x, gate, post_weight, post_bias, pre_weight, pre_bias)
     args = (h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, float(residual_scale), float(eps), with_x)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:7]):
         return _ResidualNorm.apply(*args)
@@ -659,16 +683,16 @@ def _as_list(tensors):
     return tensors
 
 
+@torch.no_grad()
 def grad_norm(grads, norm_type=2.0):
     """The norm over all elements of all gradient tensors (float32 and bfloat16, any shapes without gaps in memory): a float32 scalar on
     their device.  norm_type 2 (squares summed in float64, so nothing overflows on the way) or inf (largest magnitude).  No
     synchronisation, the same bits every run; NaN if any element is.  An empty list has norm 0, on the CPU."""
-    from . import torch_ops  # noqa: F401
     grads, code = _as_list(grads), _norm_type(norm_type)
-    _need_gpu(*grads)
     return torch.ops.adcdiff.grad_norm(grads, code) if grads else torch.zeros(())
 
 
+@torch.no_grad()
 def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, out=None):
     """Scales the gradient tensors by min(1, max_norm / (norm + 1e-6)) and returns their norm before that (see grad_norm).
 
@@ -676,7 +700,6 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, ou
     the scaled gradients go there and `grads` stay.  Tensors that are written must not overlap one another or another gradient.
     A norm that is not finite is handled as torch.nn.utils.clip_grad_norm_ does: NaN gradients from a NaN norm, zeros (and NaN for the
     infinite elements) from an infinite one; error_if_nonfinite raises before anything is written, at the price of a synchronisation."""
-    from . import torch_ops  # noqa: F401
     grads, code, max_norm = _as_list(grads), _norm_type(norm_type), float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("max_norm must not be negative or NaN, got %r" % max_norm)
@@ -686,7 +709,6 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, ou
             raise ValueError("%d outputs for %d gradients" % (len(out), len(grads)))
     if not grads:
         return torch.zeros(())
-    _need_gpu(*grads)
     if error_if_nonfinite and not bool(torch.isfinite(grad_norm(grads, norm_type))):
         raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
     if out is None:
@@ -694,30 +716,45 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, ou
     return torch.ops.adcdiff.clip_grad_norm_out(grads, max_norm, code, out)
 
 
+class _Ungraded(torch.autograd.Function):
+    """A call whose result has no gradient: asking for one raises instead of leaving it out."""
+
+    @staticmethod
+    def forward(ctx, op, *args):
+        outs = op(*args)
+        if isinstance(outs, tuple):
+            ctx.mark_non_differentiable(outs[0])     # 8-bit codes
+        return outs
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the 8-bit integer layer has no gradient: it serves trained weights")
+
+
+def _ungraded(op, *args):
+    if torch.is_grad_enabled():
+        for t in args:
+            if torch.is_tensor(t) and t.requires_grad:
+                return _Ungraded.apply(op, *args)
+    return op(*args)
+
+
 def quantize_rows(x):
     """(codes int8 [M, K], scale float32 [M]) of the rows of x [M, K] (float32 or bfloat16): scale = max|row| / 127, codes =
     row / scale rounded half to even, exactly.  For activations (a scale per token) and weights [N, K] (a scale per output channel)
     alike.  The codes' rows start on 16-byte boundaries, as gemm_int8 reads them.  A row of zeros has scale 0; a row with a NaN or an
     infinity has scale NaN, so that every product with it is NaN."""
-    from . import torch_ops  # noqa: F401
-    _need_gpu(x)
-    return torch.ops.adcdiff.quantize_rows(x)
+    return _ungraded(torch.ops.adcdiff.quantize_rows, x)
 
 
 def gemm_int8(a, a_scale, w, w_scale, bias=None, residual=None, act=0, out_dtype="bf16"):
     """act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n] + residual[m, n]) for int8 a [M, K] and w [N, K], float32 scales and
     bias, residual [M, N] in out_dtype; act 0 none, 1 SiLU.  The sum is exact (K up to 131071).  Codes whose rows do not start on
     16-byte boundaries are copied to such rows on every call: keep weights as quantize_rows returns them."""
-    from . import torch_ops  # noqa: F401
-    code = dtype_code(out_dtype)
-    _need_gpu(a, a_scale, w, w_scale, bias, residual)
-    return torch.ops.adcdiff.gemm_int8(a, a_scale, w, w_scale, bias, residual, int(act), code)
+    return _ungraded(torch.ops.adcdiff.gemm_int8, a, a_scale, w, w_scale, bias, residual, int(act), dtype_code(out_dtype))
 
 
 def linear_int8(x, w, w_scale, bias=None, residual=None, act=0, out_dtype="bf16"):
     """The 8-bit integer form of a linear layer: the rows of x [M, K] (float32 or bfloat16) are quantised as by quantize_rows and
-    multiplied with the codes w [N, K] (see gemm_int8).  For inference: it has no gradient."""
-    from . import torch_ops  # noqa: F401
-    code = dtype_code(out_dtype)
-    _need_gpu(x, w, w_scale, bias, residual)
-    return torch.ops.adcdiff.linear_int8(x, w, w_scale, bias, residual, int(act), code)
+    multiplied with the codes w [N, K] (see gemm_int8).  For inference: it has no gradient, and asking for one raises."""
+    return _ungraded(torch.ops.adcdiff.linear_int8, x, w, w_scale, bias, residual, int(act), dtype_code(out_dtype))

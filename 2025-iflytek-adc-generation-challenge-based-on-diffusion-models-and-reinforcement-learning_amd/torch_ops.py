@@ -258,6 +258,7 @@ def _define(schema, impl, fake):
     name = schema[:schema.index("(")]
     _fragment.define(schema, tags=(torch.Tag.pt2_compliant_tag,))
     _fragment.impl(name, impl, "CUDA")
+    _fragment.impl(name, impl, "CPU")        # refuses: the wrappers in ops.py raise for tensors that are not on a GPU
     torch.library.register_fake("adcdiff::" + name, fake, lib=_fragment)
     getattr(torch.ops.adcdiff, name)     # listed by names()
 

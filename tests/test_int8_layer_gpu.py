@@ -264,6 +264,15 @@ def test_refusals():
         ops.gemm_int8(a, sa, w, sw, act=3)
 
 
+def test_gradients_are_refused():
+    x = torch.randn(5, 40, device="cuda", requires_grad=True)
+    w, sw = ops.quantize_rows(torch.randn(7, 40, device="cuda"))
+    for y in (ops.linear_int8(x, w, sw), ops.quantize_rows(x)[1], ops.gemm_int8(w, sw, w, sw, bias=torch.zeros(7, device="cuda", requires_grad=True))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            y.sum().backward()
+    assert torch.equal(ops.linear_int8(x, w, sw).detach(), ops.linear_int8(x.detach(), w, sw))
+
+
 def test_operator_schemas():
     x = torch.randn(5, 40, device="cuda")
     q, s = ops.quantize_rows(x)
