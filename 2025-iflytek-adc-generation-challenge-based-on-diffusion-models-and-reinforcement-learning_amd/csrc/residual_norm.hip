@@ -34,88 +34,140 @@ struct ResNormGradParams {
     int group_rows;               // rows of one gate row (M where the gate's gradient is not summed over rows)
 };
 
-template <bool VEC, int TPR, int E>
-__device__ __forceinline__ void load_gate(const void* gate, int bf16, long long offset, int t, int D, float (&v)[E]) {
-    if (bf16) load_row<bf16_t, VEC, TPR, E>(static_cast<const bf16_t*>(gate) + offset, t, D, v);
-    else load_row<float, VEC, TPR, E>(static_cast<const float*>(gate) + offset, t, D, v);
+// A gate row of either type
+template <bool VEC, int TPR>
+struct RawGate {
+    RawRow<float, VEC, TPR> f;
+    __device__ __forceinline__ void clear() { f.clear(); }
+    __device__ __forceinline__ void load(const void* gate, int bf16, long long offset, int t, int D) {
+        if (bf16) {
+            RawRow<bf16_t, VEC, TPR> b;
+            b.load(static_cast<const bf16_t*>(gate) + offset, t, D);
+#pragma unroll
+            for (int i = 0; i < RawRow<bf16_t, VEC, TPR>::N; ++i) f.r[i] = b.r[i];
+        } else {
+            f.load(static_cast<const float*>(gate) + offset, t, D);
+        }
+    }
+    __device__ __forceinline__ void get(int bf16, float (&v)[8]) const {
+        if (bf16) {
+            RawRow<bf16_t, VEC, TPR> b;
+#pragma unroll
+            for (int i = 0; i < RawRow<bf16_t, VEC, TPR>::N; ++i) b.r[i] = f.r[i];
+            b.get(v);
+        } else {
+            f.get(v);
+        }
+    }
+};
+
+// a weight or bias, or what it is without one
+template <bool VEC, int TPR>
+__device__ __forceinline__ void load_vector(const float* p, float absent, int t, int D, float (&v)[8]) {
+    RawRow<float, VEC, TPR> r;
+    r.clear();
+    if (p) r.load(p, t, D);
+    r.get(v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = p ? v[e] : absent;
 }
 
-// mean and 1 / sqrt(variance + eps) of the row in v (mean = 0 for the rms norm); what stands in columns >= D is left out
-template <bool VEC, int TPR, int E, typename Sum>
-__device__ __forceinline__ void row_stats(const float (&v)[E], int kind, int t, int tid, int D, float inv_d, float eps, Sum& sum, float& mean, float& inv) {
+// bit e: element e of the thread lies inside the row
+template <bool VEC, int TPR>
+__device__ __forceinline__ unsigned inside(int t, int D) {
+    if constexpr (VEC) return t * 8 < D ? 0xffu : 0u;
+    unsigned m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m |= e * TPR + t < D ? 1u << e : 0u;
+    return m;
+}
+
+// mean and 1 / sqrt(variance + eps) of the row in v (mean = 0 for the rms norm); elements outside the row are left out
+template <typename Sum>
+__device__ __forceinline__ void row_stats(const float (&v)[8], int kind, unsigned in, int tid, float inv_d, float eps, Sum& sum, float& mean, float& inv) {
     float s[1] = {0.0f};
     mean = 0.0f;
     if (kind == 2) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[0] += column<VEC, TPR>(t, e) < D ? v[e] : 0.0f;
+        for (int e = 0; e < 8; ++e) s[0] += in >> e & 1 ? v[e] : 0.0f;
         sum(s, tid);
         mean = s[0] * inv_d;
         s[0] = 0.0f;
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float c = column<VEC, TPR>(t, e) < D ? v[e] - mean : 0.0f;
+    for (int e = 0; e < 8; ++e) {
+        const float c = in >> e & 1 ? v[e] - mean : 0.0f;
         s[0] = fmaf(c, c, s[0]);
     }
     sum(s, tid);
     inv = 1.0f / sqrtf(fmaf(s[0], inv_d, eps));
 }
 
-template <typename T, typename R, bool VEC, int TPR, int V>
-__global__ __launch_bounds__(kThreads) void residual_norm_kernel(const ResNormParams p) {
-    constexpr int E = 8 * V, TEAMS = kThreads / TPR;
-    __shared__ float red[2 * (kThreads / 64)];
-    const int tid = threadIdx.x, t = tid % TPR, D = p.D;
+template <int TPR>
+constexpr int threads_for() { return TPR > kThreads ? TPR : kThreads; }
+
+// A team of TPR threads per row, eight columns per thread; weights, biases and a gate shared by all rows stay in registers over the rows of a
+// workgroup, and the next row is on its way while the one in hand is reduced.
+template <typename T, typename R, bool VEC, int TPR>
+__global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_kernel(const ResNormParams p) {
+    constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
+    __shared__ float red[2 * (THREADS / 64)];
+    const int tid = threadIdx.x, t = tid % TPR, team = tid / TPR, D = p.D;
+    const unsigned in = inside<VEC, TPR>(t, D);
+    const bool one_gate = p.gate && p.gate_share >= p.M, row_gate = p.gate && !one_gate;
+    RawRow<R, VEC, TPR> rx;
+    RawRow<T, VEC, TPR> rh;
+    RawGate<VEC, TPR> rg;
+    rx.clear(); rh.clear(); rg.clear();
+    auto fetch = [&](long long row) __attribute__((always_inline)) {
+        if (row < p.M) {
+            rx.load(static_cast<const R*>(p.x) + row * p.ldx, t, D);
+            if (p.h) rh.load(static_cast<const T*>(p.h) + row * p.ldh, t, D);
+            if (row_gate) rg.load(p.gate, p.gate_bf16, (p.gate_share == 1 ? row : row / p.gate_share) * p.ldg, t, D);
+        }
+    };
+    const long long step = (long long)gridDim.x * TEAMS;
+    fetch((long long)blockIdx.x * TEAMS + team);
+    float post_w[8], post_b[8], pre_w[8], pre_b[8], gate[8];
+    load_vector<VEC, TPR>(p.post_w, 1.0f, t, D, post_w);
+    load_vector<VEC, TPR>(p.post_b, 0.0f, t, D, post_b);
+    load_vector<VEC, TPR>(p.pre_w, 1.0f, t, D, pre_w);
+    load_vector<VEC, TPR>(p.pre_b, 0.0f, t, D, pre_b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gate[e] = 1.0f;
+    if (one_gate) {
+        RawGate<VEC, TPR> g;
+        g.load(p.gate, p.gate_bf16, 0, t, D);
+        g.get(p.gate_bf16, gate);
+    }
     TeamSum<TPR, 1> sum(red);
-    // Teams wider than a wave are one per workgroup, so the barriers inside the sums are met by every thread.
-    for (long long row = (long long)blockIdx.x * TEAMS + tid / TPR; row < p.M; row += (long long)gridDim.x * TEAMS) {
-        float v[E], w[E];
+    // every team of a workgroup makes the same turns: the sums of teams wider than a wave have barriers in them
+    for (long long base = (long long)blockIdx.x * TEAMS; base < p.M; base += step) {
+        const long long row = base + team;
+        const bool live = row < p.M;
+        float v[8], u[8];
+        rx.get(v);
+        rh.get(u);
+        if (row_gate) rg.get(p.gate_bf16, gate);
+        fetch(row + step);
         float post_mean = 0.0f, post_inv = 1.0f, pre_mean = 0.0f, pre_inv = 1.0f;
-        load_row<R, VEC, TPR, E>(static_cast<const R*>(p.x) + row * p.ldx, t, D, v);
         if (p.h) {
-            float u[E];
-            load_row<T, VEC, TPR, E>(static_cast<const T*>(p.h) + row * p.ldh, t, D, u);
             if (p.post) {
-                row_stats<VEC, TPR, E>(u, p.post, t, tid, D, p.inv_d, p.eps, sum, post_mean, post_inv);
+                row_stats(u, p.post, in, tid, p.inv_d, p.eps, sum, post_mean, post_inv);
 #pragma unroll
-                for (int e = 0; e < E; ++e) u[e] = (u[e] - post_mean) * post_inv;
-                if (p.post_w) {
-                    load_row<float, VEC, TPR, E>(p.post_w, t, D, w);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) u[e] *= w[e];
-                }
-                if (p.post_b) {
-                    load_row<float, VEC, TPR, E>(p.post_b, t, D, w);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) u[e] += w[e];
-                }
-            }
-            if (p.gate) {
-                load_gate<VEC, TPR, E>(p.gate, p.gate_bf16, (p.gate_share == 1 ? row : row / p.gate_share) * p.ldg, t, D, w);
-#pragma unroll
-                for (int e = 0; e < E; ++e) u[e] *= w[e];
+                for (int e = 0; e < 8; ++e) u[e] = fmaf((u[e] - post_mean) * post_inv, post_w[e], post_b[e]);
             }
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = fmaf(p.scale, v[e], u[e]);
+            for (int e = 0; e < 8; ++e) v[e] = fmaf(p.scale, v[e], gate[e] * u[e]);
         }
-        if (p.xn) store_row<R, VEC, TPR, E>(static_cast<R*>(p.xn) + row * p.ldxn, t, D, v);
+        if (p.xn && live) store_row<R, VEC, TPR, 8>(static_cast<R*>(p.xn) + row * p.ldxn, t, D, v);
         if (p.pre) {
-            row_stats<VEC, TPR, E>(v, p.pre, t, tid, D, p.inv_d, p.eps, sum, pre_mean, pre_inv);
+            row_stats(v, p.pre, in, tid, p.inv_d, p.eps, sum, pre_mean, pre_inv);
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = (v[e] - pre_mean) * pre_inv;
-            if (p.pre_w) {
-                load_row<float, VEC, TPR, E>(p.pre_w, t, D, w);
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] *= w[e];
-            }
-            if (p.pre_b) {
-                load_row<float, VEC, TPR, E>(p.pre_b, t, D, w);
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] += w[e];
-            }
-            store_row<T, VEC, TPR, E>(static_cast<T*>(p.y) + row * p.ldy, t, D, v);
+            for (int e = 0; e < 8; ++e) v[e] = fmaf((v[e] - pre_mean) * pre_inv, pre_w[e], pre_b[e]);
+            if (live) store_row<T, VEC, TPR, 8>(static_cast<T*>(p.y) + row * p.ldy, t, D, v);
         }
-        if (p.stats && t == 0) *reinterpret_cast<f32x4*>(p.stats + row * 4) = f32x4{post_mean, post_inv, pre_mean, pre_inv};
+        if (p.stats && t == 0 && live) *reinterpret_cast<f32x4*>(p.stats + row * 4) = f32x4{post_mean, post_inv, pre_mean, pre_inv};
     }
 }
 
@@ -127,14 +179,21 @@ __global__ __launch_bounds__(kThreads) void residual_norm_kernel(const ResNormPa
 // its column sums in registers, so weights cost one partial row per workgroup and the gate one row per chunk.  The partial rows are
 // added in a fixed order by column_sum_kernel: no atomics, results do not change from run to run.
 template <typename T, typename R, bool VEC, int TPR>
-__global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads) void residual_norm_grad_kernel(const ResNormGradParams q) {
-    constexpr int E = 8, THREADS = TPR > kThreads ? TPR : kThreads, TEAMS = THREADS / TPR;
+__global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(const ResNormGradParams q) {
+    constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
     __shared__ float red[4 * (THREADS / 64)];
-    __shared__ float joined[TEAMS > 1 ? THREADS * E : 1];
+    __shared__ float joined[TEAMS > 1 ? THREADS * 8 : 1];
     const ResNormParams& p = q.f;
     const int tid = threadIdx.x, t = tid % TPR, team = tid / TPR, D = p.D;
+    const unsigned in = inside<VEC, TPR>(t, D);
     TeamSum<TPR, 2> sum(red);
-    float a_pre_w[E] = {}, a_pre_b[E] = {}, a_post_w[E] = {}, a_post_b[E] = {};
+    float a_pre_w[8] = {}, a_pre_b[8] = {}, a_post_w[8] = {}, a_post_b[8] = {};
+    float post_w[8], post_b[8], pre_w[8];
+    load_vector<VEC, TPR>(p.post_w, 1.0f, t, D, post_w);
+    load_vector<VEC, TPR>(p.post_b, 0.0f, t, D, post_b);
+    load_vector<VEC, TPR>(p.pre_w, 1.0f, t, D, pre_w);
+    const bool row_gate = p.gate && p.gate_share == 1;
+    constexpr bool AHEAD = TPR < 1024;   // the next row's loads under this row's arithmetic; a team of 1024 has 128 registers per thread: none to spare
     const int teams = gridDim.x * TEAMS;
     // Every team of a workgroup makes the same number of turns (barriers inside the sums); turns without a row do nothing.
     for (int c0 = blockIdx.x * TEAMS; c0 < q.chunks; c0 += teams) {
@@ -142,137 +201,131 @@ __global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads) void residual_norm
         const int group = c / q.chunks_per_gate;
         const long long first = (long long)group * q.group_rows + (long long)(c % q.chunks_per_gate) * q.chunk_rows;
         const long long last = c < q.chunks ? min(first + q.chunk_rows, (long long)(group + 1) * q.group_rows) : first;
-        float a_gate[E] = {};
+        RawRow<R, VEC, TPR> rx, rd;
+        RawRow<T, VEC, TPR> rh, ry;
+        RawGate<VEC, TPR> rg;
+        f32x4 rs = {0.0f, 1.0f, 0.0f, 1.0f};
+        rx.clear(); rd.clear(); rh.clear(); ry.clear(); rg.clear();
+        long long gate_row = -1;
+        auto fetch = [&](long long row) __attribute__((always_inline)) {
+            if (row < last) {
+                if (p.post || p.pre) rs = *reinterpret_cast<const f32x4*>(p.stats + row * 4);
+                if (q.d_xn) rd.load(static_cast<const R*>(q.d_xn) + row * q.ld_dxn, t, D);
+                if (p.pre) rx.load(static_cast<const R*>(p.x) + row * p.ldx, t, D);
+                if (p.h) rh.load(static_cast<const T*>(p.h) + row * p.ldh, t, D);
+                if (q.d_y) ry.load(static_cast<const T*>(q.d_y) + row * q.ld_dy, t, D);
+                if (p.gate) {
+                    const long long g = row_gate ? row : row / p.gate_share;
+                    if (g != gate_row) rg.load(p.gate, p.gate_bf16, g * p.ldg, t, D);
+                    gate_row = g;
+                }
+            }
+        };
+        if constexpr (AHEAD) fetch(first);
+        float a_gate[8] = {}, gate[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gate[e] = 1.0f;
         for (int r = 0; r < q.chunk_rows; ++r) {
             const long long row = first + r;
             const bool live = row < last;
-            float d[E], v[E], u[E], w[E], s[2];
-            f32x4 st = {0.0f, 1.0f, 0.0f, 1.0f};
-#pragma unroll
-            for (int e = 0; e < E; ++e) d[e] = v[e] = u[e] = 0.0f;
-            if (live) {
-                if (p.post || p.pre) st = *reinterpret_cast<const f32x4*>(p.stats + row * 4);
-                if (q.d_xn) load_row<R, VEC, TPR, E>(static_cast<const R*>(q.d_xn) + row * q.ld_dxn, t, D, d);
-                if (p.pre) load_row<R, VEC, TPR, E>(static_cast<const R*>(p.x) + row * p.ldx, t, D, v);
-                if (p.h) load_row<T, VEC, TPR, E>(static_cast<const T*>(p.h) + row * p.ldh, t, D, u);
-            }
-            float uhat[E], gate[E];
+            float d[8], v[8], u[8], uhat[8], g[8], s[2];
+            if constexpr (!AHEAD) fetch(row);
+            const f32x4 st = rs;
+            rd.get(d);
+            rx.get(v);
+            rh.get(u);
+            ry.get(g);
+            if (p.gate) rg.get(p.gate_bf16, gate);
+            if constexpr (AHEAD) fetch(row + 1);
             if (p.h) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) gate[e] = 1.0f;
-                if (p.gate && live) load_gate<VEC, TPR, E>(p.gate, p.gate_bf16, (row / p.gate_share) * p.ldg, t, D, gate);
-#pragma unroll
-                for (int e = 0; e < E; ++e) uhat[e] = u[e];
-                if (p.post) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) uhat[e] = u[e] = (u[e] - st[0]) * st[1];
-                    if (p.post_w) {
-                        load_row<float, VEC, TPR, E>(p.post_w, t, D, w);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) u[e] *= w[e];
+                for (int e = 0; e < 8; ++e) {
+                    uhat[e] = u[e];
+                    if (p.post) {
+                        uhat[e] = (u[e] - st[0]) * st[1];
+                        u[e] = fmaf(uhat[e], post_w[e], post_b[e]);
                     }
-                    if (p.post_b) {
-                        load_row<float, VEC, TPR, E>(p.post_b, t, D, w);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) u[e] += w[e];
-                    }
+                    v[e] = fmaf(p.scale, v[e], gate[e] * u[e]);
                 }
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = fmaf(p.scale, v[e], gate[e] * u[e]);
             }
             if (p.pre) {
-                float g[E];
+                s[0] = s[1] = 0.0f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) g[e] = 0.0f;
-                if (live && q.d_y) load_row<T, VEC, TPR, E>(static_cast<const T*>(q.d_y) + row * q.ld_dy, t, D, g);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
+                for (int e = 0; e < 8; ++e) {
                     v[e] = (v[e] - st[2]) * st[3];
                     if (live) {
                         a_pre_w[e] = fmaf(g[e], v[e], a_pre_w[e]);
                         a_pre_b[e] += g[e];
                     }
+                    g[e] *= pre_w[e];
+                    if (in >> e & 1) { s[0] += g[e]; s[1] = fmaf(g[e], v[e], s[1]); }
                 }
-                if (p.pre_w) {
-                    load_row<float, VEC, TPR, E>(p.pre_w, t, D, w);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) g[e] *= w[e];
-                }
-                s[0] = s[1] = 0.0f;
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (column<VEC, TPR>(t, e) < D) { s[0] += g[e]; s[1] = fmaf(g[e], v[e], s[1]); }
                 sum(s, tid);
                 const float m0 = p.pre == 2 ? s[0] * p.inv_d : 0.0f, m1 = s[1] * p.inv_d;
 #pragma unroll
-                for (int e = 0; e < E; ++e) d[e] = fmaf(g[e] - m0 - v[e] * m1, st[3], d[e]);
+                for (int e = 0; e < 8; ++e) d[e] = fmaf(g[e] - m0 - v[e] * m1, st[3], d[e]);
             }
             if (q.d_x && live) {
-                float o[E];
+                float o[8];
 #pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = p.scale * d[e];
-                store_row<R, VEC, TPR, E>(static_cast<R*>(q.d_x) + row * q.ld_dx, t, D, o);
+                for (int e = 0; e < 8; ++e) o[e] = p.scale * d[e];
+                store_row<R, VEC, TPR, 8>(static_cast<R*>(q.d_x) + row * q.ld_dx, t, D, o);
             }
             if (p.h) {
-                if (q.d_gate) {
-                    if (p.gate_share == 1) {
-                        if (live) {
-                            float o[E];
+                if (q.d_gate && live) {
+                    if (row_gate) {
+                        float o[8];
 #pragma unroll
-                            for (int e = 0; e < E; ++e) o[e] = d[e] * u[e];
-                            if (p.gate_bf16) store_row<bf16_t, VEC, TPR, E>(static_cast<bf16_t*>(q.d_gate) + row * q.ld_dg, t, D, o);
-                            else store_row<float, VEC, TPR, E>(static_cast<float*>(q.d_gate) + row * q.ld_dg, t, D, o);
-                        }
-                    } else if (live) {
+                        for (int e = 0; e < 8; ++e) o[e] = d[e] * u[e];
+                        if (p.gate_bf16) store_row<bf16_t, VEC, TPR, 8>(static_cast<bf16_t*>(q.d_gate) + row * q.ld_dg, t, D, o);
+                        else store_row<float, VEC, TPR, 8>(static_cast<float*>(q.d_gate) + row * q.ld_dg, t, D, o);
+                    } else {
 #pragma unroll
-                        for (int e = 0; e < E; ++e) a_gate[e] = fmaf(d[e], u[e], a_gate[e]);
+                        for (int e = 0; e < 8; ++e) a_gate[e] = fmaf(d[e], u[e], a_gate[e]);
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < E; ++e) d[e] *= gate[e];
+                for (int e = 0; e < 8; ++e) d[e] *= gate[e];
                 if (p.post) {
-                    if (live) {
-#pragma unroll
-                        for (int e = 0; e < E; ++e) { a_post_w[e] = fmaf(d[e], uhat[e], a_post_w[e]); a_post_b[e] += d[e]; }
-                    }
-                    if (p.post_w) {
-                        load_row<float, VEC, TPR, E>(p.post_w, t, D, w);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) d[e] *= w[e];
-                    }
                     s[0] = s[1] = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (column<VEC, TPR>(t, e) < D) { s[0] += d[e]; s[1] = fmaf(d[e], uhat[e], s[1]); }
+                    for (int e = 0; e < 8; ++e) {
+                        if (live) {
+                            a_post_w[e] = fmaf(d[e], uhat[e], a_post_w[e]);
+                            a_post_b[e] += d[e];
+                        }
+                        d[e] *= post_w[e];
+                        if (in >> e & 1) { s[0] += d[e]; s[1] = fmaf(d[e], uhat[e], s[1]); }
+                    }
                     sum(s, tid);
                     const float m0 = p.post == 2 ? s[0] * p.inv_d : 0.0f, m1 = s[1] * p.inv_d;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) d[e] = (d[e] - m0 - uhat[e] * m1) * st[1];
+                    for (int e = 0; e < 8; ++e) d[e] = (d[e] - m0 - uhat[e] * m1) * st[1];
                 }
-                if (q.d_h && live) store_row<T, VEC, TPR, E>(static_cast<T*>(q.d_h) + row * q.ld_dh, t, D, d);
+                if (q.d_h && live) store_row<T, VEC, TPR, 8>(static_cast<T*>(q.d_h) + row * q.ld_dh, t, D, d);
             }
         }
-        if (q.d_gate && p.gate_share != 1 && c < q.chunks) {
-            if (q.chunks_per_gate > 1) store_row<float, VEC, TPR, E>(q.gate_partial + (long long)c * D, t, D, a_gate);
-            else if (p.gate_bf16) store_row<bf16_t, VEC, TPR, E>(static_cast<bf16_t*>(q.d_gate) + group * q.ld_dg, t, D, a_gate);
-            else store_row<float, VEC, TPR, E>(static_cast<float*>(q.d_gate) + group * q.ld_dg, t, D, a_gate);
+        if (q.d_gate && !row_gate && c < q.chunks) {
+            if (q.chunks_per_gate > 1) store_row<float, VEC, TPR, 8>(q.gate_partial + (long long)c * D, t, D, a_gate);
+            else if (p.gate_bf16) store_row<bf16_t, VEC, TPR, 8>(static_cast<bf16_t*>(q.d_gate) + group * q.ld_dg, t, D, a_gate);
+            else store_row<float, VEC, TPR, 8>(static_cast<float*>(q.d_gate) + group * q.ld_dg, t, D, a_gate);
         }
     }
     float* out = q.partial + (long long)blockIdx.x * q.vectors * D;
-    auto flush = [&](float (&a)[E], int slot) {
+    auto flush = [&](float (&a)[8], int slot) {
         if (slot < 0) return;
         if constexpr (TEAMS > 1) {
             __syncthreads();
 #pragma unroll
-            for (int e = 0; e < E; ++e) joined[e * THREADS + tid] = a[e];
+            for (int e = 0; e < 8; ++e) joined[e * THREADS + tid] = a[e];
             __syncthreads();
             if (team == 0) {
 #pragma unroll
-                for (int e = 0; e < E; ++e)
+                for (int e = 0; e < 8; ++e)
                     for (int k = 1; k < TEAMS; ++k) a[e] += joined[e * THREADS + k * TPR + t];
             }
         }
-        if (team == 0) store_row<float, VEC, TPR, E>(out + (long long)slot * D, t, D, a);
+        if (team == 0) store_row<float, VEC, TPR, 8>(out + (long long)slot * D, t, D, a);
     };
     flush(a_pre_w, q.slot_pre_w);
     flush(a_pre_b, q.slot_pre_b);
@@ -280,22 +333,30 @@ __global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads) void residual_norm
     flush(a_post_b, q.slot_post_b);
 }
 
-// out[seg][col] = sum over i < count of part[seg * seg_stride + i * row_stride + col], in a fixed order: 32 columns x 32 row groups
-// per workgroup, each thread a strided share of the rows, then a tree over the groups.  Segments 0 .. vectors - 1 are the weight and
-// bias gradients, the others the gate rows.
+// The partial rows added up in a fixed order.  Segments 0 .. vectors - 1 are the weight and bias gradients (a partial row from each
+// workgroup), the others the gate rows (one from each chunk).  Tall sums: a workgroup takes 32 columns of a segment with 32 threads down the rows and
+// a tree over them.  Gate rows of few chunks (flat): a thread takes one element; the tall form would start 1024 threads for every
+// 32 columns of every gate row (64 gate rows of 8 chunks, D = 2048: 13.4 us for 12 MB).
 struct ColumnSumParams {
     const float *partial, *gate_partial;
     float* out[4];
     void* d_gate;
-    long long ld_dg;
-    int D, vectors, segments, workgroups, chunks_per_gate, gate_bf16;
+    long long ld_dg, flat;      // flat: elements summed by single threads (gate rows x D, or 0)
+    int D, vectors, tall, workgroups, chunks_per_gate, gate_bf16;   // tall: segments summed by whole workgroups
 };
+
+__device__ __forceinline__ void store_gate(const ColumnSumParams& p, long long row, int col, float v) {
+    if (p.gate_bf16) static_cast<bf16_t*>(p.d_gate)[row * p.ld_dg + col] = (bf16_t)v;
+    else static_cast<float*>(p.d_gate)[row * p.ld_dg + col] = v;
+}
 
 __global__ __launch_bounds__(1024) void column_sum_kernel(const ColumnSumParams p) {
     __shared__ float part[32][33];
-    const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
-    const int col = blockIdx.x * 32 + cx;
-    for (int seg = blockIdx.y; seg < p.segments; seg += gridDim.y) {
+    const int blocks = (p.D + 31) / 32;
+    const long long tall_blocks = (long long)blocks * p.tall;
+    if (blockIdx.x < tall_blocks) {
+        const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
+        const int seg = blockIdx.x / blocks, col = blockIdx.x % blocks * 32 + cx;
         const bool weight = seg < p.vectors;
         const float* src = weight ? p.partial + (long long)seg * p.D : p.gate_partial + (long long)(seg - p.vectors) * p.chunks_per_gate * p.D;
         const long long step = weight ? (long long)p.vectors * p.D : p.D;
@@ -314,10 +375,19 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const ColumnSumParams 
         }
         if (ry == 0 && col < p.D) {
             if (weight) p.out[seg][col] = part[0][cx];
-            else if (p.gate_bf16) static_cast<bf16_t*>(p.d_gate)[(long long)(seg - p.vectors) * p.ld_dg + col] = (bf16_t)part[0][cx];
-            else static_cast<float*>(p.d_gate)[(long long)(seg - p.vectors) * p.ld_dg + col] = part[0][cx];
+            else store_gate(p, seg - p.vectors, col, part[0][cx]);
         }
-        __syncthreads();
+        return;
+    }
+    const long long stride = (gridDim.x - tall_blocks) * 1024;
+    for (long long e = (blockIdx.x - tall_blocks) * 1024 + threadIdx.x; e < p.flat; e += stride) {
+        const long long row = e / p.D;
+        const int col = (int)(e - row * p.D);
+        const float* src = p.gate_partial + row * p.chunks_per_gate * p.D + col;
+        float s = 0.0f;
+#pragma unroll 8
+        for (int i = 0; i < p.chunks_per_gate; ++i) s += src[(long long)i * p.D];
+        store_gate(p, row, col, s);
     }
 }
 
@@ -363,22 +433,25 @@ bool vector_inputs(const adcdiff_residual_norm_args& a) {
            vector_rows(a.post_weight, 0, 4) && vector_rows(a.post_bias, 0, 4) && vector_rows(a.pre_weight, 0, 4) && vector_rows(a.pre_bias, 0, 4);
 }
 
-template <typename T, typename R, bool VEC, int TPR, int V>
+int team_width(int D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
+
+template <typename T, typename R, bool VEC, int TPR>
 void launch_forward(const ResNormParams& p, hipStream_t stream) {
-    constexpr int teams = kThreads / TPR;
+    constexpr int threads = threads_for<TPR>(), teams = threads / TPR;
     const long long groups = ((long long)p.M + teams - 1) / teams;
-    hipLaunchKernelGGL((residual_norm_kernel<T, R, VEC, TPR, V>), dim3((unsigned)std::min<long long>(groups, 1 << 20)), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((residual_norm_kernel<T, R, VEC, TPR>), dim3((unsigned)std::min<long long>(groups, 2048)), dim3(threads), 0, stream, p);
 }
 
-// The narrowest team that holds the row
 template <typename T, typename R, bool VEC>
 void forward_by_width(const ResNormParams& p, hipStream_t stream) {
-    if (p.D <= 128) launch_forward<T, R, VEC, 16, 1>(p, stream);
-    else if (p.D <= 512) launch_forward<T, R, VEC, 64, 1>(p, stream);
-    else if (p.D <= 1024) launch_forward<T, R, VEC, 64, 2>(p, stream);
-    else if (p.D <= 2048) launch_forward<T, R, VEC, 64, 4>(p, stream);
-    else if (p.D <= 4096) launch_forward<T, R, VEC, 256, 2>(p, stream);
-    else launch_forward<T, R, VEC, 256, 4>(p, stream);
+    switch (team_width(p.D)) {
+        case 16: launch_forward<T, R, VEC, 16>(p, stream); break;
+        case 64: launch_forward<T, R, VEC, 64>(p, stream); break;
+        case 128: launch_forward<T, R, VEC, 128>(p, stream); break;
+        case 256: launch_forward<T, R, VEC, 256>(p, stream); break;
+        case 512: launch_forward<T, R, VEC, 512>(p, stream); break;
+        default: launch_forward<T, R, VEC, 1024>(p, stream); break;
+    }
 }
 
 template <bool VEC>
@@ -398,7 +471,7 @@ struct Cut {
     bool gate_sum;      // the gate's gradient is a sum over rows
 };
 
-int team_width(int D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
+constexpr int kMaxGroups = 512;
 
 Cut cut_rows(int M, int D, int gate_rows, bool gate_grad, int vectors) {
     Cut c{};
@@ -409,13 +482,15 @@ Cut cut_rows(int M, int D, int gate_rows, bool gate_grad, int vectors) {
     const int groups = c.gate_sum ? gate_rows : 1;
     c.group_rows = M / groups;
     if (M == 0) { c.chunks_per_gate = 1; c.chunk_rows = 1; return c; }
-    // about 1024 workgroups' worth of teams, and chunks of at least 8 rows
-    const int workers = 1024 * c.teams;
+    // Two workgroups of 256 threads fit a CU (230 registers per thread): 512 workgroups' worth of teams, and chunks of at least two rows.  More
+    // workgroups write and add more partial rows (1024: column sums of 32768 x 2048 17 us), longer chunks leave few rows waiting on each
+    // other (8 rows: 1003 x 777 24 us).
+    const int workers = kMaxGroups * c.teams;
     const int want = std::max(1, (workers + groups - 1) / groups);
-    c.chunk_rows = std::max(std::min(c.group_rows, 8), (c.group_rows + want - 1) / want);
+    c.chunk_rows = std::max(std::min(c.group_rows, 2), (c.group_rows + want - 1) / want);
     c.chunks_per_gate = (c.group_rows + c.chunk_rows - 1) / c.chunk_rows;
     c.chunks = groups * c.chunks_per_gate;
-    c.workgroups = std::min(1024, (c.chunks + c.teams - 1) / c.teams);
+    c.workgroups = std::min(kMaxGroups, (c.chunks + c.teams - 1) / c.teams);
     return c;
 }
 
@@ -524,10 +599,14 @@ extern "C" int adcdiff_residual_norm_backward(const adcdiff_residual_norm_args* 
     const int gate_segments = g->gate && (a->M == 0 || (c.gate_sum && c.chunks_per_gate > 1)) ? a->gate_rows : 0;
     const int segments = c.vectors + gate_segments;
     s.partial = q.partial; s.gate_partial = q.gate_partial; s.d_gate = g->gate; s.ld_dg = g->ld_gate;
-    s.D = a->D; s.vectors = c.vectors; s.segments = segments; s.workgroups = a->M > 0 ? c.workgroups : 0;
+    s.D = a->D; s.vectors = c.vectors; s.workgroups = a->M > 0 ? c.workgroups : 0;
     s.chunks_per_gate = a->M > 0 ? c.chunks_per_gate : 0; s.gate_bf16 = a->gate_dtype == ADCDIFF_BF16;
     if (segments == 0) return ADCDIFF_OK;
     TimingScope timing(ADCDIFF_KIND_OTHER, segments, a->D, 0, 0.0, 4.0 * workspace_floats(c, a->D), stream);
-    hipLaunchKernelGGL(column_sum_kernel, dim3((a->D + 31) / 32, std::min(segments, 65535)), dim3(1024), 0, stream, s);
+    const bool flat = s.chunks_per_gate <= 32;
+    s.tall = c.vectors + (flat ? 0 : gate_segments);
+    s.flat = flat ? (long long)gate_segments * a->D : 0;
+    const long long blocks = (long long)((a->D + 31) / 32) * s.tall + std::min<long long>((s.flat + 1023) / 1024, 4096);
+    hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)blocks), dim3(1024), 0, stream, s);
     return check_launch("residual_norm_backward: column sums");
 }

@@ -79,6 +79,50 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, int t, int D, const
     }
 }
 
+// Eight elements of a row as they stand in memory: loaded without being looked at, so that the loads of a row ahead stay in flight under the
+// arithmetic of the row in hand.  Columns as in load_row with E = 8; those >= D read as 0.
+template <typename T, bool VEC, int TPR>
+struct RawRow {
+    static constexpr int N = VEC && sizeof(T) == 2 ? 4 : 8;
+    uint32_t r[N];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = 0;
+    }
+    __device__ __forceinline__ void load(const T* __restrict__ p, int t, int D) {
+        if constexpr (VEC) {
+            clear();
+            if (t * 8 < D) {
+#pragma unroll
+                for (int i = 0; i < N / 4; ++i) {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(p + t * 8 + 4 * i);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) r[4 * i + k] = w[k];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int c = e * TPR + t;
+                if constexpr (sizeof(T) == 2) r[e] = c < D ? reinterpret_cast<const uint16_t*>(p)[c] : 0;
+                else r[e] = c < D ? reinterpret_cast<const uint32_t*>(p)[c] : 0;
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __builtin_bit_cast(float, r[e]);
+        } else if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[2 * i] = bf_lo(r[i]); v[2 * i + 1] = bf_hi(r[i]); }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = bf_lo(r[e]);
+        }
+    }
+};
+
 // Sums over a team of TPR threads; every thread receives them.  Teams wider than a wave exchange through `red`, whose two halves
 // alternate, so one barrier per call is enough (a half is written again only behind the barrier of the call in between).
 template <int TPR, int N>
