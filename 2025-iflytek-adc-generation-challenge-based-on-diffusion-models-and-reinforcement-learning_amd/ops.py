@@ -353,7 +353,8 @@ def _raw_residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias,
 
 def _raw_residual_norm_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y, post_norm, pre_norm, residual_scale,
                                 eps, need):
-    """adcdiff_residual_norm_backward: the gradients of (h, x, gate, post_weight, post_bias, pre_weight, pre_bias) that `need` asks for."""
+    """adcdiff_residual_norm_backward: the gradients of (h, x, gate, post_weight, post_bias, pre_weight, pre_bias) that `need` asks for: those of h, x
+    and gate as tensors of their own, those of the vectors as the rows of one float32 tensor behind them."""
     dev = _device_of(x, h, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y)
     if dev != _current_device():
         with torch.cuda.device(dev):
@@ -370,16 +371,20 @@ def _raw_residual_norm_backward(h, x, gate, post_weight, post_bias, pre_weight, 
         sp = stats.data_ptr()
     d_x_new, ld_dx = _gradient_rows(d_x_new, x.shape, x.dtype, "d_x_new")
     d_y, ld_dy = _gradient_rows(d_y, x.shape, _TYPES[code], "d_y")
-    outs, at = [], []
-    for t, n in zip(given, need):
-        if n:
-            if t is None:
-                raise ValueError("need asks for the gradient of an input that is not there")
-            o = t.new_empty(t.shape)
+    outs, at = [], [0] * 7
+    for i in range(3):
+        if need[i]:
+            o = given[i].new_empty(given[i].shape) if given[i] is not None else None
             outs.append(o)
-            at.append(o.data_ptr())
-        else:
-            at.append(0)
+            at[i] = 0 if o is None else o.data_ptr()
+    vectors = [i for i in range(3, 7) if need[i]]
+    if vectors:     # one allocation: at small sizes an allocation costs the host more than the kernels take
+        o = x.new_empty((len(vectors), D), dtype=torch.float32)
+        for k, i in enumerate(vectors):
+            at[i] = o.data_ptr() + 4 * D * k
+        outs.append(o)
+    if any(n and t is None for t, n in zip(given, need)):
+        raise ValueError("need asks for the gradient of an input that is not there")
     args = _pack_norm_args(*fields, 0, D, 0, D, sp)
     grads = _pack_norm_grads(0 if d_x_new is None else d_x_new.data_ptr(), ld_dx, 0 if d_y is None else d_y.data_ptr(), ld_dy, at[0], D, at[1], D, at[2], D,
                              at[3], at[4], at[5], at[6])
@@ -616,13 +621,24 @@ class _ResidualNorm(torch.autograd.Function):
         return (outs[0] if with_x else None), (outs[-2] if pre_norm else None)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_x_new, d_y):
-        need = list(ctx.needs_input_grad[:7])
-        if (d_x_new is None and d_y is None) or not any(need):
-            return (None,) * 12
-        outs = iter(torch.ops.adcdiff.residual_norm_backward(*ctx.saved_tensors, d_x_new, d_y, *ctx.args, need))
-        return tuple(next(outs) if n else None for n in need) + (None,) * 5
+        if torch.is_grad_enabled():         # create_graph: the gradients carry on without a gradient of their own
+            return _residual_norm_backward_once(ctx, d_x_new, d_y)
+        return _residual_norm_backward(ctx, d_x_new, d_y)
+
+
+def _residual_norm_backward(ctx, d_x_new, d_y):
+    need = ctx.needs_input_grad[:7]
+    if d_x_new is None and d_y is None:
+        return (None,) * 12
+    outs = torch.ops.adcdiff.residual_norm_backward.default(*ctx.saved_tensors, d_x_new, d_y, *ctx.args, need)
+    if any(need[3:]):
+        outs[-1:] = outs[-1].unbind(0)
+    outs = iter(outs)
+    return (*[next(outs) if n else None for n in need], None, None, None, None, None)
+
+
+_residual_norm_backward_once = torch.autograd.function.once_differentiable(_residual_norm_backward)
 
 
 def _norm_code(norm, what):

@@ -274,8 +274,9 @@ def _fake_residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias
 
 def _fake_residual_norm_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y, post_norm, pre_norm,
                                  residual_scale, eps, need):
-    given = (h, x, gate, post_weight, post_bias, pre_weight, pre_bias)
-    return [t.new_empty(t.shape) for t, n in zip(given, need) if n]
+    outs = [t.new_empty(t.shape) for t, n in zip((h, x, gate), need) if n]
+    vectors = sum(bool(n) for n in need[3:])
+    return outs + ([x.new_empty((vectors, x.shape[1]), dtype=torch.float32)] if vectors else [])
 
 
 def _fake_quantize_rows(x):
