@@ -12,13 +12,15 @@ namespace adcdiff {
 namespace {
 
 constexpr int kTable = 120;          // tensors per launch: 120 * 32 bytes of kernel arguments
-constexpr long long kChunk = 16384;  // elements of one workgroup
+constexpr long long kChunk = 8192;   // elements of one workgroup: 44 M gradients 42 us (4096: 48, 16384: 44, 65536: 46; 4.2 TB/s, read only)
+constexpr long long kPiece = 2048;   // elements of one wave where a single workgroup does the whole call
+constexpr int kFewPieces = 64;       // up to here: four rounds of loads for its 16 waves, against three launches
 
 struct GradEntry {
     const void* grad;
     void* out;
     long long numel;
-    int first_chunk;                 // among the launch's chunks
+    int first_chunk;                 // among the launch's chunks (or pieces)
     int types;                       // bit 0: grad is bf16, bit 1: out is bf16
 };
 
@@ -67,6 +69,45 @@ __device__ __forceinline__ typename Op::Acc block_join(typename Op::Acc s, typen
     return s;
 }
 
+// A thread's share of a chunk: eight 16-byte loads in flight, then what is left
+template <typename Op, int THREADS, typename In>
+__device__ __forceinline__ typename Op::Acc reduce_chunk(const In* __restrict__ p, int cnt, int tid) {
+    constexpr int W = 16 / sizeof(In), U = 8;
+    typename Op::Acc s = Op::zero();
+    auto add = [&](const u32x4 w) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t bits = w[k];      // (a bit cast of a vector's element itself reads element 0)
+            if constexpr (sizeof(In) == 2) {
+                Op::add(s, bf_lo(bits));
+                Op::add(s, bf_hi(bits));
+            } else {
+                Op::add(s, __builtin_bit_cast(float, bits));
+            }
+        }
+    };
+    int i = tid * W;
+    for (; i + (U - 1) * THREADS * W + W <= cnt; i += U * THREADS * W) {
+        u32x4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = *reinterpret_cast<const u32x4_any*>(p + i + u * THREADS * W);
+#pragma unroll
+        for (int u = 0; u < U; ++u) add(w[u]);
+    }
+    for (; i + W <= cnt; i += THREADS * W) add(*reinterpret_cast<const u32x4_any*>(p + i));
+    for (i = cnt / W * W + tid; i < cnt; i += THREADS) {
+        if constexpr (sizeof(In) == 2) Op::add(s, bf_lo(p[i]));
+        else Op::add(s, p[i]);
+    }
+    return s;
+}
+
+template <typename Op, int THREADS>
+__device__ __forceinline__ typename Op::Acc reduce_part(const GradEntry& d, long long base, int cnt, int tid) {
+    if (d.types & 1) return reduce_chunk<Op, THREADS>(static_cast<const uint16_t*>(d.grad) + base, cnt, tid);
+    return reduce_chunk<Op, THREADS>(static_cast<const float*>(d.grad) + base, cnt, tid);
+}
+
 template <typename Op>
 __global__ __launch_bounds__(256) void grad_partial_kernel(const GradTable g, typename Op::Acc* __restrict__ partial) {
     __shared__ typename Op::Acc red[4];
@@ -74,26 +115,7 @@ __global__ __launch_bounds__(256) void grad_partial_kernel(const GradTable g, ty
     const GradEntry& d = g.t[find_entry(g, blockIdx.x)];
     const long long base = (long long)((int)blockIdx.x - d.first_chunk) * kChunk;
     const int cnt = (int)min(kChunk, d.numel - base);
-    typename Op::Acc s = Op::zero();
-    if (d.types & 1) {
-        const uint16_t* p = static_cast<const uint16_t*>(d.grad) + base;
-#pragma unroll 4
-        for (int i = tid * 8; i + 7 < cnt; i += 2048) {
-            const u32x4 v = *reinterpret_cast<const u32x4_any*>(p + i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) { Op::add(s, bf_lo(v[k])); Op::add(s, bf_hi(v[k])); }
-        }
-        for (int i = (cnt & ~7) + tid; i < cnt; i += 256) Op::add(s, bf_lo(p[i]));
-    } else {
-        const float* p = static_cast<const float*>(d.grad) + base;
-#pragma unroll 4
-        for (int i = tid * 4; i + 3 < cnt; i += 1024) {
-            const f32x4 v = *reinterpret_cast<const f32x4_any*>(p + i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) Op::add(s, v[k]);
-        }
-        for (int i = (cnt & ~3) + tid; i < cnt; i += 256) Op::add(s, p[i]);
-    }
+    typename Op::Acc s = reduce_part<Op, 256>(d, base, cnt, tid);
     s = block_join<Op, 256>(s, red);
     if (tid == 0) partial[blockIdx.x] = s;
 }
@@ -101,7 +123,12 @@ __global__ __launch_bounds__(256) void grad_partial_kernel(const GradTable g, ty
 __device__ __forceinline__ float as_norm(double s) { return (float)sqrt(s); }
 __device__ __forceinline__ float as_norm(uint32_t s) { return __builtin_bit_cast(float, s); }
 
-// norm, and the clipping factor min(1, max_norm / (norm + 1e-6)); a NaN norm gives a NaN factor
+// min(1, max_norm / (norm + 1e-6)); NaN for a NaN norm
+__device__ __forceinline__ float clip_factor(float max_norm, float norm) {
+    const float f = max_norm / (norm + 1e-6f);
+    return f >= 1.0f ? 1.0f : f;
+}
+
 template <typename Op>
 __global__ __launch_bounds__(1024) void grad_total_kernel(const typename Op::Acc* __restrict__ partial, int n, float max_norm, float* __restrict__ norm,
                                                           float* __restrict__ factor) {
@@ -112,24 +139,21 @@ __global__ __launch_bounds__(1024) void grad_total_kernel(const typename Op::Acc
     if (threadIdx.x == 0) {
         const float v = as_norm(s);
         *norm = v;
-        if (factor) {
-            const float f = max_norm / (v + 1e-6f);
-            *factor = f >= 1.0f ? 1.0f : f;
-        }
+        if (factor) *factor = clip_factor(max_norm, v);
     }
 }
 
 // In place p and o are the same memory, so four vectors are loaded before the first is stored: a thread's loads are then in flight
 // together without the compiler having to prove that a store leaves the next load alone.
-template <typename In, typename Out>
-__device__ __forceinline__ void scale_chunk(const In* p, Out* o, int cnt, float f) {
+template <int THREADS, typename In, typename Out>
+__device__ __forceinline__ void scale_chunk(const In* p, Out* o, int cnt, float f, int tid) {
     constexpr int W = sizeof(In) == 2 ? 8 : 4, U = 4;
     const int whole = cnt / W * W;
-    for (int i0 = threadIdx.x * W; i0 < whole; i0 += 256 * W * U) {
+    for (int i0 = tid * W; i0 < whole; i0 += THREADS * W * U) {
         float v[U][W];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * 256 * W;
+            const int i = i0 + u * THREADS * W;
             if (i < whole) {
                 if constexpr (sizeof(In) == 2) {
                     const u32x4 w = *reinterpret_cast<const u32x4_any*>(p + i);
@@ -144,7 +168,7 @@ __device__ __forceinline__ void scale_chunk(const In* p, Out* o, int cnt, float 
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * 256 * W;
+            const int i = i0 + u * THREADS * W;
             if (i < whole) {
                 if constexpr (sizeof(Out) == 4) {
 #pragma unroll
@@ -161,7 +185,21 @@ __device__ __forceinline__ void scale_chunk(const In* p, Out* o, int cnt, float 
             }
         }
     }
-    for (int i = whole + threadIdx.x; i < cnt; i += 256) o[i] = (Out)((float)p[i] * f);
+    for (int i = whole + tid; i < cnt; i += THREADS) o[i] = (Out)((float)p[i] * f);
+}
+
+template <int THREADS>
+__device__ __forceinline__ void scale_part(const GradEntry& d, long long base, int cnt, float f, int tid) {
+    const bf16_t* pb = static_cast<const bf16_t*>(d.grad) + base;
+    const float* pf = static_cast<const float*>(d.grad) + base;
+    bf16_t* ob = static_cast<bf16_t*>(d.out) + base;
+    float* of = static_cast<float*>(d.out) + base;
+    switch (d.types) {
+        case 0: scale_chunk<THREADS>(pf, of, cnt, f, tid); break;
+        case 1: scale_chunk<THREADS>(pb, of, cnt, f, tid); break;
+        case 2: scale_chunk<THREADS>(pf, ob, cnt, f, tid); break;
+        default: scale_chunk<THREADS>(pb, ob, cnt, f, tid); break;
+    }
 }
 
 __global__ __launch_bounds__(256) void grad_scale_kernel(const GradTable g, const float* __restrict__ factor) {
@@ -170,19 +208,34 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const GradTable g, cons
     if (f == 1.0f && d.out == d.grad) return;   // in place: g * 1 is what is there
     const long long base = (long long)((int)blockIdx.x - d.first_chunk) * kChunk;
     const int cnt = (int)min(kChunk, d.numel - base);
-    const bf16_t* pb = static_cast<const bf16_t*>(d.grad) + base;
-    const float* pf = static_cast<const float*>(d.grad) + base;
-    bf16_t* ob = static_cast<bf16_t*>(d.out) + base;
-    float* of = static_cast<float*>(d.out) + base;
-    switch (d.types) {
-        case 0: scale_chunk(pf, of, cnt, f); break;
-        case 1: scale_chunk(pb, of, cnt, f); break;
-        case 2: scale_chunk(pf, ob, cnt, f); break;
-        default: scale_chunk(pb, ob, cnt, f); break;
+    scale_part<256>(d, base, cnt, f, threadIdx.x);
+}
+
+// The whole call in one workgroup, where the gradients are few: a wave takes pieces of kPiece elements, for the norm and again for the scaling.
+template <typename Op>
+__global__ __launch_bounds__(1024) void grad_small_kernel(const GradTable g, int pieces, float max_norm, float* __restrict__ norm, int clip) {
+    __shared__ typename Op::Acc red[16];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    typename Op::Acc s = Op::zero();
+    for (int i = wave; i < pieces; i += 16) {
+        const GradEntry& d = g.t[find_entry(g, i)];
+        const long long base = (long long)(i - d.first_chunk) * kPiece;
+        s = Op::join(s, reduce_part<Op, 64>(d, base, (int)min(kPiece, d.numel - base), lane));
+    }
+    const float v = as_norm(block_join<Op, 1024>(s, red));
+    if (threadIdx.x == 0) *norm = v;
+    const float f = clip_factor(max_norm, v);
+    if (!clip) return;
+    for (int i = wave; i < pieces; i += 16) {
+        const GradEntry& d = g.t[find_entry(g, i)];
+        if (f == 1.0f && d.out == d.grad) continue;
+        const long long base = (long long)(i - d.first_chunk) * kPiece;
+        scale_part<64>(d, base, (int)min(kPiece, d.numel - base), f, lane);
     }
 }
 
-long long chunks_of(long long numel) { return (numel + kChunk - 1) / kChunk; }
+long long parts_of(long long numel, long long part) { return (numel + part - 1) / part; }
+long long chunks_of(long long numel) { return parts_of(numel, kChunk); }
 
 int check_tensors(const char* who, const adcdiff_grad_tensor* ts, int n, bool clip, long long* chunks) {
     if (n < 0 || (n > 0 && !ts)) return fail(ADCDIFF_E_BADARG, "%s: null table or %d tensors", who, n);
@@ -225,7 +278,7 @@ int check_overlap(const adcdiff_grad_tensor* ts, int n) {
 
 // Calls launch(table, chunks of the table, chunks before it) for the tensors in groups of kTable
 template <typename F>
-void for_tables(const adcdiff_grad_tensor* ts, int n, F launch) {
+void for_tables(const adcdiff_grad_tensor* ts, int n, long long part, F launch) {
     GradTable table;
     table.n = 0;
     int chunks = 0, before = 0;
@@ -234,7 +287,7 @@ void for_tables(const adcdiff_grad_tensor* ts, int n, F launch) {
             GradEntry& e = table.t[table.n++];
             e.grad = ts[i].grad; e.out = ts[i].out; e.numel = ts[i].numel; e.first_chunk = chunks;
             e.types = (ts[i].dtype == ADCDIFF_BF16 ? 1 : 0) | (ts[i].out && ts[i].out_dtype == ADCDIFF_BF16 ? 2 : 0);
-            chunks += (int)chunks_of(ts[i].numel);
+            chunks += (int)parts_of(ts[i].numel, part);
         }
         if (table.n == kTable || (i == n - 1 && table.n > 0)) {
             launch(table, chunks, before);
@@ -250,7 +303,7 @@ constexpr size_t kHead = 64;   // bytes in front of the partial results: the cli
 template <typename Op>
 int norm_launches(const char* who, const adcdiff_grad_tensor* ts, int n, long long chunks, float max_norm, float* norm, float* factor, void* partial_, hipStream_t stream) {
     typename Op::Acc* partial = static_cast<typename Op::Acc*>(partial_);
-    for_tables(ts, n, [&](const GradTable& t, int count, int before) {
+    for_tables(ts, n, kChunk, [&](const GradTable& t, int count, int before) {
         TimingScope timing(ADCDIFF_KIND_OTHER, count, (int)kChunk, 0, 0.0, 4.0 * count * kChunk, stream);
         hipLaunchKernelGGL(grad_partial_kernel<Op>, dim3(count), dim3(256), 0, stream, t, partial + before);
     });
@@ -281,10 +334,20 @@ int run(const char* who, const adcdiff_grad_tensor* ts, int n, int norm_type, bo
     hipStream_t stream = as_stream(stream_);
     float* factor = clip ? static_cast<float*>(workspace) : nullptr;
     void* partial = static_cast<char*>(workspace) + kHead;
+    long long pieces = 0;
+    for (int i = 0; i < n && pieces <= kFewPieces; ++i) pieces += parts_of(ts[i].numel, kPiece);
+    if (n <= kTable && pieces > 0 && pieces <= kFewPieces) {
+        for_tables(ts, n, kPiece, [&](const GradTable& t, int count, int) {   // one table
+            TimingScope timing(ADCDIFF_KIND_OTHER, count, (int)kPiece, 0, 0.0, (clip ? 12.0 : 4.0) * count * kPiece, stream);
+            if (norm_type == 2) hipLaunchKernelGGL(grad_small_kernel<SumSquares>, dim3(1), dim3(1024), 0, stream, t, count, (float)max_norm, norm, (int)clip);
+            else hipLaunchKernelGGL(grad_small_kernel<MaxAbs>, dim3(1), dim3(1024), 0, stream, t, count, (float)max_norm, norm, (int)clip);
+        });
+        return check_launch(who);
+    }
     rc = norm_type == 2 ? norm_launches<SumSquares>(who, ts, n, chunks, (float)max_norm, norm, factor, partial, stream)
                         : norm_launches<MaxAbs>(who, ts, n, chunks, (float)max_norm, norm, factor, partial, stream);
     if (rc != ADCDIFF_OK || !clip) return rc;
-    for_tables(ts, n, [&](const GradTable& t, int count, int) {
+    for_tables(ts, n, kChunk, [&](const GradTable& t, int count, int) {
         TimingScope timing(ADCDIFF_KIND_OTHER, count, (int)kChunk, 0, 0.0, 8.0 * count * kChunk, stream);
         hipLaunchKernelGGL(grad_scale_kernel, dim3(count), dim3(256), 0, stream, t, factor);
     });
