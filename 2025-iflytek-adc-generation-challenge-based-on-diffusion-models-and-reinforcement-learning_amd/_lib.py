@@ -157,8 +157,9 @@ SIGNATURES = {
     "adcdiff_grad_norm": (C.c_int, [c_fp, C.c_int, C.c_int, c_fp, c_fp, C.c_size_t, c_fp]),
     "adcdiff_clip_grad_norm": (C.c_int, [c_fp, C.c_int, C.c_int, C.c_double, c_fp, c_fp, C.c_size_t, c_fp]),
     "adcdiff_quantize_rows": (C.c_int, [c_fp, C.c_longlong, C.c_int, C.c_int, C.c_int, c_fp, C.c_longlong, c_fp, c_fp]),
-    "adcdiff_gemm_i8_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
-    "adcdiff_gemm_i8": (C.c_int, [c_fp, c_fp, C.c_size_t, c_fp]),
+    "adcdiff_gemm_i8": (C.c_int, [c_fp, c_fp]),
+    "adcdiff_linear_i8_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "adcdiff_linear_i8": (C.c_int, [c_fp, C.c_longlong, C.c_int, c_fp, c_fp, C.c_size_t, c_fp]),
     "adcdiff_pitch_rows_i8": (C.c_int, [c_fp, C.c_longlong, C.c_int, C.c_int, c_fp, C.c_longlong, c_fp]),
     "adcdiff_debug_set": (C.c_int, [C.c_char_p, C.c_longlong]),
     "adcdiff_debug_get": (C.c_int, [C.c_char_p, C.POINTER(C.c_longlong)]),

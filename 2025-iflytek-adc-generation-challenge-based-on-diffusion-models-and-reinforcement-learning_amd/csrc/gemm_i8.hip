@@ -636,10 +636,9 @@ extern "C" int adcdiff_pitch_rows_i8(const int8_t* src, long long ld_src, int M,
     return check_launch("pitch_rows_i8");
 }
 
-extern "C" size_t adcdiff_gemm_i8_workspace_bytes(int, int, int) { return 0; }
-
-extern "C" int adcdiff_gemm_i8(const adcdiff_gemm_i8_args* a, void*, size_t, adcdiff_stream_t stream_) {
-    using namespace adcdiff;
+namespace adcdiff {
+namespace {
+int check_gemm(const adcdiff_gemm_i8_args* a) {
     if (!a) return fail(ADCDIFF_E_BADARG, "gemm_i8: null args");
     if (a->M < 0 || a->N < 1 || a->K < 1 || a->K > kMaxK) return fail(ADCDIFF_E_BADARG, "gemm_i8: M %d, N %d, K %d (1..%d)", a->M, a->N, a->K, kMaxK);
     if (!type_ok(a->out_dtype) || (a->act != 0 && a->act != 1)) return fail(ADCDIFF_E_BADARG, "gemm_i8: type %d, act %d", a->out_dtype, a->act);
@@ -648,6 +647,15 @@ extern "C" int adcdiff_gemm_i8(const adcdiff_gemm_i8_args* a, void*, size_t, adc
     if (!aligned16(a->a) || !aligned16(a->w) || a->lda % 16 != 0 || a->ldw % 16 != 0 || a->lda < a->K || a->ldw < a->K)
         return fail(ADCDIFF_E_BADARG, "gemm_i8: the rows of a and w start on 16-byte boundaries and hold %d columns (pitches %lld, %lld)", a->K, a->lda, a->ldw);
     if (a->ldo < a->N || (a->residual && a->ldr < a->N)) return fail(ADCDIFF_E_BADARG, "gemm_i8: a row pitch below %d columns", a->N);
+    return ADCDIFF_OK;
+}
+}  // namespace
+}  // namespace adcdiff
+
+extern "C" int adcdiff_gemm_i8(const adcdiff_gemm_i8_args* a, adcdiff_stream_t stream_) {
+    using namespace adcdiff;
+    const int rc = check_gemm(a);
+    if (rc != ADCDIFF_OK || a->M == 0) return rc;
     hipStream_t stream = as_stream(stream_);
     I8Params p{a->a, a->w, a->a_scale, a->w_scale, a->bias, a->residual, a->out, a->lda, a->ldw, a->ldr, a->ldo, a->M, a->N, a->K, a->act, false};
     const int so = type_size(a->out_dtype);
@@ -655,4 +663,27 @@ extern "C" int adcdiff_gemm_i8(const adcdiff_gemm_i8_args* a, void*, size_t, adc
     TimingScope timing(ADCDIFF_KIND_OTHER, a->M, a->N, a->K, 2.0 * a->M * a->N * a->K,
                        (double)a->M * a->K + (double)a->N * a->K + (double)a->M * a->N * so * (a->residual ? 2 : 1), stream);
     return a->out_dtype == ADCDIFF_BF16 ? launch_gemm<bf16_t>(p, stream) : launch_gemm<float>(p, stream);
+}
+
+extern "C" size_t adcdiff_linear_i8_workspace_bytes(int M, int K) {
+    if (M < 0 || K < 1) return 0;
+    return ((size_t)K + 15) / 16 * 16 * (size_t)M + 4 * (size_t)M + 16;
+}
+
+extern "C" int adcdiff_linear_i8(const void* x, long long ldx, int dtype, const adcdiff_gemm_i8_args* a, void* workspace, size_t workspace_bytes,
+                                 adcdiff_stream_t stream) {
+    using namespace adcdiff;
+    if (!a || a->M < 0 || a->K < 1) return fail(ADCDIFF_E_BADARG, "linear_i8: null args, or %d rows of %d columns", a ? a->M : 0, a ? a->K : 0);
+    const size_t need = adcdiff_linear_i8_workspace_bytes(a->M, a->K);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+        return fail(ADCDIFF_E_WORKSPACE, "linear_i8: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    const long long pitch = ((long long)a->K + 15) / 16 * 16;
+    adcdiff_gemm_i8_args g = *a;
+    g.a = static_cast<const int8_t*>(workspace);
+    g.lda = pitch;
+    g.a_scale = reinterpret_cast<const float*>(g.a + pitch * a->M);
+    int rc = check_gemm(&g);     // before the first launch: a refused call leaves nothing behind
+    if (rc != ADCDIFF_OK) return rc;
+    rc = adcdiff_quantize_rows(x, ldx, dtype, a->M, a->K, static_cast<int8_t*>(workspace), pitch, const_cast<float*>(g.a_scale), stream);
+    return rc != ADCDIFF_OK ? rc : adcdiff_gemm_i8(&g, stream);
 }

@@ -502,34 +502,59 @@ def _i8_rows(t, what, stream):
     return o, pitch
 
 
+def _layer_output(like, M, N, K, w, w_scale, bias, residual, out_dtype):
+    """(out, pointers of w_scale and bias, pointer and pitch of the residual) after the checks that both forms of the layer share"""
+    if K < 1 or N < 1:
+        raise ValueError("no columns: K %d, N %d" % (K, N))
+    if w.dtype is not torch.int8:
+        raise ValueError("w must be int8, got %s" % w.dtype)
+    vectors = _vector(w_scale, N, "w_scale"), _vector(bias, N, "bias")
+    out = like.new_empty((M, N), dtype=_TYPES[out_dtype])
+    if residual is None:
+        return out, vectors, 0, 0
+    if residual.shape != (M, N) or residual.dtype is not out.dtype:
+        raise ValueError("residual must be %s %s, got %s %s" % (out.dtype, (M, N), residual.dtype, tuple(residual.shape)))
+    return out, vectors, residual.data_ptr(), _pitch(residual, "residual")
+
+
 def _raw_gemm_int8(a, a_scale, w, w_scale, bias, residual, act, out_dtype):
     dev = _device_of(a, a_scale, w, w_scale, bias, residual)
     if dev != _current_device():
         with torch.cuda.device(dev):
             return _raw_gemm_int8(a, a_scale, w, w_scale, bias, residual, act, out_dtype)
-    if a.dtype is not torch.int8 or w.dtype is not torch.int8:
-        raise ValueError("a and w must be int8, got %s and %s" % (a.dtype, w.dtype))
+    if a.dtype is not torch.int8:
+        raise ValueError("a must be int8, got %s" % a.dtype)
     if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
         raise ValueError("a [M, K] and w [N, K] do not fit: %s, %s" % (tuple(a.shape), tuple(w.shape)))
     M, K = a.shape
     N = w.shape[0]
-    if K < 1 or N < 1:
-        raise ValueError("no columns: a %s, w %s" % (tuple(a.shape), tuple(w.shape)))
-    scales = _vector(a_scale, M, "a_scale"), _vector(w_scale, N, "w_scale"), _vector(bias, N, "bias")
-    out = a_scale.new_empty((M, N), dtype=_TYPES[out_dtype])
-    res, ldr = 0, 0
-    if residual is not None:
-        if residual.shape != (M, N) or residual.dtype is not out.dtype:
-            raise ValueError("residual must be %s %s, got %s %s" % (out.dtype, (M, N), residual.dtype, tuple(residual.shape)))
-        res, ldr = residual.data_ptr(), _pitch(residual, "residual")
+    out, vectors, res, ldr = _layer_output(a, M, N, K, w, w_scale, bias, residual, out_dtype)
+    scale = _vector(a_scale, M, "a_scale")
     stream = _stream_of(dev)
     a, lda = _i8_rows(a, "a", stream)
     w, ldw = _i8_rows(w, "w", stream)
-    lib = _lib.load()
-    need = lib.adcdiff_gemm_i8_workspace_bytes(M, N, K)
-    ws = a.new_empty((need,)) if need else None
-    check(lib.adcdiff_gemm_i8(_pack_gemm_i8(M, N, K, a.data_ptr(), lda, w.data_ptr(), ldw, *scales, res, ldr, act, out_dtype, out.data_ptr(), N),
-                              ws.data_ptr() if need else 0, need, stream))
+    check(_lib.load().adcdiff_gemm_i8(_pack_gemm_i8(M, N, K, a.data_ptr(), lda, w.data_ptr(), ldw, scale, *vectors, res, ldr, act, out_dtype, out.data_ptr(),
+                                                    N), stream))
+    return out
+
+
+def _raw_linear_int8(x, w, w_scale, bias, residual, act, out_dtype):
+    dev = _device_of(x, w, w_scale, bias, residual)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _raw_linear_int8(x, w, w_scale, bias, residual, act, out_dtype)
+    code, ldx = _code(x, "x"), _pitch(x, "x")
+    if w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError("x [M, K] and w [N, K] do not fit: %s, %s" % (tuple(x.shape), tuple(w.shape)))
+    M, K = x.shape
+    N = w.shape[0]
+    out, vectors, res, ldr = _layer_output(x, M, N, K, w, w_scale, bias, residual, out_dtype)
+    stream = _stream_of(dev)
+    w, ldw = _i8_rows(w, "w", stream)
+    need = (K + 15) // 16 * 16 * M + 4 * M + 16          # adcdiff_linear_i8_workspace_bytes
+    ws = x.new_empty((need,), dtype=torch.uint8)
+    check(_lib.load().adcdiff_linear_i8(x.data_ptr(), ldx, code, _pack_gemm_i8(M, N, K, 0, 0, w.data_ptr(), ldw, 0, *vectors, res, ldr, act, out_dtype,
+                                                                             out.data_ptr(), N), ws.data_ptr(), need, stream))
     return out
 
 
@@ -699,16 +724,22 @@ def _as_list(tensors):
     return tensors
 
 
-@torch.no_grad()
+def _outside_autograd(op, grads, *args):
+    """The norm of gradients that themselves require one (create_graph) is not differentiated."""
+    if any(map(operator.attrgetter("requires_grad"), grads)):
+        with torch.no_grad():
+            return op(grads, *args)
+    return op(grads, *args)
+
+
 def grad_norm(grads, norm_type=2.0):
     """The norm over all elements of all gradient tensors (float32 and bfloat16, any shapes without gaps in memory): a float32 scalar on
     their device.  norm_type 2 (squares summed in float64, so nothing overflows on the way) or inf (largest magnitude).  No
     synchronisation, the same bits every run; NaN if any element is.  An empty list has norm 0, on the CPU."""
     grads, code = _as_list(grads), _norm_type(norm_type)
-    return torch.ops.adcdiff.grad_norm(grads, code) if grads else torch.zeros(())
+    return _outside_autograd(torch.ops.adcdiff.grad_norm, grads, code) if grads else torch.zeros(())
 
 
-@torch.no_grad()
 def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, out=None):
     """Scales the gradient tensors by min(1, max_norm / (norm + 1e-6)) and returns their norm before that (see grad_norm).
 
@@ -728,8 +759,8 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, ou
     if error_if_nonfinite and not bool(torch.isfinite(grad_norm(grads, norm_type))):
         raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
     if out is None:
-        return torch.ops.adcdiff.clip_grad_norm_(grads, max_norm, code)
-    return torch.ops.adcdiff.clip_grad_norm_out(grads, max_norm, code, out)
+        return _outside_autograd(torch.ops.adcdiff.clip_grad_norm_, grads, max_norm, code)
+    return _outside_autograd(torch.ops.adcdiff.clip_grad_norm_out, grads, max_norm, code, out)
 
 
 class _Ungraded(torch.autograd.Function):

@@ -302,12 +302,7 @@ _define("gemm_int8(Tensor a, Tensor a_scale, Tensor w, Tensor w_scale, Tensor? b
         ops._raw_gemm_int8, lambda a, a_scale, w, w_scale, bias, residual, act, out_dtype: a.new_empty((a.shape[0], w.shape[0]), dtype=_td(out_dtype)))
 
 
-def _linear_int8(x, w, w_scale, bias, residual, act, out_dtype):
-    a, a_scale = ops._raw_quantize_rows(x)
-    return ops._raw_gemm_int8(a, a_scale, w, w_scale, bias, residual, act, out_dtype)
-
-
-_define("linear_int8(Tensor x, Tensor w, Tensor w_scale, Tensor? bias, Tensor? residual, int act, int out_dtype) -> Tensor", _linear_int8,
+_define("linear_int8(Tensor x, Tensor w, Tensor w_scale, Tensor? bias, Tensor? residual, int act, int out_dtype) -> Tensor", ops._raw_linear_int8,
         lambda x, w, w_scale, bias, residual, act, out_dtype: x.new_empty((x.shape[0], w.shape[0]), dtype=_td(out_dtype)))
 
 

@@ -434,8 +434,7 @@ int adcdiff_quantize_rows(const void* x, long long ldx, int dtype, int M, int K,
 /* out[m, n] = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n] + residual[m, n]) on v_mfma_i32_16x16x64_i8: the sum is exact
  * (int32, K <= 131071), the rest float32 with one rounding to out_dtype.  act: 0 none, 1 SiLU.
  *   a [M, lda], w [N, ldw] int8 with rows on 16-byte boundaries (pointer and pitch; bytes behind K may hold anything), a_scale [M],
- *   w_scale [N] float32; bias [N] float32 or NULL; residual [M, ldr] in out_dtype or NULL (may alias out); out [M, ldo].
- * workspace: adcdiff_gemm_i8_workspace_bytes(M, N, K) bytes on a 16-byte boundary (0: none needed), not shared by calls that overlap. */
+ *   w_scale [N] float32; bias [N] float32 or NULL; residual [M, ldr] in out_dtype or NULL (may alias out); out [M, ldo]. */
 typedef struct adcdiff_gemm_i8_args {
     int M, N, K;
     const int8_t* a;
@@ -449,8 +448,13 @@ typedef struct adcdiff_gemm_i8_args {
     void* out;
     long long ldo;
 } adcdiff_gemm_i8_args;
-size_t adcdiff_gemm_i8_workspace_bytes(int M, int N, int K);
-int adcdiff_gemm_i8(const adcdiff_gemm_i8_args* args, void* workspace, size_t workspace_bytes, adcdiff_stream_t stream);
+int adcdiff_gemm_i8(const adcdiff_gemm_i8_args* args, adcdiff_stream_t stream);
+
+/* The layer on float rows: adcdiff_quantize_rows of x [M, K] into the workspace, then adcdiff_gemm_i8 of those codes (a, lda and a_scale of
+ * the arguments are not read).  The workspace holds the codes and their scales; calls that overlap do not share one. */
+size_t adcdiff_linear_i8_workspace_bytes(int M, int K);
+int adcdiff_linear_i8(const void* x, long long ldx, int dtype, const adcdiff_gemm_i8_args* args, void* workspace, size_t workspace_bytes,
+                      adcdiff_stream_t stream);
 
 /* Codes copied to rows on 16-byte boundaries: dst [M, ld_dst] (ld_dst a multiple of 16, >= K) from src [M, ld_src] at any alignment; the
  * columns behind K are written as 0. */

@@ -157,8 +157,18 @@ def _gemm_args(**over):
     (dict(ldo=7), "pitch"), (dict(residual=4096, ldr=7), "pitch"),
 ])
 def test_gemm_i8_refusals(over, words):
-    assert _lib.load().adcdiff_gemm_i8(C.byref(_gemm_args(**over)), None, 0, None) == -1
+    assert _lib.load().adcdiff_gemm_i8(C.byref(_gemm_args(**over)), None) == -1
     assert words in _message()
+
+
+def test_linear_i8_refusals():
+    lib = _lib.load()
+    need = lib.adcdiff_linear_i8_workspace_bytes(4, 32)
+    assert need >= 4 * 32 + 4 * 4 and lib.adcdiff_linear_i8_workspace_bytes(4, 0) == 0
+    for args, ws, size, code, words in ((dict(), 4096, need - 1, -4, "workspace"), (dict(), None, need, -4, "workspace"), (dict(), 4100, need, -4, "workspace"),
+                                        (dict(K=0), 4096, need, -1, "columns"), (dict(act=9), 4096, need, -1, "act"), (dict(w=None), 4096, need, -1, "null")):
+        assert lib.adcdiff_linear_i8(4096, 32, 0, C.byref(_gemm_args(**args)), ws, size, None) == code and words in _message()
+    assert lib.adcdiff_linear_i8(4096, 31, 0, C.byref(_gemm_args()), 4096, need, None) == -1 and "pitch" in _message()
 
 
 def test_row_quantiser_refusals():
