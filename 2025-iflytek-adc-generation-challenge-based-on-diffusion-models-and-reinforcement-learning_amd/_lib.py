@@ -168,7 +168,10 @@ SIGNATURES = {
     "adcdiff_matrix_core_probe": (C.c_int, [C.c_int, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_double)]),
 }
 
+BINDING_PATH = os.path.join(HERE, "libadcdiff_torch.so")
+
 _lib = None
+_binding = False
 
 
 class AdcdiffError(RuntimeError):
@@ -183,7 +186,7 @@ def load():
     if not os.path.exists(LIB_PATH):
         raise AdcdiffError("%s is missing: run `python -c 'import __graft_entry__ as g; g.build()'` (hipcc, gfx950). "
                            "There is no CPU or PyTorch fallback for this path." % LIB_PATH)
-    lib = C.CDLL(LIB_PATH)
+    lib = C.CDLL(LIB_PATH, mode=C.RTLD_GLOBAL)     # the torch binding resolves the C entry points from it
     for name, (res, args) in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.restype = res
@@ -192,6 +195,18 @@ def load():
         raise AdcdiffError("libadcdiff.so has ABI version %d, expected 3" % lib.adcdiff_abi_version())
     _lib = lib
     return lib
+
+
+def load_binding():
+    """Load libadcdiff_torch.so (the operators that csrc/torch_binding.cpp registers); raises if it was not built."""
+    global _binding
+    if not _binding:
+        load()
+        if not os.path.exists(BINDING_PATH):
+            raise AdcdiffError("%s is missing: run `python -c 'import __graft_entry__ as g; g.build()'`." % BINDING_PATH)
+        import torch
+        torch.ops.load_library(BINDING_PATH)
+        _binding = True
 
 
 def check(rc):

@@ -12,6 +12,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libadcdiff.so")
+BINDING = os.path.join(HERE, "libadcdiff_torch.so")    # csrc/torch_binding.cpp: host code only, against the installed torch
 SOURCES = [("gemm.hip", []), ("gemm_tr.hip", []), ("elementwise.hip", ["-ffp-contract=off"]), ("unet.hip", []), ("train.hip", []),
            ("residual_norm.hip", []), ("grad_norm.hip", []), ("gemm_i8.hip", [])]
 # packed float32 instructions stay off: some of their forms have given wrong results on this hardware now and then
@@ -55,7 +56,25 @@ def build_library(force=False, verbose=False):
         if verbose:
             print(" ".join(cmd))
         subprocess.run(cmd, check=True)
+    build_binding(force, verbose)
     return LIB
+
+
+def build_binding(force=False, verbose=False):
+    """The PyTorch operators over the C ABI; the adcdiff_* symbols are resolved from libadcdiff.so when it is loaded."""
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    import torch
+    from torch.utils import cpp_extension
+    deps = [src, os.path.join(os.path.dirname(HERE), "include", "adcdiff.h"), torch.__file__]
+    if force or _stale(BINDING, deps):
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+               "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I/opt/rocm/include"]
+        cmd += ["-I" + p for p in cpp_extension.include_paths()] + [src, "-o", BINDING]
+        cmd += ["-L" + p for p in cpp_extension.library_paths()] + ["-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+        if verbose:
+            print(" ".join(cmd))
+        subprocess.run(cmd, check=True)
+    return BINDING
 
 
 if __name__ == "__main__":

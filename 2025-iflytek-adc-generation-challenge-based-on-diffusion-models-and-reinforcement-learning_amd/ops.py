@@ -8,10 +8,7 @@ The public functions (gemm, groupnorm_silu, philox_normal, ddpm_step, ddim_step,
 the PyTorch dispatcher: they call the custom operators ``torch.ops.adcdiff.*`` registered in ``torch_ops.py``
 (torch.library.custom_op with fake-tensor rules), whose implementations are the ``_raw_*`` ctypes wrappers below.
 """
-import array
 import ctypes as C
-import operator
-import struct
 
 import torch
 
@@ -222,342 +219,6 @@ def _raw_latent_summary(x):
     return out
 
 
-# ---- gated residual norms, gradient norm, 8-bit integer layer --------------------------------------------------------
-_CODES = {torch.float32: F32, torch.bfloat16: BF16}
-_TYPES = {F32: torch.float32, BF16: torch.bfloat16}
-_NORMS = {None: 0, "rms": 1, "layer": 2}
-_dtype_of = operator.attrgetter("dtype")
-
-
-_current_device, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-
-# The C structs of include/adcdiff.h as one pack call each: filling a ctypes.Structure field by field takes several microseconds.
-_pack_norm_args = struct.Struct("8iQqQqQqQQQQffQqQqQ").pack       # adcdiff_residual_norm_args
-_pack_norm_grads = struct.Struct("QqQqQqQqQqQQQQ").pack           # adcdiff_residual_norm_grads
-_pack_gemm_i8 = struct.Struct("iii4xQqQqQQQQqiiQq").pack          # adcdiff_gemm_i8_args
-
-
-def _device_of(*tensors):
-    """The index of the one GPU that holds all the tensors."""
-    dev = -2
-    for t in tensors:
-        if t is not None:
-            i = t.get_device()
-            if i != dev:
-                if i < 0:
-                    _need_gpu(t)
-                if dev != -2:
-                    raise ValueError("tensors on different devices: cuda:%d and cuda:%d" % (dev, i))
-                dev = i
-    return dev
-
-
-def _code(t, what):
-    code = _CODES.get(t.dtype)
-    if code is None:
-        raise ValueError("%s must be float32 or bfloat16, got %s" % (what, t.dtype))
-    return code
-
-
-def _pitch(t, what):
-    """Row pitch in elements of a 2-D tensor whose rows are contiguous and do not overlap."""
-    strides = t.stride()
-    if len(strides) != 2:
-        raise ValueError("%s must be two-dimensional, got shape %s" % (what, tuple(t.shape)))
-    rows, cols = t.shape
-    if strides[1] != 1 and cols > 1:
-        raise ValueError("the rows of %s must be contiguous, got strides %s" % (what, strides))
-    if rows <= 1:
-        return cols
-    if strides[0] < cols:
-        raise ValueError("the rows of %s overlap: strides %s" % (what, strides))
-    return strides[0]
-
-
-def _vector(t, n, what):
-    """Address of an optional contiguous float32 vector, 0 for None."""
-    if t is None:
-        return 0
-    if t.dtype is not torch.float32 or t.shape != (n,) or not t.is_contiguous():
-        raise ValueError("%s must be a contiguous float32 vector of %d elements, got %s %s" % (what, n, t.dtype, tuple(t.shape)))
-    return t.data_ptr()
-
-
-def _gradient_rows(t, like_shape, like_type, what):
-    """(tensor, pitch) of an optional incoming gradient: t itself, or a copy where its rows are not contiguous or overlap (expanded)."""
-    if t is None:
-        return None, 0
-    if t.shape != like_shape or t.dtype is not like_type:
-        raise ValueError("%s must be %s %s, got %s %s" % (what, like_type, tuple(like_shape), t.dtype, tuple(t.shape)))
-    (rows, cols), (s0, s1) = like_shape, t.stride()
-    if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1):
-        t = t.contiguous()
-        return t, cols
-    return t, (s0 if rows > 1 else cols)
-
-
-def _norm_inputs(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps):
-    """(M, D, type of y, the fields of adcdiff_residual_norm_args up to eps)"""
-    ldx, stream_code = _pitch(x, "x"), _code(x, "x")
-    M, D = shape = x.shape
-    if h is not None:
-        if h.shape != shape:
-            raise ValueError("h %s and x %s differ in shape" % (tuple(h.shape), tuple(shape)))
-        hp, ldh, code = h.data_ptr(), _pitch(h, "h"), _code(h, "h")
-    elif gate is not None or post_norm or residual_scale != 1.0:
-        raise ValueError("a gate, a post norm or a residual scale needs h")
-    else:
-        hp, ldh, code = 0, 0, stream_code
-    gp = ldg = gate_code = gate_rows = 0
-    if gate is not None:
-        gate_rows = gate.shape[0]
-        if gate.dim() != 2 or gate.shape[1] != D or (M > 0 and (gate_rows < 1 or M % gate_rows != 0)):
-            raise ValueError("gate must be [G, %d] with G dividing %d rows, got %s" % (D, M, tuple(gate.shape)))
-        gp, gate_code = gate.data_ptr(), _code(gate, "gate")
-        if gate_rows > 1 and gate.stride(0) == 0 and (D <= 1 or gate.stride(1) == 1):
-            ldg = 0                    # one row expanded over the groups
-        else:
-            ldg = _pitch(gate, "gate")
-    if not post_norm and (post_weight is not None or post_bias is not None):
-        raise ValueError("post_weight / post_bias without a post norm")
-    if not pre_norm and (pre_weight is not None or pre_bias is not None):
-        raise ValueError("pre_weight / pre_bias without a pre norm")
-    return M, D, code, (M, D, code, stream_code, gate_code, post_norm, pre_norm, gate_rows, hp, ldh, x.data_ptr(), ldx, gp, ldg,
-                        _vector(post_weight, D, "post_weight"), _vector(post_bias, D, "post_bias"), _vector(pre_weight, D, "pre_weight"),
-                        _vector(pre_bias, D, "pre_bias"), residual_scale, eps)
-
-
-def _raw_residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x, with_stats):
-    """adcdiff_residual_norm: [x_new where with_x] + [y where pre_norm] + [stats [M, 4] where with_stats]."""
-    dev = _device_of(x, h, gate, post_weight, post_bias, pre_weight, pre_bias)
-    if dev != _current_device():
-        with torch.cuda.device(dev):
-            return _raw_residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x, with_stats)
-    M, D, _, fields = _norm_inputs(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps)
-    outs, xp, yp, sp = [], 0, 0, 0
-    if with_x:
-        o = x.new_empty((M, D))
-        xp = o.data_ptr()
-        outs.append(o)
-    if pre_norm:
-        o = (x if h is None else h).new_empty((M, D))
-        yp = o.data_ptr()
-        outs.append(o)
-    if with_stats:
-        o = x.new_empty((M, 4), dtype=torch.float32)
-        sp = o.data_ptr()
-        outs.append(o)
-    check(_lib.load().adcdiff_residual_norm(_pack_norm_args(*fields, xp, D, yp, D, sp), _stream_of(dev)))
-    return outs
-
-
-def _raw_residual_norm_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y, post_norm, pre_norm, residual_scale,
-                                eps, need):
-    """adcdiff_residual_norm_backward: the gradients of (h, x, gate, post_weight, post_bias, pre_weight, pre_bias) that `need` asks for: those of h, x
-    and gate as tensors of their own, those of the vectors as the rows of one float32 tensor behind them."""
-    dev = _device_of(x, h, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y)
-    if dev != _current_device():
-        with torch.cuda.device(dev):
-            return _raw_residual_norm_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y, post_norm, pre_norm,
-                                               residual_scale, eps, need)
-    M, D, code, fields = _norm_inputs(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps)
-    given = (h, x, gate, post_weight, post_bias, pre_weight, pre_bias)
-    if len(need) != 7:
-        raise ValueError("need has one entry for each of the seven inputs")
-    sp = 0
-    if post_norm or pre_norm:
-        if stats is None or stats.dtype is not torch.float32 or stats.shape != (M, 4) or not stats.is_contiguous():
-            raise ValueError("stats must be the contiguous float32 [%d, 4] tensor of the forward pass" % M)
-        sp = stats.data_ptr()
-    d_x_new, ld_dx = _gradient_rows(d_x_new, x.shape, x.dtype, "d_x_new")
-    d_y, ld_dy = _gradient_rows(d_y, x.shape, _TYPES[code], "d_y")
-    outs, at = [], [0] * 7
-    for i in range(3):
-        if need[i]:
-            o = given[i].new_empty(given[i].shape) if given[i] is not None else None
-            outs.append(o)
-            at[i] = 0 if o is None else o.data_ptr()
-    vectors = [i for i in range(3, 7) if need[i]]
-    if vectors:     # one allocation: at small sizes an allocation costs the host more than the kernels take
-        o = x.new_empty((len(vectors), D), dtype=torch.float32)
-        for k, i in enumerate(vectors):
-            at[i] = o.data_ptr() + 4 * D * k
-        outs.append(o)
-    if any(n and t is None for t, n in zip(given, need)):
-        raise ValueError("need asks for the gradient of an input that is not there")
-    args = _pack_norm_args(*fields, 0, D, 0, D, sp)
-    grads = _pack_norm_grads(0 if d_x_new is None else d_x_new.data_ptr(), ld_dx, 0 if d_y is None else d_y.data_ptr(), ld_dy, at[0], D, at[1], D, at[2], D,
-                             at[3], at[4], at[5], at[6])
-    lib = _lib.load()
-    need_bytes = lib.adcdiff_residual_norm_backward_workspace_bytes(args, grads)
-    ws = x.new_empty((need_bytes,), dtype=torch.uint8)
-    check(lib.adcdiff_residual_norm_backward(args, grads, ws.data_ptr(), need_bytes, _stream_of(dev)))
-    return outs
-
-
-def _dense(t):
-    """Whether the elements of t fill one block of memory, in any order."""
-    if t.layout != torch.strided:
-        return False
-    if t.is_contiguous():
-        return True
-    expect = 1
-    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if stride != expect:
-            return False
-        expect *= size
-    return True
-
-
-def _same_device(tensors):
-    devices = set(map(torch.Tensor.get_device, tensors))
-    if len(devices) != 1 or -1 in devices:
-        _need_gpu(*tensors)
-        raise ValueError("gradients on different devices")
-    return devices.pop()
-
-
-def _codes_of(tensors, what):
-    """Type codes of the tensors: one number where they are all alike, else a list."""
-    types = set(map(_dtype_of, tensors))
-    for t in types:
-        if t not in _CODES:
-            raise ValueError("%s must be float32 or bfloat16, got %s" % (what, t))
-    return _CODES[types.pop()] if len(types) == 1 else [_CODES[t.dtype] for t in tensors]
-
-
-def _grad_table(grads, out):
-    """(device, host array of adcdiff_grad_tensor): four 64-bit words for each tensor, the two types in the last"""
-    n = len(grads)
-    dev = _same_device(grads)
-    if not all(map(torch.Tensor.is_contiguous, grads)):
-        for i, g in enumerate(grads):
-            if not _dense(g):
-                raise ValueError("gradient %d has gaps or overlaps in memory: shape %s, strides %s" % (i, tuple(g.shape), g.stride()))
-    rows = array.array("q", bytes(32 * n))
-    pointers = array.array("q", map(torch.Tensor.data_ptr, grads))
-    codes = _codes_of(grads, "gradients")
-    rows[0::4], rows[2::4] = pointers, array.array("q", map(torch.Tensor.numel, grads))
-    if out is None:
-        rows[1::4], out_codes = pointers, codes
-    else:
-        if _same_device(out) != dev:
-            raise ValueError("gradients and outputs on different devices")
-        for i, (g, o) in enumerate(zip(grads, out)):
-            if o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
-                raise ValueError("output %d must be like its gradient in shape and strides" % i)
-        rows[1::4], out_codes = array.array("q", map(torch.Tensor.data_ptr, out)), _codes_of(out, "outputs")
-    if type(codes) is int and type(out_codes) is int:
-        rows[3::4] = array.array("q", [codes | out_codes << 32]) * n
-    else:
-        codes, out_codes = ([c] * n if type(c) is int else c for c in (codes, out_codes))
-        rows[3::4] = array.array("q", [c | o << 32 for c, o in zip(codes, out_codes)])
-    return dev, rows
-
-
-def _raw_grad_norm(grads, norm_type, max_norm=None, out=None):
-    """adcdiff_grad_norm, or adcdiff_clip_grad_norm with a max_norm: the norm, a float32 scalar on the gradients' device."""
-    dev, table = _grad_table(grads, out)
-    if dev != _current_device():
-        with torch.cuda.device(dev):
-            return _raw_grad_norm(grads, norm_type, max_norm, out)
-    lib = _lib.load()
-    n, at = len(grads), table.buffer_info()[0]
-    need = lib.adcdiff_grad_norm_workspace_bytes(at, n)
-    norm = grads[0].new_empty((), dtype=torch.float32)
-    ws = grads[0].new_empty((need,), dtype=torch.uint8)
-    if max_norm is None:
-        check(lib.adcdiff_grad_norm(at, n, norm_type, norm.data_ptr(), ws.data_ptr(), need, _stream_of(dev)))
-    else:
-        check(lib.adcdiff_clip_grad_norm(at, n, norm_type, max_norm, norm.data_ptr(), ws.data_ptr(), need, _stream_of(dev)))
-        torch.autograd.graph.increment_version(grads if out is None else out)    # the library wrote the tensors behind torch's back
-    return norm
-
-
-def _raw_quantize_rows(x):
-    dev = _device_of(x)
-    if dev != _current_device():
-        with torch.cuda.device(dev):
-            return _raw_quantize_rows(x)
-    code, ldx = _code(x, "x"), _pitch(x, "x")
-    M, K = x.shape
-    if K < 1:
-        raise ValueError("rows of no columns have no scale")
-    pitch = (K + 15) // 16 * 16
-    q = x.new_empty((M, pitch), dtype=torch.int8)
-    scale = x.new_empty((M,), dtype=torch.float32)
-    check(_lib.load().adcdiff_quantize_rows(x.data_ptr(), ldx, code, M, K, q.data_ptr(), pitch, scale.data_ptr(), _stream_of(dev)))
-    return (q if pitch == K else q[:, :K]), scale
-
-
-def _i8_rows(t, what, stream):
-    """(tensor, pitch) of 8-bit codes with rows on 16-byte boundaries: t itself, or a copy with that layout."""
-    ld = _pitch(t, what)
-    M, K = t.shape
-    pitch = (K + 15) // 16 * 16
-    if t.data_ptr() % 16 == 0 and (ld % 16 == 0 or M <= 1):
-        return t, (ld if M > 1 else pitch)
-    o = t.new_empty((M, pitch))
-    check(_lib.load().adcdiff_pitch_rows_i8(t.data_ptr(), ld, M, K, o.data_ptr(), pitch, stream))
-    return o, pitch
-
-
-def _layer_output(like, M, N, K, w, w_scale, bias, residual, out_dtype):
-    """(out, pointers of w_scale and bias, pointer and pitch of the residual) after the checks that both forms of the layer share"""
-    if K < 1 or N < 1:
-        raise ValueError("no columns: K %d, N %d" % (K, N))
-    if w.dtype is not torch.int8:
-        raise ValueError("w must be int8, got %s" % w.dtype)
-    vectors = _vector(w_scale, N, "w_scale"), _vector(bias, N, "bias")
-    out = like.new_empty((M, N), dtype=_TYPES[out_dtype])
-    if residual is None:
-        return out, vectors, 0, 0
-    if residual.shape != (M, N) or residual.dtype is not out.dtype:
-        raise ValueError("residual must be %s %s, got %s %s" % (out.dtype, (M, N), residual.dtype, tuple(residual.shape)))
-    return out, vectors, residual.data_ptr(), _pitch(residual, "residual")
-
-
-def _raw_gemm_int8(a, a_scale, w, w_scale, bias, residual, act, out_dtype):
-    dev = _device_of(a, a_scale, w, w_scale, bias, residual)
-    if dev != _current_device():
-        with torch.cuda.device(dev):
-            return _raw_gemm_int8(a, a_scale, w, w_scale, bias, residual, act, out_dtype)
-    if a.dtype is not torch.int8:
-        raise ValueError("a must be int8, got %s" % a.dtype)
-    if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
-        raise ValueError("a [M, K] and w [N, K] do not fit: %s, %s" % (tuple(a.shape), tuple(w.shape)))
-    M, K = a.shape
-    N = w.shape[0]
-    out, vectors, res, ldr = _layer_output(a, M, N, K, w, w_scale, bias, residual, out_dtype)
-    scale = _vector(a_scale, M, "a_scale")
-    stream = _stream_of(dev)
-    a, lda = _i8_rows(a, "a", stream)
-    w, ldw = _i8_rows(w, "w", stream)
-    check(_lib.load().adcdiff_gemm_i8(_pack_gemm_i8(M, N, K, a.data_ptr(), lda, w.data_ptr(), ldw, scale, *vectors, res, ldr, act, out_dtype, out.data_ptr(),
-                                                    N), stream))
-    return out
-
-
-def _raw_linear_int8(x, w, w_scale, bias, residual, act, out_dtype):
-    dev = _device_of(x, w, w_scale, bias, residual)
-    if dev != _current_device():
-        with torch.cuda.device(dev):
-            return _raw_linear_int8(x, w, w_scale, bias, residual, act, out_dtype)
-    code, ldx = _code(x, "x"), _pitch(x, "x")
-    if w.dim() != 2 or x.shape[1] != w.shape[1]:
-        raise ValueError("x [M, K] and w [N, K] do not fit: %s, %s" % (tuple(x.shape), tuple(w.shape)))
-    M, K = x.shape
-    N = w.shape[0]
-    out, vectors, res, ldr = _layer_output(x, M, N, K, w, w_scale, bias, residual, out_dtype)
-    stream = _stream_of(dev)
-    w, ldw = _i8_rows(w, "w", stream)
-    need = (K + 15) // 16 * 16 * M + 4 * M + 16          # adcdiff_linear_i8_workspace_bytes
-    ws = x.new_empty((need,), dtype=torch.uint8)
-    check(_lib.load().adcdiff_linear_i8(x.data_ptr(), ldx, code, _pack_gemm_i8(M, N, K, 0, 0, w.data_ptr(), ldw, 0, *vectors, res, ldr, act, out_dtype,
-                                                                             out.data_ptr(), N), ws.data_ptr(), need, stream))
-    return out
-
-
 class timing:
     """Context manager over adcdiff_timing_begin/_end: ``with ops.timing(4096) as t: ...; t.records``."""
 
@@ -633,51 +294,29 @@ def latent_summary(x):
     return torch.ops.adcdiff.latent_summary(x)
 
 
-class _ResidualNorm(torch.autograd.Function):
-    """Autograd link of residual_norm / row_norm over torch.ops.adcdiff.residual_norm and residual_norm_backward."""
-
-    @staticmethod
-    def forward(ctx, h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x):
-        outs = torch.ops.adcdiff.residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps,
-                                               with_x, True)
-        ctx.save_for_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, outs[-1])
-        ctx.args = (post_norm, pre_norm, residual_scale, eps)
-        ctx.set_materialize_grads(False)
-        return (outs[0] if with_x else None), (outs[-2] if pre_norm else None)
-
-    @staticmethod
-    def backward(ctx, d_x_new, d_y):
-        if torch.is_grad_enabled():         # create_graph: the gradients carry on without a gradient of their own
-            return _residual_norm_backward_once(ctx, d_x_new, d_y)
-        return _residual_norm_backward(ctx, d_x_new, d_y)
+# ---- gated residual norms, gradient norm, 8-bit integer layer: checks, allocation and autograd in csrc/torch_binding.cpp ----
+_NORMS = {None: 0, "rms": 1, "layer": 2}
+_operators = {}
 
 
-def _residual_norm_backward(ctx, d_x_new, d_y):
-    need = ctx.needs_input_grad[:7]
-    if d_x_new is None and d_y is None:
-        return (None,) * 12
-    outs = torch.ops.adcdiff.residual_norm_backward.default(*ctx.saved_tensors, d_x_new, d_y, *ctx.args, need)
-    if any(need[3:]):
-        outs[-1:] = outs[-1].unbind(0)
-    outs = iter(outs)
-    return (*[next(outs) if n else None for n in need], None, None, None, None, None)
-
-
-_residual_norm_backward_once = torch.autograd.function.once_differentiable(_residual_norm_backward)
+def _call(name, *args):
+    """torch.ops.adcdiff.<name>(*args); what the library refuses is raised as AdcdiffError."""
+    op = _operators.get(name)
+    if op is None:
+        _lib.load_binding()     # says so if it was not built
+        op = _operators[name] = getattr(torch.ops.adcdiff, name).default
+    try:
+        return op(*args)
+    except RuntimeError as e:
+        if str(e).startswith("adcdiff"):
+            raise AdcdiffError(str(e).split("\nException raised from")[0]) from None
+        raise
 
 
 def _norm_code(norm, what):
     if norm not in _NORMS:
         raise ValueError("%s must be None, 'rms' or 'layer', got %r" % (what, norm))
     return _NORMS[norm]
-
-
-def _residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x):
-    args = (h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, float(residual_scale), float(eps), with_x)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:7]):
-        return _ResidualNorm.apply(*args)
-    outs = torch.ops.adcdiff.residual_norm(*args, False)
-    return (outs[0] if with_x else None), (outs[-1] if pre_norm else None)
 
 
 def residual_norm(h, x, gate=None, post_norm=None, post_weight=None, post_bias=None, pre_norm=None, pre_weight=None, pre_bias=None,
@@ -697,15 +336,16 @@ def residual_norm(h, x, gate=None, post_norm=None, post_weight=None, post_bias=N
     accumulation belongs to the stream of a leaf's first use), or torch.ops.adcdiff.residual_norm_backward is called directly."""
     if gate is not None and gate.dim() == 1:
         gate = gate.unsqueeze(0)
-    return _residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, _norm_code(post_norm, "post_norm"),
-                          _norm_code(pre_norm, "pre_norm"), residual_scale, eps, True)
+    outs = _call("residual_norm", h, x, gate, post_weight, post_bias, pre_weight, pre_bias, _norm_code(post_norm, "post_norm"),
+                 _norm_code(pre_norm, "pre_norm"), residual_scale, eps, True, False)
+    return outs[0], (outs[1] if pre_norm else None)
 
 
 def row_norm(x, norm="rms", weight=None, bias=None, eps=1e-6):
     """The norm in front of a first block: "rms" or "layer" of the rows of x [M, D], in x's type.  Differentiable like residual_norm."""
     if norm is None:
         raise ValueError("norm must be 'rms' or 'layer'")
-    return _residual_norm(None, x, None, None, None, weight, bias, 0, _norm_code(norm, "norm"), 1.0, eps, False)[1]
+    return _call("residual_norm", None, x, None, None, None, weight, bias, 0, _norm_code(norm, "norm"), 1.0, eps, False, False)[0]
 
 
 def _norm_type(norm_type):
@@ -724,20 +364,12 @@ def _as_list(tensors):
     return tensors
 
 
-def _outside_autograd(op, grads, *args):
-    """The norm of gradients that themselves require one (create_graph) is not differentiated."""
-    if any(map(operator.attrgetter("requires_grad"), grads)):
-        with torch.no_grad():
-            return op(grads, *args)
-    return op(grads, *args)
-
-
 def grad_norm(grads, norm_type=2.0):
     """The norm over all elements of all gradient tensors (float32 and bfloat16, any shapes without gaps in memory): a float32 scalar on
     their device.  norm_type 2 (squares summed in float64, so nothing overflows on the way) or inf (largest magnitude).  No
     synchronisation, the same bits every run; NaN if any element is.  An empty list has norm 0, on the CPU."""
     grads, code = _as_list(grads), _norm_type(norm_type)
-    return _outside_autograd(torch.ops.adcdiff.grad_norm, grads, code) if grads else torch.zeros(())
+    return _call("grad_norm", grads, code) if grads else torch.zeros(())
 
 
 def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, out=None):
@@ -759,31 +391,8 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, ou
     if error_if_nonfinite and not bool(torch.isfinite(grad_norm(grads, norm_type))):
         raise RuntimeError("the norm of the gradients is not finite, so they cannot be clipped")
     if out is None:
-        return _outside_autograd(torch.ops.adcdiff.clip_grad_norm_, grads, max_norm, code)
-    return _outside_autograd(torch.ops.adcdiff.clip_grad_norm_out, grads, max_norm, code, out)
-
-
-class _Ungraded(torch.autograd.Function):
-    """A call whose result has no gradient: asking for one raises instead of leaving it out."""
-
-    @staticmethod
-    def forward(ctx, op, *args):
-        outs = op(*args)
-        if isinstance(outs, tuple):
-            ctx.mark_non_differentiable(outs[0])     # 8-bit codes
-        return outs
-
-    @staticmethod
-    def backward(ctx, *grads):
-        raise RuntimeError("the 8-bit integer layer has no gradient: it serves trained weights")
-
-
-def _ungraded(op, *args):
-    if torch.is_grad_enabled():
-        for t in args:
-            if torch.is_tensor(t) and t.requires_grad:
-                return _Ungraded.apply(op, *args)
-    return op(*args)
+        return _call("clip_grad_norm_", grads, max_norm, code)
+    return _call("clip_grad_norm_out", grads, max_norm, code, out)
 
 
 def quantize_rows(x):
@@ -791,17 +400,17 @@ def quantize_rows(x):
     row / scale rounded half to even, exactly.  For activations (a scale per token) and weights [N, K] (a scale per output channel)
     alike.  The codes' rows start on 16-byte boundaries, as gemm_int8 reads them.  A row of zeros has scale 0; a row with a NaN or an
     infinity has scale NaN, so that every product with it is NaN."""
-    return _ungraded(torch.ops.adcdiff.quantize_rows, x)
+    return _call("quantize_rows", x)
 
 
 def gemm_int8(a, a_scale, w, w_scale, bias=None, residual=None, act=0, out_dtype="bf16"):
     """act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n] + residual[m, n]) for int8 a [M, K] and w [N, K], float32 scales and
     bias, residual [M, N] in out_dtype; act 0 none, 1 SiLU.  The sum is exact (K up to 131071).  Codes whose rows do not start on
     16-byte boundaries are copied to such rows on every call: keep weights as quantize_rows returns them."""
-    return _ungraded(torch.ops.adcdiff.gemm_int8, a, a_scale, w, w_scale, bias, residual, int(act), dtype_code(out_dtype))
+    return _call("gemm_int8", a, a_scale, w, w_scale, bias, residual, int(act), dtype_code(out_dtype))
 
 
 def linear_int8(x, w, w_scale, bias=None, residual=None, act=0, out_dtype="bf16"):
     """The 8-bit integer form of a linear layer: the rows of x [M, K] (float32 or bfloat16) are quantised as by quantize_rows and
     multiplied with the codes w [N, K] (see gemm_int8).  For inference: it has no gradient, and asking for one raises."""
-    return _ungraded(torch.ops.adcdiff.linear_int8, x, w, w_scale, bias, residual, int(act), dtype_code(out_dtype))
+    return _call("linear_int8", x, w, w_scale, bias, residual, int(act), dtype_code(out_dtype))

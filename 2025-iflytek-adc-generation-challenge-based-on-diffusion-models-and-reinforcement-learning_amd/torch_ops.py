@@ -19,6 +19,7 @@ The training loss stays a ``torch.autograd.Function`` (models/diffusion_model.py
 which an autograd formula returning one tensor per parameter could not do without a copy.
 """
 import ctypes as C
+import os
 from typing import List, Optional, Tuple
 
 import torch
@@ -249,20 +250,7 @@ def unet_backward(handle: int, d_eps: Tensor, grad_pointers: Tensor, grad_arena:
 
 
 # ------------------------------------------------- gated residual norms, gradient norm, 8-bit integer layer
-# Defined on the dispatcher directly: torch.library.custom_op wraps every call in checks that take 15 us on the host, which is
-# several times what these kernels take at small sizes.
-_fragment = torch.library.Library("adcdiff", "FRAGMENT")
-
-
-def _define(schema, impl, fake):
-    name = schema[:schema.index("(")]
-    _fragment.define(schema, tags=(torch.Tag.pt2_compliant_tag,))
-    _fragment.impl(name, impl, "CUDA")
-    _fragment.impl(name, impl, "CPU")        # refuses: the wrappers in ops.py raise for tensors that are not on a GPU
-    torch.library.register_fake("adcdiff::" + name, fake, lib=_fragment)
-    getattr(torch.ops.adcdiff, name)     # listed by names()
-
-
+# Defined, implemented and differentiated in csrc/torch_binding.cpp; the fake-tensor rules are here.
 def _fake_residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x, with_stats):
     outs = [x.new_empty(x.shape)] if with_x else []
     if pre_norm:
@@ -274,9 +262,7 @@ def _fake_residual_norm(h, x, gate, post_weight, post_bias, pre_weight, pre_bias
 
 def _fake_residual_norm_backward(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y, post_norm, pre_norm,
                                  residual_scale, eps, need):
-    outs = [t.new_empty(t.shape) for t, n in zip((h, x, gate), need) if n]
-    vectors = sum(bool(n) for n in need[3:])
-    return outs + ([x.new_empty((vectors, x.shape[1]), dtype=torch.float32)] if vectors else [])
+    return [t.new_empty(t.shape) for t, n in zip((h, x, gate, post_weight, post_bias, pre_weight, pre_bias), need) if n]
 
 
 def _fake_quantize_rows(x):
@@ -284,26 +270,25 @@ def _fake_quantize_rows(x):
     return x.new_empty((M, (K + 15) // 16 * 16), dtype=torch.int8)[:, :K], x.new_empty((M,), dtype=torch.float32)
 
 
-_NORM_INPUTS = "Tensor? h, Tensor x, Tensor? gate, Tensor? post_weight, Tensor? post_bias, Tensor? pre_weight, Tensor? pre_bias"
-_define("residual_norm(" + _NORM_INPUTS + ", int post_norm, int pre_norm, float residual_scale, float eps, bool with_x, bool with_stats) -> Tensor[]",
-        ops._raw_residual_norm, _fake_residual_norm)
-_define("residual_norm_backward(" + _NORM_INPUTS + ", Tensor? stats, Tensor? d_x_new, Tensor? d_y, int post_norm, int pre_norm, "
-        "float residual_scale, float eps, bool[] need) -> Tensor[]", ops._raw_residual_norm_backward, _fake_residual_norm_backward)
-_define("grad_norm(Tensor[] grads, int norm_type) -> Tensor", ops._raw_grad_norm,
-        lambda grads, norm_type: grads[0].new_empty((), dtype=torch.float32))
-_define("clip_grad_norm_(Tensor(a!)[] grads, float max_norm, int norm_type) -> Tensor",
-        lambda grads, max_norm, norm_type: ops._raw_grad_norm(grads, norm_type, max_norm),
-        lambda grads, max_norm, norm_type: grads[0].new_empty((), dtype=torch.float32))
-_define("clip_grad_norm_out(Tensor[] grads, float max_norm, int norm_type, Tensor(a!)[] out) -> Tensor",
-        lambda grads, max_norm, norm_type, out: ops._raw_grad_norm(grads, norm_type, max_norm, out),
-        lambda grads, max_norm, norm_type, out: grads[0].new_empty((), dtype=torch.float32))
-_define("quantize_rows(Tensor x) -> (Tensor, Tensor)", ops._raw_quantize_rows, _fake_quantize_rows)
-_define("gemm_int8(Tensor a, Tensor a_scale, Tensor w, Tensor w_scale, Tensor? bias, Tensor? residual, int act, int out_dtype) -> Tensor",
-        ops._raw_gemm_int8, lambda a, a_scale, w, w_scale, bias, residual, act, out_dtype: a.new_empty((a.shape[0], w.shape[0]), dtype=_td(out_dtype)))
+def _fake_norm(grads, *args):
+    return grads[0].new_empty((), dtype=torch.float32)
 
 
-_define("linear_int8(Tensor x, Tensor w, Tensor w_scale, Tensor? bias, Tensor? residual, int act, int out_dtype) -> Tensor", ops._raw_linear_int8,
-        lambda x, w, w_scale, bias, residual, act, out_dtype: x.new_empty((x.shape[0], w.shape[0]), dtype=_td(out_dtype)))
+_FAKES = {
+    "residual_norm": _fake_residual_norm,
+    "residual_norm_backward": _fake_residual_norm_backward,
+    "grad_norm": _fake_norm,
+    "clip_grad_norm_": _fake_norm,
+    "clip_grad_norm_out": _fake_norm,
+    "quantize_rows": _fake_quantize_rows,
+    "gemm_int8": lambda a, a_scale, w, w_scale, bias, residual, act, out_dtype: a.new_empty((a.shape[0], w.shape[0]), dtype=_td(out_dtype)),
+    "linear_int8": lambda x, w, w_scale, bias, residual, act, out_dtype: x.new_empty((x.shape[0], w.shape[0]), dtype=_td(out_dtype)),
+}
+if os.path.exists(_lib.LIB_PATH) and os.path.exists(_lib.BINDING_PATH):     # a tree that is not built yet still imports; ops.py says so on use
+    _lib.load_binding()
+    for _name, _fake in _FAKES.items():
+        torch.library.register_fake("adcdiff::" + _name, _fake)
+        getattr(torch.ops.adcdiff, _name)     # listed by names()
 
 
 def names():

@@ -68,12 +68,6 @@ def test_empty_list_has_norm_zero():
     assert float(ops.grad_norm([])) == 0.0 and float(ops.clip_grad_norm_([], 1.0)) == 0.0
 
 
-def test_dense_layouts():
-    t = torch.zeros(6, 4, 5)
-    assert ops._dense(t) and ops._dense(t.permute(2, 0, 1)) and ops._dense(torch.zeros(0, 3)) and ops._dense(torch.zeros(()))
-    assert not ops._dense(t[:, ::2]) and not ops._dense(torch.zeros(1).expand(4)) and not ops._dense(t[:, :, :3])
-
-
 def _norm_args(**over):
     a = _lib.ResidualNormArgs()
     given = dict(M=4, D=32, dtype=1, stream_dtype=0, gate_dtype=1, post_norm=1, pre_norm=1, gate_rows=2, h=4096, ldh=32, x=8192, ldx=32, gate=16384, ldg=32,

@@ -151,8 +151,7 @@ def test_partial_gradients():
     xn, y, stats = torch.ops.adcdiff.residual_norm(*[s[k] for k in NAMES], 1, 2, 0.5, 1e-6, True, True)
 
     def back(d_x, d_y, need):
-        outs = torch.ops.adcdiff.residual_norm_backward(*[s[k] for k in NAMES], stats, d_x, d_y, 1, 2, 0.5, 1e-6, need)
-        return outs[:sum(need[:3])] + [row for t in outs[sum(need[:3]):] for row in t]
+        return torch.ops.adcdiff.residual_norm_backward(*[s[k] for k in NAMES], stats, d_x, d_y, 1, 2, 0.5, 1e-6, need)
     full = back(s["d_x"], s["d_y"], [True] * 7)
     for i in range(7):
         if i == 2:      # the gate's gradient decides how rows are cut: the sums of the others then differ in order
@@ -267,6 +266,36 @@ def test_autograd_function_under_capture():
         a, b = ops.residual_norm(fresh[0], fresh[1], gate=fresh[2], post_norm="rms", pre_norm="layer")
         assert torch.equal(a, xn) and torch.equal(b, y)
         assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad((a, b), fresh, (s["d_x"], s["d_y"])), grads))
+
+
+def test_differentiable_once():
+    s = _inputs(6, 64, F, F, F, 2, "rms", "rms")
+    h, x = s["h"].clone().requires_grad_(True), s["x"].clone().requires_grad_(True)
+    xn, y = ops.residual_norm(h, x, gate=s["gate"], post_norm="rms", pre_norm="rms")
+    g, = torch.autograd.grad(y.square().sum(), h, create_graph=True)
+    plain, = torch.autograd.grad(ops.residual_norm(h, x, gate=s["gate"], post_norm="rms", pre_norm="rms")[1].square().sum(), h)
+    assert torch.equal(g.detach(), plain)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        g.sum().backward()
+
+
+def test_outputs_without_gradient_inputs_have_none():
+    s = _inputs(6, 64, F, F, F, 2, "rms", "rms")
+    x = s["x"].clone().requires_grad_(True)
+    assert not ops.residual_norm(s["h"], s["x"], pre_norm="rms")[1].requires_grad
+    xn, y = ops.residual_norm(s["h"], x, pre_norm="rms")
+    assert xn.requires_grad and y.requires_grad
+    with torch.no_grad():
+        assert not ops.residual_norm(s["h"], x, pre_norm="rms")[1].requires_grad
+    g, = torch.autograd.grad(y.sum(), x)                 # x_new not used
+    want = ref.residual_norm(s["h"], s["x"], None, None, None, None, "rms", None, None, 1.0, 1e-6, None, torch.ones_like(s["x"]))["x"]
+    ref.close(g, *want, F, ref.STEPS + 64)
+    x_changed = x.detach().clone().requires_grad_(True)
+    y = ops.row_norm(x_changed)
+    with torch.no_grad():
+        x_changed.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
 
 
 def test_refusals():
