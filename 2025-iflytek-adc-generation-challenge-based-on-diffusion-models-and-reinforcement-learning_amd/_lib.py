@@ -107,6 +107,10 @@ class GemmI8Args(C.Structure):
                 ("out_dtype", C.c_int), ("out", c_fp), ("ldo", C.c_longlong)]
 
 
+class I8Copy(C.Structure):
+    _fields_ = [("src", c_fp), ("ld_src", C.c_longlong), ("dst", c_fp), ("ld_dst", C.c_longlong), ("M", C.c_int), ("K", C.c_int)]
+
+
 OPT_CHUNK = 4096
 OPT_NOALLOC_MAX_CHUNKS = 65536
 KIND_GEMM_F32, KIND_GEMM_BF16, KIND_GROUPNORM, KIND_UPDATE, KIND_GEMM_BF16_T256, KIND_OTHER, KIND_GEMM_BF16_W256 = 0, 1, 2, 3, 4, 5, 6
@@ -149,18 +153,17 @@ SIGNATURES = {
     "adcdiff_clip_adamw_workspace_bytes": (C.c_size_t, [C.c_longlong]),
     "adcdiff_clip_adamw_step": (C.c_int, [c_fp, C.c_int, C.c_longlong, C.POINTER(AdamWArgs), c_fp, c_fp, C.c_size_t, c_fp]),
     "adcdiff_clip_adamw_step_noalloc": (C.c_int, [c_fp, C.c_int, C.c_longlong, C.POINTER(AdamWArgs), c_fp, c_fp]),
-    # structs as addresses: C.byref(struct), or the bytes that ops.py packs
-    "adcdiff_residual_norm": (C.c_int, [c_fp, c_fp]),
-    "adcdiff_residual_norm_backward_workspace_bytes": (C.c_size_t, [c_fp, c_fp]),
-    "adcdiff_residual_norm_backward": (C.c_int, [c_fp, c_fp, c_fp, C.c_size_t, c_fp]),
-    "adcdiff_grad_norm_workspace_bytes": (C.c_size_t, [c_fp, C.c_int]),
-    "adcdiff_grad_norm": (C.c_int, [c_fp, C.c_int, C.c_int, c_fp, c_fp, C.c_size_t, c_fp]),
-    "adcdiff_clip_grad_norm": (C.c_int, [c_fp, C.c_int, C.c_int, C.c_double, c_fp, c_fp, C.c_size_t, c_fp]),
+    "adcdiff_residual_norm": (C.c_int, [C.POINTER(ResidualNormArgs), c_fp]),
+    "adcdiff_residual_norm_backward_workspace_bytes": (C.c_size_t, [C.POINTER(ResidualNormArgs), C.POINTER(ResidualNormGrads)]),
+    "adcdiff_residual_norm_backward": (C.c_int, [C.POINTER(ResidualNormArgs), C.POINTER(ResidualNormGrads), c_fp, C.c_size_t, c_fp]),
+    "adcdiff_grad_norm_workspace_bytes": (C.c_size_t, [C.POINTER(GradTensor), C.c_int]),
+    "adcdiff_grad_norm": (C.c_int, [C.POINTER(GradTensor), C.c_int, C.c_int, c_fp, c_fp, C.c_size_t, c_fp]),
+    "adcdiff_clip_grad_norm": (C.c_int, [C.POINTER(GradTensor), C.c_int, C.c_int, C.c_double, c_fp, c_fp, C.c_size_t, c_fp]),
     "adcdiff_quantize_rows": (C.c_int, [c_fp, C.c_longlong, C.c_int, C.c_int, C.c_int, c_fp, C.c_longlong, c_fp, c_fp]),
-    "adcdiff_gemm_i8": (C.c_int, [c_fp, c_fp]),
+    "adcdiff_gemm_i8": (C.c_int, [C.POINTER(GemmI8Args), c_fp]),
     "adcdiff_linear_i8_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
-    "adcdiff_linear_i8": (C.c_int, [c_fp, C.c_longlong, C.c_int, c_fp, c_fp, C.c_size_t, c_fp]),
-    "adcdiff_pitch_rows_i8": (C.c_int, [c_fp, C.c_longlong, C.c_int, C.c_int, c_fp, C.c_longlong, c_fp]),
+    "adcdiff_linear_i8": (C.c_int, [c_fp, C.c_longlong, C.c_int, C.POINTER(GemmI8Args), c_fp, C.c_size_t, c_fp]),
+    "adcdiff_pitch_rows_i8": (C.c_int, [C.POINTER(I8Copy), C.c_int, c_fp]),
     "adcdiff_debug_set": (C.c_int, [C.c_char_p, C.c_longlong]),
     "adcdiff_debug_get": (C.c_int, [C.c_char_p, C.POINTER(C.c_longlong)]),
     "adcdiff_timing_begin": (C.c_int, [C.c_int]),

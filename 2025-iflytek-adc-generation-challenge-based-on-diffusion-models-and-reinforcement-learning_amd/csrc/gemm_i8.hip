@@ -9,6 +9,7 @@ namespace adcdiff {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(1)));   // global memory takes 16-byte loads at any address
 
 // ------------------------------------------------------------------ codes of rows
 // A code is rne(x * 127 / top), exactly: t = x * (127 / top) in float32 is off by at most 127 * 2^-23 < 1.6e-5 (one division, one
@@ -122,19 +123,30 @@ void quantize_by_width(const void* x, long long ldx, int M, int K, int Kp, int8_
     else hipLaunchKernelGGL((quantize_long_rows_kernel<T>), dim3(std::min(M, 1 << 20)), dim3(1024), 0, stream, static_cast<const T*>(x), ldx, M, K, Kp, q, ldq, scale);
 }
 
-__global__ __launch_bounds__(256) void pitch_rows_kernel(const int8_t* __restrict__ src, long long ld_src, int M, int K, int8_t* __restrict__ dst, long long ld_dst) {
+struct PitchParams {
+    adcdiff_i8_copy c[2];
+    unsigned first;   // the second copy's first workgroup
+};
+
+__global__ __launch_bounds__(256) void pitch_rows_kernel(const PitchParams p) {
     // sixteen columns per thread: byte loads at any alignment, one 16-byte store
-    const long long per_row = ld_dst / 16;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= per_row * M) return;
-    const long long row = i / per_row, c = (i - row * per_row) * 16;
-    const int8_t* s = src + row * ld_src + c;
-    const int n = (int)min(16LL, max(0LL, (long long)K - c));
+    const bool second = blockIdx.x >= p.first;
+    const adcdiff_i8_copy& c = p.c[second];
+    const long long per_row = c.ld_dst / 16;
+    const long long i = (long long)(blockIdx.x - (second ? p.first : 0u)) * 256 + threadIdx.x;
+    if (i >= per_row * c.M) return;
+    const long long row = i / per_row, col = (i - row * per_row) * 16;
+    const int8_t* s = c.src + row * c.ld_src + col;
+    const int n = (int)min(16LL, max(0LL, (long long)c.K - col));
     u32x4 w = {0, 0, 0, 0};
+    if (n == 16) {
+        w = *reinterpret_cast<const u32x4_any*>(s);
+    } else {
 #pragma unroll
-    for (int b = 0; b < 16; ++b)
-        if (b < n) w[b >> 2] |= (uint32_t)(uint8_t)s[b] << (8 * (b & 3));
-    *reinterpret_cast<u32x4*>(dst + row * ld_dst + c) = w;
+        for (int b = 0; b < 15; ++b)
+            if (b < n) w[b >> 2] |= (uint32_t)(uint8_t)s[b] << (8 * (b & 3));
+    }
+    *reinterpret_cast<u32x4*>(c.dst + row * c.ld_dst + col) = w;
 }
 
 // ------------------------------------------------------------------ product
@@ -623,16 +635,27 @@ extern "C" int adcdiff_quantize_rows(const void* x, long long ldx, int dtype, in
     return check_launch("quantize_rows");
 }
 
-extern "C" int adcdiff_pitch_rows_i8(const int8_t* src, long long ld_src, int M, int K, int8_t* dst, long long ld_dst, adcdiff_stream_t stream_) {
+extern "C" int adcdiff_pitch_rows_i8(const adcdiff_i8_copy* copies, int n, adcdiff_stream_t stream_) {
     using namespace adcdiff;
-    if (M < 0 || K < 1 || ld_src < K || ld_dst < K || ld_dst % 16 != 0) return fail(ADCDIFF_E_BADARG, "pitch_rows_i8: %d rows of %d columns, pitches %lld -> %lld", M, K, ld_src, ld_dst);
-    if (M == 0) return ADCDIFF_OK;
-    if (!src || !dst || !aligned16(dst)) return fail(ADCDIFF_E_BADARG, "pitch_rows_i8: null pointer, or a destination off its 16-byte boundary");
-    const long long threads = ld_dst / 16 * M;
-    if (threads > 0x7fffffffLL * 128) return fail(ADCDIFF_E_BADARG, "pitch_rows_i8: too many rows");
+    if (!copies || n < 1 || n > 2) return fail(ADCDIFF_E_BADARG, "pitch_rows_i8: null table or %d copies", n);
+    PitchParams p{};
+    long long blocks[2] = {0, 0};
+    double bytes = 0.0;
+    for (int i = 0; i < n; ++i) {
+        const adcdiff_i8_copy& c = copies[i];
+        if (c.M < 0 || c.K < 1 || c.ld_src < c.K || c.ld_dst < c.K || c.ld_dst % 16 != 0)
+            return fail(ADCDIFF_E_BADARG, "pitch_rows_i8: %d rows of %d columns, pitches %lld -> %lld", c.M, c.K, c.ld_src, c.ld_dst);
+        if (c.M > 0 && (!c.src || !c.dst || !aligned16(c.dst))) return fail(ADCDIFF_E_BADARG, "pitch_rows_i8: null pointer, or a destination off its 16-byte boundary");
+        p.c[i] = c;
+        blocks[i] = (c.ld_dst / 16 * c.M + 255) / 256;
+        bytes += 2.0 * c.M * c.K;
+    }
+    if (blocks[0] + blocks[1] > 0xffffff) return fail(ADCDIFF_E_BADARG, "pitch_rows_i8: too many rows");
+    if (blocks[0] + blocks[1] == 0) return ADCDIFF_OK;
+    p.first = (unsigned)blocks[0];
     hipStream_t stream = as_stream(stream_);
-    TimingScope timing(ADCDIFF_KIND_OTHER, M, K, 0, 0.0, 2.0 * M * K, stream);
-    hipLaunchKernelGGL(pitch_rows_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, src, ld_src, M, K, dst, ld_dst);
+    TimingScope timing(ADCDIFF_KIND_OTHER, copies[0].M, copies[0].K, 0, 0.0, bytes, stream);
+    hipLaunchKernelGGL(pitch_rows_kernel, dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), 0, stream, p);
     return check_launch("pitch_rows_i8");
 }
 

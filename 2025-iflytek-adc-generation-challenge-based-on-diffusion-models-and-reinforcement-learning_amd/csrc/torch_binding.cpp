@@ -264,24 +264,29 @@ std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
     return {K == pitch16(K) ? q : q.narrow(1, 0, K), scale};
 }
 
-// 8-bit codes with rows on 16-byte boundaries: t itself, or a copy with that layout
-Tensor rows16(const Tensor& t, const char* what, int64_t* ld, c10::Device dev) {
-    TORCH_CHECK_VALUE(t.scalar_type() == at::kChar, what, " must be int8, got ", t.scalar_type());
-    *ld = pitch_of(t, what);
-    const int64_t M = t.size(0), K = t.size(1);
-    if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 && (*ld % 16 == 0 || M <= 1)) {
-        if (M <= 1) *ld = pitch16(K);
-        return t;
+// Codes as the product reads them: rows on 16-byte boundaries.  Those that are not are copied, all of a call in one launch.
+struct Rows16 {
+    adcdiff_i8_copy copies[2];
+    int n = 0;
+    // t itself, or the copy it will be; *ld: its pitch
+    Tensor add(const Tensor& t, const char* what, long long* ld) {
+        TORCH_CHECK_VALUE(t.scalar_type() == at::kChar, what, " must be int8, got ", t.scalar_type());
+        const int64_t pitch = pitch_of(t, what), M = t.size(0), K = t.size(1);
+        *ld = M > 1 ? pitch : pitch16(K);
+        if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 && *ld % 16 == 0) return t;
+        Tensor o = at::empty({M, pitch16(K)}, t.options());
+        *ld = pitch16(K);
+        copies[n++] = adcdiff_i8_copy{t.const_data_ptr<int8_t>(), pitch, o.mutable_data_ptr<int8_t>(), pitch16(K), narrow(M, "rows"), narrow(K, "columns")};
+        return o;
     }
-    Tensor o = at::empty({M, pitch16(K)}, t.options());
-    check(adcdiff_pitch_rows_i8(t.const_data_ptr<int8_t>(), *ld, narrow(M, "rows"), narrow(K, "columns"), o.mutable_data_ptr<int8_t>(), pitch16(K), stream_of(dev)));
-    *ld = pitch16(K);
-    return o;
-}
+    void run(c10::Device dev) {
+        if (n) check(adcdiff_pitch_rows_i8(copies, n, stream_of(dev)));
+    }
+};
 
 // The arguments that both forms of the layer share; fills `out` and `held` (what has to live until the launch)
 adcdiff_gemm_i8_args layer_args(const Tensor& left, const Tensor& w, const Tensor& w_scale, const OptTensor& bias, const OptTensor& residual, int64_t act,
-                                int64_t out_dtype, c10::Device dev, Tensor* out, Tensor* held) {
+                                int64_t out_dtype, Rows16* rows, Tensor* out, Tensor* held) {
     TORCH_CHECK_VALUE(left.dim() == 2 && w.dim() == 2 && left.size(1) == w.size(1), "rows ", left.sizes(), " and weights ", w.sizes(), " do not fit");
     const int64_t M = left.size(0), K = left.size(1), N = w.size(0);
     TORCH_CHECK_VALUE(K > 0 && N > 0, "no columns: K ", K, ", N ", N);
@@ -300,10 +305,8 @@ adcdiff_gemm_i8_args layer_args(const Tensor& left, const Tensor& w, const Tenso
         p.residual = residual->const_data_ptr();
         p.ldr = pitch_of(*residual, "residual");
     }
-    int64_t ldw;
-    *held = rows16(w, "w", &ldw, dev);
+    *held = rows->add(w, "w", &p.ldw);
     p.w = held->const_data_ptr<int8_t>();
-    p.ldw = ldw;
     p.out = out->mutable_data_ptr();
     p.ldo = N;
     return p;
@@ -314,12 +317,12 @@ Tensor gemm_int8(const Tensor& a, const Tensor& a_scale, const Tensor& w, const 
     const c10::Device dev = one_device({&a, &a_scale, &w, &w_scale, ptr(bias), ptr(residual)});
     const c10::DeviceGuard guard(dev);
     Tensor out, held_w;
-    adcdiff_gemm_i8_args p = layer_args(a, w, w_scale, bias, residual, act, out_dtype, dev, &out, &held_w);
+    Rows16 rows;
+    adcdiff_gemm_i8_args p = layer_args(a, w, w_scale, bias, residual, act, out_dtype, &rows, &out, &held_w);
     p.a_scale = vector_of(a_scale, a.size(0), "a_scale");
-    int64_t lda;
-    const Tensor held_a = rows16(a, "a", &lda, dev);
+    const Tensor held_a = rows.add(a, "a", &p.lda);
     p.a = held_a.const_data_ptr<int8_t>();
-    p.lda = lda;
+    rows.run(dev);
     check(adcdiff_gemm_i8(&p, stream_of(dev)));
     return out;
 }
@@ -330,7 +333,9 @@ Tensor linear_int8(const Tensor& x, const Tensor& w, const Tensor& w_scale, cons
     const int64_t ldx = pitch_of(x, "x");
     const c10::DeviceGuard guard(dev);
     Tensor out, held_w;
-    const adcdiff_gemm_i8_args p = layer_args(x, w, w_scale, bias, residual, act, out_dtype, dev, &out, &held_w);
+    Rows16 rows;
+    const adcdiff_gemm_i8_args p = layer_args(x, w, w_scale, bias, residual, act, out_dtype, &rows, &out, &held_w);
+    rows.run(dev);
     const size_t bytes = adcdiff_linear_i8_workspace_bytes(p.M, p.K);
     Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
     check(adcdiff_linear_i8(x.const_data_ptr(), ldx, code, &p, ws.mutable_data_ptr(), bytes, stream_of(dev)));

@@ -456,9 +456,16 @@ size_t adcdiff_linear_i8_workspace_bytes(int M, int K);
 int adcdiff_linear_i8(const void* x, long long ldx, int dtype, const adcdiff_gemm_i8_args* args, void* workspace, size_t workspace_bytes,
                       adcdiff_stream_t stream);
 
-/* Codes copied to rows on 16-byte boundaries: dst [M, ld_dst] (ld_dst a multiple of 16, >= K) from src [M, ld_src] at any alignment; the
- * columns behind K are written as 0. */
-int adcdiff_pitch_rows_i8(const int8_t* src, long long ld_src, int M, int K, int8_t* dst, long long ld_dst, adcdiff_stream_t stream);
+/* Codes copied to rows on 16-byte boundaries, one or two matrices in one launch: dst [M, ld_dst] (ld_dst a multiple of 16, >= K) from src
+ * [M, ld_src] at any alignment; the columns behind K are written as 0. */
+typedef struct adcdiff_i8_copy {
+    const int8_t* src;
+    long long ld_src;
+    int8_t* dst;
+    long long ld_dst;
+    int M, K;
+} adcdiff_i8_copy;
+int adcdiff_pitch_rows_i8(const adcdiff_i8_copy* copies, int n, adcdiff_stream_t stream);
 
 /* ------------------------------------------------------------------ measurement ------ */
 

@@ -170,8 +170,10 @@ def test_row_quantiser_refusals():
     for args, words in (((4096, 32, 0, -1, 32, 4096, 32, 4096), "rows"), ((4096, 32, 0, 4, 0, 4096, 32, 4096), "columns"), ((4096, 32, 3, 4, 32, 4096, 32, 4096), "type"),
                         ((None, 32, 0, 4, 32, 4096, 32, 4096), "null"), ((4096, 31, 0, 4, 32, 4096, 32, 4096), "pitch"), ((4096, 32, 0, 4, 32, 4096, 31, 4096), "pitch")):
         assert lib.adcdiff_quantize_rows(*args, None) == -1 and words in _message()
-    for args in ((4096, 31, 4, 32, 4096, 32), (4096, 32, 4, 32, 4096, 40), (4096, 32, 4, 32, 4100, 32), (None, 32, 4, 32, 4096, 32)):
-        assert lib.adcdiff_pitch_rows_i8(*args, None) == -1 and "pitch_rows_i8" in _message()
+    for src, ld_src, M, K, dst, ld_dst in ((4096, 31, 4, 32, 4096, 32), (4096, 32, 4, 32, 4096, 40), (4096, 32, 4, 32, 4100, 32), (None, 32, 4, 32, 4096, 32), (4096, 32, 4, 0, 4096, 32)):
+        bad = (_lib.I8Copy * 2)(_lib.I8Copy(4096, 32, 4096, 32, 4, 32), _lib.I8Copy(src, ld_src, dst, ld_dst, M, K))
+        assert lib.adcdiff_pitch_rows_i8(bad, 2, None) == -1 and "pitch_rows_i8" in _message()
+    assert lib.adcdiff_pitch_rows_i8(None, 1, None) == -1 and lib.adcdiff_pitch_rows_i8(bad, 3, None) == -1
 
 
 def test_new_structs_match_the_header_layout(tmp_path):
@@ -182,7 +184,7 @@ def test_new_structs_match_the_header_layout(tmp_path):
     if gcc is None:
         pytest.skip("gcc not available")
     pairs = [("adcdiff_residual_norm_args", _lib.ResidualNormArgs), ("adcdiff_residual_norm_grads", _lib.ResidualNormGrads),
-             ("adcdiff_grad_tensor", _lib.GradTensor), ("adcdiff_gemm_i8_args", _lib.GemmI8Args)]
+             ("adcdiff_grad_tensor", _lib.GradTensor), ("adcdiff_gemm_i8_args", _lib.GemmI8Args), ("adcdiff_i8_copy", _lib.I8Copy)]
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "adcdiff.h"', 'int main(void) {']
     for cname, ct in pairs:
         lines.append('printf("%s size %%zu\\n", sizeof(%s));' % (cname, cname))
