@@ -12,28 +12,55 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(1)));   // global memory takes 16-byte loads at any address
 
 // ------------------------------------------------------------------ codes of rows
-// A code is rne(x * 127 / top), exactly: t = x * (127 / top) in float32 is off by at most 127 * 2^-23 < 1.6e-5 (one division, one
-// product), so its rounding can only differ from the quotient's where t lies within that of a half; there the quotient is formed
-// in float64, where x * 127 is exact and the division's error is far below the distance of any quotient of two float32 numbers from a
-// half (>= 2^-26).  Below 1e-30, where 127 / top nears overflow, every element takes that path.
-__device__ __forceinline__ int code_of(float x, float top, float inv, bool tiny) {
-    const float t = x * inv, r = rintf(t);
-    if (tiny || fabsf(fabsf(t - r) - 0.5f) < 3.1e-5f) return (int)rint((double)x * 127.0 / (double)top);
-    return (int)r;
-}
-
+// A code is rne(x * 127 / top), exactly.
+// bfloat16 rows: x * 127 is exact in float32, and one correction of the product with 1 / top gives the correctly rounded quotient; a half
+// is then a half, and no other quotient of two 8-bit significands comes closer to one than 2^-10.  No branch: a value of top / 2, which is
+// such a half, stands in every second group of 512 codes.
+// float32 rows: t = x * (127 / top) is off by at most 127 * 2^-23 < 1.6e-5, so its rounding can only differ where t lies within that of a
+// half; there the quotient is formed in float64, where x * 127 is exact and the division's error is far below the distance of any
+// quotient of two float32 numbers from a half (>= 2^-26).  One test for N codes: a wave meets such a value in one group of thirty.
+// Rows whose maximum nears overflow or the subnormals (times 127, or 127 / top) take the float64 form throughout.
 struct RowScale {
     float top, inv, scale;
-    bool poison, tiny, zero;
+    bool none, far;                        // none: a row of zeros, or one with a NaN or an infinity: codes 0
     __device__ __forceinline__ explicit RowScale(uint32_t top_bits) {
         top = __builtin_bit_cast(float, top_bits);
-        poison = top_bits >= 0x7f800000u;   // infinity or NaN (NaN's bits are the larger)
-        zero = top_bits == 0u;
-        tiny = top < 1e-30f;
+        const bool poison = top_bits >= 0x7f800000u;   // infinity or NaN (NaN's bits are the larger)
+        none = poison || top_bits == 0u;
+        far = top < 1e-30f || top > 1e36f;
         inv = 127.0f / top;
         scale = poison ? __builtin_nanf("") : top / 127.0f;
     }
-    __device__ __forceinline__ int code(float x) const { return poison || zero ? 0 : code_of(x, top, inv, tiny); }
+    template <bool BF16, int N>
+    __device__ __forceinline__ void codes(const float (&x)[N], int (&q)[N]) const {
+        bool exact = far;
+        const float rtop = BF16 ? 1.0f / top : 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            if constexpr (BF16) {
+                const float p = x[e] * 127.0f, t = p * rtop;
+                q[e] = (int)rintf(fmaf(fmaf(-t, top, p), rtop, t));
+            } else {
+                const float t = x[e] * inv, r = rintf(t);
+                exact |= fabsf(fabsf(t - r) - 0.5f) < 3.1e-5f;
+                q[e] = (int)r;
+            }
+        }
+        if (exact) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) q[e] = (int)rint((double)x[e] * 127.0 / (double)top);
+        }
+        if (none) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) q[e] = 0;
+        }
+    }
+    __device__ __forceinline__ int code(float x) const {   // of either type
+        const float v[1] = {x};
+        int q[1];
+        codes<false>(v, q);
+        return q[0];
+    }
 };
 
 template <int TPR>
@@ -43,8 +70,9 @@ __device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red, int tid)
     if constexpr (TPR > 64) {
         if ((tid & 63) == 0) red[tid >> 6] = v;
         __syncthreads();
+        const int first = (tid >> 6) / (TPR / 64) * (TPR / 64);
 #pragma unroll
-        for (int w = 0; w < TPR / 64; ++w) v = max(v, red[w]);
+        for (int w = 0; w < TPR / 64; ++w) v = max(v, red[first + w]);
         __syncthreads();   // the next row writes red again
     }
     return v;
@@ -54,10 +82,10 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cas
 
 // one row per team, held in registers between the maximum and the codes
 template <typename T, bool VEC, int TPR, int V>
-__global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int8_t* __restrict__ q,
+__global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads) void quantize_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int8_t* __restrict__ q,
                                                                  long long ldq, float* __restrict__ scale) {
-    constexpr int E = 8 * V, TEAMS = kThreads / TPR;
-    __shared__ uint32_t red[kThreads / 64];
+    constexpr int E = 8 * V, THREADS = TPR > kThreads ? TPR : kThreads, TEAMS = THREADS / TPR;
+    __shared__ uint32_t red[THREADS / 64];
     const int tid = threadIdx.x, t = tid % TPR;
     // a team wider than a wave is alone in its workgroup, so the barriers of the maximum are met by every thread
     for (long long row = (long long)blockIdx.x * TEAMS + tid / TPR; row < M; row += (long long)gridDim.x * TEAMS) {
@@ -73,9 +101,14 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const T* __rest
             for (int j = 0; j < V; ++j) {
                 const int c = (j * TPR + t) * 8;
                 if (c < Kp) {
+                    float part[8];
+                    int code[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) part[i] = v[j * 8 + i];
+                    s.template codes<sizeof(T) == 2>(part, code);
                     uint32_t w[2] = {0, 0};
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)s.code(v[j * 8 + i]) & 0xffu) << (8 * (i & 3));
+                    for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)code[i] & 0xffu) << (8 * (i & 3));
                     *reinterpret_cast<uint2*>(out + c) = uint2{w[0], w[1]};
                 }
             }
@@ -108,8 +141,8 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(const T* __res
 
 template <typename T, bool VEC, int TPR, int V>
 void launch_quantize(const void* x, long long ldx, int M, int K, int Kp, int8_t* q, long long ldq, float* scale, hipStream_t stream) {
-    constexpr int teams = kThreads / TPR;
-    hipLaunchKernelGGL((quantize_rows_kernel<T, VEC, TPR, V>), dim3((unsigned)std::min(((long long)M + teams - 1) / teams, 1LL << 20)), dim3(kThreads), 0, stream,
+    constexpr int threads = TPR > kThreads ? TPR : kThreads, teams = threads / TPR;
+    hipLaunchKernelGGL((quantize_rows_kernel<T, VEC, TPR, V>), dim3((unsigned)std::min(((long long)M + teams - 1) / teams, 1LL << 20)), dim3(threads), 0, stream,
                        static_cast<const T*>(x), ldx, M, K, Kp, q, ldq, scale);
 }
 
@@ -117,9 +150,11 @@ template <typename T, bool VEC>
 void quantize_by_width(const void* x, long long ldx, int M, int K, int Kp, int8_t* q, long long ldq, float* scale, hipStream_t stream) {
     if (Kp <= 128) launch_quantize<T, VEC, 16, 1>(x, ldx, M, K, Kp, q, ldq, scale, stream);
     else if (Kp <= 512) launch_quantize<T, VEC, 64, 1>(x, ldx, M, K, Kp, q, ldq, scale, stream);
-    else if (Kp <= 2048) launch_quantize<T, VEC, 256, 1>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+    // few rows: the latency of one row counts (32 x 2048: 256 threads 2.5 us, 128 threads 2.8); many: the barriers of wide teams (65536 x 2048: 87, 75 us)
+    else if (Kp <= 2048 && M < 2048) launch_quantize<T, VEC, 256, 1>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+    else if (Kp <= 2048) launch_quantize<T, VEC, 128, 2>(x, ldx, M, K, Kp, q, ldq, scale, stream);
     else if (Kp <= 4096) launch_quantize<T, VEC, 256, 2>(x, ldx, M, K, Kp, q, ldq, scale, stream);
-    else if (Kp <= 8192) launch_quantize<T, VEC, 256, 4>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+    else if (Kp <= 8192) launch_quantize<T, VEC, 512, 2>(x, ldx, M, K, Kp, q, ldq, scale, stream);
     else hipLaunchKernelGGL((quantize_long_rows_kernel<T>), dim3(std::min(M, 1 << 20)), dim3(1024), 0, stream, static_cast<const T*>(x), ldx, M, K, Kp, q, ldq, scale);
 }
 

@@ -37,6 +37,28 @@ def test_codes(K, dtype):
         _same_codes(x.to(dtype))
 
 
+@pytest.mark.parametrize("M, K", [(2048, 2048), (2050, 1000), (5001, 1300), (70000, 64), (4097, 513)])
+@pytest.mark.parametrize("dtype", [F, BF])
+def test_codes_of_many_rows(M, K, dtype):
+    x = torch.randn(M, K, device="cuda") * torch.exp(3 * torch.randn(M, 1, device="cuda"))
+    _same_codes(x.to(dtype))
+
+
+def test_every_bfloat16_quotient():
+    """all pairs of 8-bit significands, over a range of exponents: each row one maximum against every smaller magnitude"""
+    sig = torch.arange(128, 256, device="cuda", dtype=torch.float64)
+    values = torch.cat([sig * 2.0 ** -e for e in range(0, 9)])
+    for shift in (0, 20, -100, 110, 118, -120):
+        tops = sig * 2.0 ** shift
+        x = (values[None, :] * 2.0 ** shift).expand(128, -1).clone()
+        x = torch.where(x <= tops[:, None], x, 0.0)
+        x[:, 0] = tops
+        x[:, 1::2] *= -1
+        assert torch.equal(x.to(BF).double(), x)
+        _same_codes(x.to(BF))
+        _same_codes(x.to(F))
+
+
 @pytest.mark.parametrize("dtype", [F, BF])
 def test_codes_on_ties(dtype):
     """rows whose quotients are exact halves, and float32 neighbours of halves"""
