@@ -262,9 +262,12 @@ __device__ __forceinline__ void finish8(const I8Params& p, int m, int n, const i
 // ---- BM x BN tile through a ring of LDS stages ------------------------------------------------------------------------------------
 // Eight waves (2 x 4); a stage is 128 columns of the tile's rows, filled by LDS-DMA (64 lanes x 16 bytes = eight rows of 128 bytes per
 // instruction).  The chunk c of a row lies at position c ^ ((row >> 1) & 7), applied to the source address, so fragment reads are free of bank
-// conflicts.  STAGES - 1 tiles are under way; a stage is refilled behind the barrier that follows the last wait for its reads.  The loop is
-// bound by the LDS-DMA (one instruction of 1 KiB per CU every 21 ns), hence the deep ring and, for the same output, the larger tile; two waves per
-// SIMD cover each other's LDS reads.  The weights are the MFMA's first operand: a lane's four results are consecutive outputs of a row.
+// conflicts.  STAGES - 1 tiles are under way; a stage is refilled behind the barrier that follows the last wait for its reads.  The weights are
+// the MFMA's first operand: a lane's four results are consecutive outputs of a row.
+// The loop is bound by LDS: a K tile of 128 x 128 takes 0.7 us whether one workgroup runs or all do, with the rows' lines in L2 or not
+// (a prefetch into L2 and an order of tiles that shares more rows there changed nothing), which is its 96 KiB of fragment reads and 32 KiB of DMA
+// writes at 64 bytes per cycle.  So two or three workgroups share a CU (two stages of 32 KiB, three of 16 KiB): each covers the others' barriers and
+// epilogues (4096 x 2048 x 2048: 26 us, four stages and one workgroup 32 us, 256 x 128 tiles 27 us).
 template <typename Out, int BM, int BN, int STAGES>
 __global__ __launch_bounds__(512) void gemm_i8_ring_kernel(const I8Params p) {
     constexpr int TM = BM / 32, TN = BN / 64, PIECES = (BM + BN) / 64, STAGE = (BM + BN) * 128, PITCH = BN + 4;
@@ -622,10 +625,10 @@ int launch_ring(const I8Params& p, hipStream_t stream) {
 // Which kernel: measured on all of them over 1..65536 rows, 512..4096 outputs, 512..8192 columns (us, M x N x K).
 //   few rows: the smallest split tile that still gives at most one workgroup per CU
 //     32 x 2048 x 4096: 16 x 16 tile 7.1, 32 x 16 8.6, 32 x 32 10.2;  64 x 2048 x 2048: 6.9, 6.0, 6.7;  128 x 2048 x 2048: 11.4, 8.8, 7.2, 64 x 64 ring 7.9
-//   more: the least of these estimates, which are fits to the measured times (kt: K tiles of 128; one round: 256 workgroups)
-//     64 x 64 ring    2.5 + rounds (1.0 + 0.28 kt), two workgroups to a CU:  512 x 2048 x 2048 9.2 (128 x 128: 14.4), 1024 x 2048 x 2048 11.9 (15.7)
-//     128 x 128 ring  whole rounds (4.8 + 0.66 kt):  2048 x 2048 x 2048 17.3 (64 x 64: 22.1, 256 x 256: 27.7)
-//     256 x 256       whole rounds (10.7 + 1.5 kt), less where half the CUs stay free:  8192 x 2048 x 2048 34.3 (60.1), 65536 x 512 x 512 33.3 (59.7)
+//   more: the least of three estimates fitted to the measured times (kt: K tiles of 128, r: tiles / 256 CUs, at least 1)
+//     64 x 64 ring     2.0 + 0.65 r + (0.09 + 0.25 r) kt:   512 x 2048 x 2048 8.6 (128 x 128: 15.0, 256 x 256: 25.6), 1024 x 2048 x 2048 11.2 (15.9, 26.0)
+//     128 x 128 ring   3.7 + 2.9 r + (0.23 + 0.42 r) kt:    2048 x 2048 x 2048 16.8 (20.6, 27.3), 4096 x 2048 x 2048 26.0 (37.9, 29.4)
+//     256 x 256        a round of 256 workgroups 10.9 + 1.45 kt, one of at most 128 11 + 1.1 kt:  8192 x 2048 x 2048 34.1 (66.9, 46.1), 65536 x 512 x 512 33.4 (52.8, 41.9)
 template <typename Out>
 int launch_gemm(const I8Params& p, hipStream_t stream) {
     auto tiles = [&](int bm, int bn) { return (((long long)p.M + bm - 1) / bm) * (((long long)p.N + bn - 1) / bn); };
@@ -633,15 +636,15 @@ int launch_gemm(const I8Params& p, hipStream_t stream) {
     if (tiles(32, 16) <= 256) return launch_split<Out, 32, 16, 8, 4>(p, stream);
     if (tiles(32, 32) <= 256) return launch_split<Out, 32, 32, 8, 2>(p, stream);
     const double kt = (p.K + 127) / 128;
-    auto rounds = [](long long n) { return (double)((n + 255) / 256); };
-    const double t64 = 2.5 + std::max(1.0, tiles(64, 64) / 256.0) * (1.0 + 0.28 * kt);
-    const double t128 = rounds(tiles(128, 128)) * (4.8 + 0.66 * kt);
+    const double r64 = std::max(1.0, tiles(64, 64) / 256.0), r128 = std::max(1.0, tiles(128, 128) / 256.0);
+    const double t64 = 2.0 + 0.65 * r64 + (0.09 + 0.25 * r64) * kt, t128 = 3.7 + 2.9 * r128 + (0.23 + 0.42 * r128) * kt;
     // the 256 x 256 kernel needs whole tiles in every direction and 32-bit offsets inside them
     if (p.M >= 256 && p.N >= 256 && p.K >= 256 && p.lda < (1 << 23) && p.ldw < (1 << 23)) {
-        const double t256 = rounds(tiles(256, 256)) * (10.7 + 1.5 * kt) * (tiles(256, 256) <= 128 ? 0.85 : 1.0);
+        const long long n = tiles(256, 256), last = n % 256;
+        const double t256 = (double)((n + 127) / 256) * (10.9 + 1.45 * kt) + (last > 0 && last <= 128 ? 11.0 + 1.1 * kt : 0.0);
         if (t256 < std::min(t64, t128)) return launch_w4_side<Out>(p, stream);
     }
-    return t64 < t128 ? launch_ring<Out, 64, 64, 4>(p, stream) : launch_ring<Out, 128, 128, 4>(p, stream);
+    return t64 < t128 ? launch_ring<Out, 64, 64, 3>(p, stream) : launch_ring<Out, 128, 128, 2>(p, stream);
 }
 
 constexpr int kMaxK = 131071;   // 128 * 128 * K stays below 2^31
