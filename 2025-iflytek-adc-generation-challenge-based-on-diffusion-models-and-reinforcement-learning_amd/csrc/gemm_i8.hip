@@ -2,6 +2,7 @@
 //   out[m, n] = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n] + residual[m, n]).
 // The sum runs on v_mfma_i32_16x16x64_i8 and is exact; what follows is float32 and rounded once.
 #include <algorithm>
+#include <atomic>
 
 #include "row_access.h"
 
@@ -82,9 +83,9 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cas
 
 // one row per team, held in registers between the maximum and the codes
 template <typename T, bool VEC, int TPR, int V>
-__global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads) void quantize_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int8_t* __restrict__ q,
+__global__ __launch_bounds__(threads_for<TPR>()) void quantize_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int8_t* __restrict__ q,
                                                                  long long ldq, float* __restrict__ scale) {
-    constexpr int E = 8 * V, THREADS = TPR > kThreads ? TPR : kThreads, TEAMS = THREADS / TPR;
+    constexpr int E = 8 * V, THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
     __shared__ uint32_t red[THREADS / 64];
     const int tid = threadIdx.x, t = tid % TPR;
     // a team wider than a wave is alone in its workgroup, so the barriers of the maximum are met by every thread
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(const T* __res
 
 template <typename T, bool VEC, int TPR, int V>
 void launch_quantize(const void* x, long long ldx, int M, int K, int Kp, int8_t* q, long long ldq, float* scale, hipStream_t stream) {
-    constexpr int threads = TPR > kThreads ? TPR : kThreads, teams = threads / TPR;
+    constexpr int threads = threads_for<TPR>(), teams = threads / TPR;
     hipLaunchKernelGGL((quantize_rows_kernel<T, VEC, TPR, V>), dim3((unsigned)std::min(((long long)M + teams - 1) / teams, 1LL << 20)), dim3(threads), 0, stream,
                        static_cast<const T*>(x), ldx, M, K, Kp, q, ldq, scale);
 }
@@ -588,8 +589,9 @@ __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(const I8Params p) {
 template <typename Out, int SIDE>
 int launch_w4(const I8Params& p, hipStream_t stream) {
     constexpr int smem = 2 * 65536;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_i8_w4_kernel<Out, SIDE>), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (attr != hipSuccess) return fail(ADCDIFF_E_LAUNCH, "gemm_i8: hipFuncSetAttribute: %s", hipGetErrorString(attr));
+    static std::atomic<bool> done[64];
+    const int rc = allow_lds("gemm_i8", reinterpret_cast<const void*>(&gemm_i8_w4_kernel<Out, SIDE>), smem, done);
+    if (rc != ADCDIFF_OK) return rc;
     const long long tiles = (((long long)p.M + 255) / 256) * (((long long)p.N + 255) / 256);
     if (tiles > 0xffffff) return fail(ADCDIFF_E_BADARG, "gemm_i8: %d x %d outputs are too many for one call", p.M, p.N);
     hipLaunchKernelGGL((gemm_i8_w4_kernel<Out, SIDE>), dim3((unsigned)tiles), dim3(256), smem, stream, p);
@@ -614,8 +616,9 @@ int launch_split(const I8Params& p, hipStream_t stream) {
 template <typename Out, int BM, int BN, int STAGES>
 int launch_ring(const I8Params& p, hipStream_t stream) {
     constexpr int smem = std::max((BM + BN) * 128 * STAGES, BM * (BN + 4) * 4);
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_i8_ring_kernel<Out, BM, BN, STAGES>), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (attr != hipSuccess) return fail(ADCDIFF_E_LAUNCH, "gemm_i8: hipFuncSetAttribute: %s", hipGetErrorString(attr));
+    static std::atomic<bool> done[64];
+    const int rc = allow_lds("gemm_i8", reinterpret_cast<const void*>(&gemm_i8_ring_kernel<Out, BM, BN, STAGES>), smem, done);
+    if (rc != ADCDIFF_OK) return rc;
     const long long tiles = (((long long)p.M + BM - 1) / BM) * (((long long)p.N + BN - 1) / BN);
     if (tiles > 0x7fffff) return fail(ADCDIFF_E_BADARG, "gemm_i8: %d x %d outputs are too many for one call", p.M, p.N);
     hipLaunchKernelGGL((gemm_i8_ring_kernel<Out, BM, BN, STAGES>), dim3((unsigned)tiles), dim3(512), smem, stream, p);

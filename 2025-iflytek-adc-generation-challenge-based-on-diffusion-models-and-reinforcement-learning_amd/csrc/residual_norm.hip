@@ -6,6 +6,8 @@
 // A team of TPR threads owns a row and holds it in registers (V vectors of 8 columns per thread), so every pass over the row after the
 // first load is free; both kernels are bound by HBM.  Statistics are two-pass (mean, then centred squares) on those registers.
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "row_access.h"
 
@@ -72,6 +74,14 @@ __device__ __forceinline__ void load_vector(const float* p, float absent, int t,
     for (int e = 0; e < 8; ++e) v[e] = p ? v[e] : absent;
 }
 
+// A thread's team: the same for a whole wave unless teams are narrower, which keeps row addresses out of the vector registers
+template <int TPR>
+__device__ __forceinline__ int team_of(int tid) {
+    if constexpr (TPR >= kThreads) return 0;
+    else if constexpr (TPR >= 64) return __builtin_amdgcn_readfirstlane(tid / TPR);
+    else return tid / TPR;
+}
+
 // bit e: element e of the thread lies inside the row
 template <bool VEC, int TPR>
 __device__ __forceinline__ unsigned inside(int t, int D) {
@@ -103,16 +113,13 @@ __device__ __forceinline__ void row_stats(const float (&v)[8], int kind, unsigne
     inv = 1.0f / sqrtf(fmaf(s[0], inv_d, eps));
 }
 
-template <int TPR>
-constexpr int threads_for() { return TPR > kThreads ? TPR : kThreads; }
-
 // A team of TPR threads per row, eight columns per thread; weights, biases and a gate shared by all rows stay in registers over the rows of a
 // workgroup, and the next row is on its way while the one in hand is reduced.
 template <typename T, typename R, bool VEC, int TPR>
 __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_kernel(const ResNormParams p) {
     constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
     __shared__ float red[2 * (THREADS / 64)];
-    const int tid = threadIdx.x, t = tid % TPR, team = tid / TPR, D = p.D;
+    const int tid = threadIdx.x, t = TEAMS == 1 ? tid : tid % TPR, team = team_of<TPR>(tid), D = p.D;
     const unsigned in = inside<VEC, TPR>(t, D);
     const bool one_gate = p.gate && p.gate_share >= p.M, row_gate = p.gate && !one_gate;
     RawRow<R, VEC, TPR> rx;
@@ -171,6 +178,59 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_kernel(const
     }
 }
 
+// Eight column sums of a thread.  In registers, or (a team of 1024 threads has 128 registers per thread) in LDS, where each thread owns its words.
+template <bool IN_LDS>
+struct ColumnSums {
+    float a[8];
+    __device__ __forceinline__ void init(float*, int) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = 0.0f;
+    }
+    __device__ __forceinline__ void add_product(const float (&x)[8], const float (&y)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = fmaf(x[e], y[e], a[e]);
+    }
+    __device__ __forceinline__ void add(const float (&x)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] += x[e];
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = a[e];
+    }
+};
+template <>
+struct ColumnSums<true> {
+    f32x4* p;   // two vectors of four, 1024 threads apart
+    __device__ __forceinline__ void init(float* lds, int tid) {
+        p = reinterpret_cast<f32x4*>(lds) + tid;
+        p[0] = p[1024] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __device__ __forceinline__ void add_product(const float (&x)[8], const float (&y)[8]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            f32x4 v = p[1024 * h];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(x[4 * h + e], y[4 * h + e], v[e]);
+            p[1024 * h] = v;
+        }
+    }
+    __device__ __forceinline__ void add(const float (&x)[8]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            f32x4 v = p[1024 * h];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += x[4 * h + e];
+            p[1024 * h] = v;
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = p[1024 * (e >> 2)][e & 3];
+    }
+};
+constexpr int kWideSums = 4 * 8 * 1024 * 4;   // bytes of LDS for the four vectors of a team of 1024
+
 // Gradients.  With u = N_post(h), xhat / uhat the normalised rows, g the gradient of a norm's output times its weight:
 //   d = d_x' + (g - [mean g] - xhat mean(g xhat)) / deviation      (g = d_y . pre_weight)
 //   d_x = residual_scale d,   d_gate = d . u,   d_h = N_post's gradient of d . gate,   d_weight = sum over rows of d_y . xhat, ...
@@ -181,19 +241,29 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_kernel(const
 template <typename T, typename R, bool VEC, int TPR>
 __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(const ResNormGradParams q) {
     constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
+    constexpr bool WIDE = TPR == 1024;
+    constexpr int TPW = TPR < 64 ? TPR : 64;   // columns of a wave in `joined`: a wave's own teams are added by shuffles first
     __shared__ float red[4 * (THREADS / 64)];
-    __shared__ float joined[TEAMS > 1 ? THREADS * 8 : 1];
+    __shared__ float joined[TEAMS > 1 ? THREADS / 64 * TPW * 8 : 1];
+    extern __shared__ __attribute__((aligned(16))) float wide[];     // kWideSums bytes where WIDE
     const ResNormParams& p = q.f;
-    const int tid = threadIdx.x, t = tid % TPR, team = tid / TPR, D = p.D;
+    const int tid = threadIdx.x, t = TEAMS == 1 ? tid : tid % TPR, team = team_of<TPR>(tid), D = p.D;
     const unsigned in = inside<VEC, TPR>(t, D);
     TeamSum<TPR, 2> sum(red);
-    float a_pre_w[8] = {}, a_pre_b[8] = {}, a_post_w[8] = {}, a_post_b[8] = {};
+    ColumnSums<WIDE> a_pre_w, a_pre_b, a_post_w, a_post_b;
+    a_pre_w.init(wide, tid);
+    a_pre_b.init(wide + 8192, tid);
+    a_post_w.init(wide + 2 * 8192, tid);
+    a_post_b.init(wide + 3 * 8192, tid);
+    // Teams of 768 and 1024 have 168 and 128 registers per thread: they load the weights where they are used, and no row ahead.
+    constexpr bool LEAN = TPR > 512;
     float post_w[8], post_b[8], pre_w[8];
-    load_vector<VEC, TPR>(p.post_w, 1.0f, t, D, post_w);
-    load_vector<VEC, TPR>(p.post_b, 0.0f, t, D, post_b);
-    load_vector<VEC, TPR>(p.pre_w, 1.0f, t, D, pre_w);
+    if constexpr (!LEAN) {
+        load_vector<VEC, TPR>(p.post_w, 1.0f, t, D, post_w);
+        load_vector<VEC, TPR>(p.post_b, 0.0f, t, D, post_b);
+        load_vector<VEC, TPR>(p.pre_w, 1.0f, t, D, pre_w);
+    }
     const bool row_gate = p.gate && p.gate_share == 1;
-    constexpr bool AHEAD = TPR < 1024;   // the next row's loads under this row's arithmetic; a team of 1024 has 128 registers per thread: none to spare
     const int teams = gridDim.x * TEAMS;
     // Every team of a workgroup makes the same number of turns (barriers inside the sums); turns without a row do nothing.
     for (int c0 = blockIdx.x * TEAMS; c0 < q.chunks; c0 += teams) {
@@ -221,7 +291,7 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
                 }
             }
         };
-        if constexpr (AHEAD) fetch(first);
+        if constexpr (!LEAN) fetch(first);
         float a_gate[8] = {}, gate[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) gate[e] = 1.0f;
@@ -229,15 +299,19 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
             const long long row = first + r;
             const bool live = row < last;
             float d[8], v[8], u[8], uhat[8], g[8], s[2];
-            if constexpr (!AHEAD) fetch(row);
+            if constexpr (LEAN) fetch(row);
             const f32x4 st = rs;
             rd.get(d);
             rx.get(v);
             rh.get(u);
             ry.get(g);
             if (p.gate) rg.get(p.gate_bf16, gate);
-            if constexpr (AHEAD) fetch(row + 1);
+            if constexpr (!LEAN) fetch(row + 1);   // under this row's arithmetic
             if (p.h) {
+                if constexpr (LEAN) {
+                    load_vector<VEC, TPR>(p.post_w, 1.0f, t, D, post_w);
+                    load_vector<VEC, TPR>(p.post_b, 0.0f, t, D, post_b);
+                }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     uhat[e] = u[e];
@@ -249,14 +323,18 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
                 }
             }
             if (p.pre) {
+                if constexpr (LEAN) load_vector<VEC, TPR>(p.pre_w, 1.0f, t, D, pre_w);
                 s[0] = s[1] = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     v[e] = (v[e] - st[2]) * st[3];
-                    if (live) {
-                        a_pre_w[e] = fmaf(g[e], v[e], a_pre_w[e]);
-                        a_pre_b[e] += g[e];
-                    }
+                }
+                if (live) {
+                    a_pre_w.add_product(g, v);
+                    a_pre_b.add(g);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
                     g[e] *= pre_w[e];
                     if (in >> e & 1) { s[0] += g[e]; s[1] = fmaf(g[e], v[e], s[1]); }
                 }
@@ -287,13 +365,14 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[e] *= gate[e];
                 if (p.post) {
+                    if constexpr (LEAN) load_vector<VEC, TPR>(p.post_w, 1.0f, t, D, post_w);
+                    if (live) {
+                        a_post_w.add_product(d, uhat);
+                        a_post_b.add(d);
+                    }
                     s[0] = s[1] = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        if (live) {
-                            a_post_w[e] = fmaf(d[e], uhat[e], a_post_w[e]);
-                            a_post_b[e] += d[e];
-                        }
                         d[e] *= post_w[e];
                         if (in >> e & 1) { s[0] += d[e]; s[1] = fmaf(d[e], uhat[e], s[1]); }
                     }
@@ -312,17 +391,28 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
         }
     }
     float* out = q.partial + (long long)blockIdx.x * q.vectors * D;
-    auto flush = [&](float (&a)[8], int slot) {
+    auto flush = [&](const ColumnSums<WIDE>& sums, int slot) {
         if (slot < 0) return;
+        float a[8];
+        sums.get(a);
         if constexpr (TEAMS > 1) {
-            __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) joined[e * THREADS + tid] = a[e];
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int m = TPR; m < 64; m <<= 1) a[e] += __shfl_xor(a[e], m);
             __syncthreads();
-            if (team == 0) {
+            const int row = tid / 64, col = tid % TPW;
+            if (TPR >= 64 || (tid & 63) < TPR) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) joined[(row * 8 + e) * TPW + col] = a[e];
+            }
+            __syncthreads();
+            if (team == 0) {   // waves of the same columns: every WAVES-th one
+                constexpr int WAVES = TPR > 64 ? TPR / 64 : 1;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    for (int k = 1; k < TEAMS; ++k) a[e] += joined[e * THREADS + k * TPR + t];
+#pragma unroll
+                    for (int k = WAVES; k < THREADS / 64; k += WAVES) a[e] += joined[((row + k) * 8 + e) * TPW + col];
             }
         }
         if (team == 0) store_row<float, VEC, TPR, 8>(out + (long long)slot * D, t, D, a);
@@ -433,7 +523,36 @@ bool vector_inputs(const adcdiff_residual_norm_args& a) {
            vector_rows(a.post_weight, 0, 4) && vector_rows(a.post_bias, 0, 4) && vector_rows(a.pre_weight, 0, 4) && vector_rows(a.pre_bias, 0, 4);
 }
 
-int team_width(int D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
+// Threads for a row of D columns, eight each.  Rows that are read in single elements take the next power of two.
+int team_width(int D, bool vec) {
+    const int waves = (D + 511) / 512;
+    if (vec && D <= 128) return 16;
+    if (vec && D <= 256) return 32;
+    if (!vec) return waves <= 1 ? 64 : waves <= 2 ? 128 : waves <= 4 ? 256 : waves <= 8 ? 512 : 1024;
+    return 64 * (waves <= 6 ? waves : waves <= 8 ? 8 : waves <= 12 ? 12 : 16);
+}
+
+// Calls f(std::integral_constant<int, threads>) for the team of a row
+template <bool VEC, typename F>
+void for_width(int tpr, F f) {
+    if constexpr (VEC) {
+        switch (tpr) {
+            case 16: return f(std::integral_constant<int, 16>());
+            case 32: return f(std::integral_constant<int, 32>());
+            case 192: return f(std::integral_constant<int, 192>());
+            case 320: return f(std::integral_constant<int, 320>());
+            case 384: return f(std::integral_constant<int, 384>());
+            case 768: return f(std::integral_constant<int, 768>());
+        }
+    }
+    switch (tpr) {
+        case 64: return f(std::integral_constant<int, 64>());
+        case 128: return f(std::integral_constant<int, 128>());
+        case 256: return f(std::integral_constant<int, 256>());
+        case 512: return f(std::integral_constant<int, 512>());
+        default: return f(std::integral_constant<int, 1024>());
+    }
+}
 
 template <typename T, typename R, bool VEC, int TPR>
 void launch_forward(const ResNormParams& p, hipStream_t stream) {
@@ -444,14 +563,7 @@ void launch_forward(const ResNormParams& p, hipStream_t stream) {
 
 template <typename T, typename R, bool VEC>
 void forward_by_width(const ResNormParams& p, hipStream_t stream) {
-    switch (team_width(p.D)) {
-        case 16: launch_forward<T, R, VEC, 16>(p, stream); break;
-        case 64: launch_forward<T, R, VEC, 64>(p, stream); break;
-        case 128: launch_forward<T, R, VEC, 128>(p, stream); break;
-        case 256: launch_forward<T, R, VEC, 256>(p, stream); break;
-        case 512: launch_forward<T, R, VEC, 512>(p, stream); break;
-        default: launch_forward<T, R, VEC, 1024>(p, stream); break;
-    }
+    for_width<VEC>(team_width(p.D, VEC), [&](auto tpr) { launch_forward<T, R, VEC, decltype(tpr)::value>(p, stream); });
 }
 
 template <bool VEC>
@@ -473,10 +585,10 @@ struct Cut {
 
 constexpr int kMaxGroups = 512;
 
-Cut cut_rows(int M, int D, int gate_rows, bool gate_grad, int vectors) {
+Cut cut_rows(int M, int D, bool vec, int gate_rows, bool gate_grad, int vectors) {
     Cut c{};
-    c.tpr = team_width(D);
-    c.teams = std::max(kThreads, c.tpr) / c.tpr;
+    c.tpr = team_width(D, vec);
+    c.teams = c.tpr >= kThreads ? 1 : kThreads / c.tpr;
     c.vectors = vectors;
     c.gate_sum = gate_grad && gate_rows > 0 && M / std::max(gate_rows, 1) != 1;
     const int groups = c.gate_sum ? gate_rows : 1;
@@ -501,27 +613,37 @@ size_t workspace_floats(const Cut& c, int D) {
 }
 
 template <typename T, typename R, bool VEC>
-void backward_by_width(const ResNormGradParams& q, const Cut& c, hipStream_t stream) {
-    const dim3 grid(c.workgroups);
-    switch (c.tpr) {
-        case 16: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 16>), grid, dim3(kThreads), 0, stream, q); break;
-        case 64: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 64>), grid, dim3(kThreads), 0, stream, q); break;
-        case 128: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 128>), grid, dim3(kThreads), 0, stream, q); break;
-        case 256: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 256>), grid, dim3(kThreads), 0, stream, q); break;
-        case 512: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 512>), grid, dim3(512), 0, stream, q); break;
-        default: hipLaunchKernelGGL((residual_norm_grad_kernel<T, R, VEC, 1024>), grid, dim3(1024), 0, stream, q); break;
-    }
+int backward_by_width(const ResNormGradParams& q, const Cut& c, hipStream_t stream) {
+    int rc = ADCDIFF_OK;
+    for_width<VEC>(c.tpr, [&](auto tpr) {
+        constexpr int TPR = decltype(tpr)::value;
+        const auto kernel = &residual_norm_grad_kernel<T, R, VEC, TPR>;
+        constexpr int lds = TPR == 1024 ? kWideSums : 0;
+        if constexpr (lds > 0) {
+            static std::atomic<bool> done[64];
+            rc = allow_lds("residual_norm_backward", reinterpret_cast<const void*>(kernel), lds, done);
+            if (rc != ADCDIFF_OK) return;
+        }
+        hipLaunchKernelGGL(kernel, dim3(c.workgroups), dim3(threads_for<TPR>()), lds, stream, q);
+    });
+    return rc;
 }
 
 template <bool VEC>
-void backward_by_type(const ResNormGradParams& q, const Cut& c, int dtype, int stream_dtype, hipStream_t stream) {
+int backward_by_type(const ResNormGradParams& q, const Cut& c, int dtype, int stream_dtype, hipStream_t stream) {
     if (dtype == ADCDIFF_BF16) {
-        if (stream_dtype == ADCDIFF_BF16) backward_by_width<bf16_t, bf16_t, VEC>(q, c, stream);
-        else backward_by_width<bf16_t, float, VEC>(q, c, stream);
+        if (stream_dtype == ADCDIFF_BF16) return backward_by_width<bf16_t, bf16_t, VEC>(q, c, stream);
+        return backward_by_width<bf16_t, float, VEC>(q, c, stream);
     } else {
-        if (stream_dtype == ADCDIFF_BF16) backward_by_width<float, bf16_t, VEC>(q, c, stream);
-        else backward_by_width<float, float, VEC>(q, c, stream);
+        if (stream_dtype == ADCDIFF_BF16) return backward_by_width<float, bf16_t, VEC>(q, c, stream);
+        return backward_by_width<float, float, VEC>(q, c, stream);
     }
+}
+
+bool vector_backward(const adcdiff_residual_norm_args& a, const adcdiff_residual_norm_grads& g) {
+    const int st = type_size(a.dtype), sr = type_size(a.stream_dtype), sg = type_size(a.gate_dtype);
+    return vector_inputs(a) && vector_rows(g.d_x_new, g.ld_d_x_new, sr) && vector_rows(g.d_y, g.ld_d_y, st) && vector_rows(g.h, g.ld_h, st) &&
+           vector_rows(g.x, g.ld_x, sr) && vector_rows(g.gate, a.gate_rows > 1 ? g.ld_gate : 0, sg);
 }
 
 int vector_count(const adcdiff_residual_norm_grads& g) { return !!g.post_weight + !!g.post_bias + !!g.pre_weight + !!g.pre_bias; }
@@ -550,7 +672,7 @@ extern "C" int adcdiff_residual_norm(const adcdiff_residual_norm_args* a, adcdif
 extern "C" size_t adcdiff_residual_norm_backward_workspace_bytes(const adcdiff_residual_norm_args* a, const adcdiff_residual_norm_grads* g) {
     using namespace adcdiff;
     if (check_args("residual_norm_backward", a) != ADCDIFF_OK || !g) return 0;
-    return std::max<size_t>(16, workspace_floats(cut_rows(a->M, a->D, a->gate ? a->gate_rows : 0, g->gate != nullptr, vector_count(*g)), a->D) * 4);
+    return std::max<size_t>(16, workspace_floats(cut_rows(a->M, a->D, vector_backward(*a, *g), a->gate ? a->gate_rows : 0, g->gate != nullptr, vector_count(*g)), a->D) * 4);
 }
 
 extern "C" int adcdiff_residual_norm_backward(const adcdiff_residual_norm_args* a, const adcdiff_residual_norm_grads* g, void* workspace,
@@ -569,12 +691,12 @@ extern "C" int adcdiff_residual_norm_backward(const adcdiff_residual_norm_args* 
     if ((g->d_x_new && g->ld_d_x_new < a->D) || (g->d_y && g->ld_d_y < a->D) || (g->h && g->ld_h < a->D) || (g->x && g->ld_x < a->D) ||
         (g->gate && a->gate_rows > 1 && g->ld_gate < a->D))
         return fail(ADCDIFF_E_BADARG, "residual_norm_backward: a row pitch below %d columns", a->D);
-    const Cut c = cut_rows(a->M, a->D, a->gate ? a->gate_rows : 0, g->gate != nullptr, vector_count(*g));
+    const Cut c = cut_rows(a->M, a->D, vector_backward(*a, *g), a->gate ? a->gate_rows : 0, g->gate != nullptr, vector_count(*g));
     const size_t need = std::max<size_t>(16, workspace_floats(c, a->D) * 4);
     if (!workspace || !aligned16(workspace) || workspace_bytes < need)
         return fail(ADCDIFF_E_WORKSPACE, "residual_norm_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     hipStream_t stream = as_stream(stream_);
-    const int st = type_size(a->dtype), sr = type_size(a->stream_dtype), sg = type_size(a->gate_dtype);
+    const int st = type_size(a->dtype), sr = type_size(a->stream_dtype);
     ResNormGradParams q{};
     q.f = forward_params(*a);
     q.d_xn = g->d_x_new; q.d_y = g->d_y; q.d_h = g->h; q.d_x = g->x; q.d_gate = g->gate;
@@ -589,10 +711,8 @@ extern "C" int adcdiff_residual_norm_backward(const adcdiff_residual_norm_args* 
     q.slot_pre_w = place(g->pre_weight); q.slot_pre_b = place(g->pre_bias); q.slot_post_w = place(g->post_weight); q.slot_post_b = place(g->post_bias);
     if (a->M > 0) {
         TimingScope timing(ADCDIFF_KIND_OTHER, a->M, a->D, 0, 0.0, (double)a->M * a->D * ((a->h ? 2.0 : 0.0) * st + (g->d_y ? st : 0) + 2.0 * sr + (g->d_x_new ? sr : 0)), stream);
-        const bool vec = vector_inputs(*a) && vector_rows(g->d_x_new, g->ld_d_x_new, sr) && vector_rows(g->d_y, g->ld_d_y, st) &&
-                         vector_rows(g->h, g->ld_h, st) && vector_rows(g->x, g->ld_x, sr) && vector_rows(g->gate, a->gate_rows > 1 ? g->ld_gate : 0, sg);
-        if (vec) backward_by_type<true>(q, c, a->dtype, a->stream_dtype, stream);
-        else backward_by_type<false>(q, c, a->dtype, a->stream_dtype, stream);
+        rc = vector_backward(*a, *g) ? backward_by_type<true>(q, c, a->dtype, a->stream_dtype, stream) : backward_by_type<false>(q, c, a->dtype, a->stream_dtype, stream);
+        if (rc != ADCDIFF_OK) return rc;
         rc = check_launch("residual_norm_backward");
         if (rc != ADCDIFF_OK) return rc;
     }

@@ -1,10 +1,14 @@
 // Rows held in the registers of a team of threads: loads, stores and sums shared by the row kernels (norms, row quantiser).
 #pragma once
+#include <atomic>
+
 #include "common.h"
 
 namespace adcdiff {
 
-constexpr int kThreads = 256;   // threads of a row kernel's workgroup (more where one row needs a wider team)
+constexpr int kThreads = 256;   // threads of a row kernel's workgroup: as many teams as fit, or one team where a row needs a wider one
+template <int TPR>
+constexpr int threads_for() { return TPR >= kThreads ? TPR : kThreads / TPR * TPR; }
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v) { return (float)v; }
@@ -134,7 +138,7 @@ struct TeamSum {
 #pragma unroll
         for (int n = 0; n < N; ++n) s[n] = lanes_allsum<(TPR < 64 ? TPR : 64)>(s[n], 0);
         if constexpr (TPR > 64) {
-            constexpr int WAVES = TPR / 64, SLOTS = (TPR > kThreads ? TPR : kThreads) / 64;
+            constexpr int WAVES = TPR / 64, SLOTS = threads_for<TPR>() / 64;
             float* buf = red + half * SLOTS * N;
             const int wave = tid >> 6;
             if ((tid & 63) == 0) {
@@ -160,5 +164,17 @@ inline int type_size(int dtype) { return dtype == ADCDIFF_BF16 ? 2 : 4; }
 
 // rows on 16-byte boundaries (vector accesses), or absent
 inline bool vector_rows(const void* p, long long ld, int size) { return !p || (aligned16(p) && (ld * size & 15) == 0); }
+
+// Lets a kernel use `bytes` of dynamic LDS on the current device; done[device] remembers that it was said
+inline int allow_lds(const char* who, const void* kernel, int bytes, std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess || dev < 0 || dev >= 64) return fail(ADCDIFF_E_LAUNCH, "%s: hipGetDevice: %s (device %d)", who, hipGetErrorString(e), dev);
+    if (done[dev].load(std::memory_order_relaxed)) return ADCDIFF_OK;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return fail(ADCDIFF_E_LAUNCH, "%s: hipFuncSetAttribute: %s", who, hipGetErrorString(e));
+    done[dev].store(true, std::memory_order_relaxed);
+    return ADCDIFF_OK;
+}
 
 }  // namespace adcdiff

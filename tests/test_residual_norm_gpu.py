@@ -211,6 +211,23 @@ def test_offsets_past_32_bits():
     assert torch.equal(p[0], q[0]) and torch.equal(p[1], q[1])
 
 
+@pytest.mark.parametrize("D", [96, 777, 2048, 8192])
+def test_stream_in_place(D):
+    """x_new over x and y over h (C ABI), with rows enough for every workgroup to take several"""
+    import ctypes as C
+    from adcdiff import _lib
+    s = _inputs(9001, D, BF, F, F, 1, "rms", "layer")
+    want = ops.residual_norm(s["h"], s["x"], gate=s["gate"], post_norm="rms", pre_norm="layer", residual_scale=0.5)
+    a = _lib.ResidualNormArgs()
+    a.M, a.D, a.dtype, a.stream_dtype, a.gate_dtype, a.post_norm, a.pre_norm, a.gate_rows = 9001, D, 1, 0, 0, 1, 2, 1
+    a.h = a.y = s["h"].data_ptr()
+    a.x = a.x_new = s["x"].data_ptr()
+    a.gate, a.residual_scale, a.eps = s["gate"].data_ptr(), 0.5, 1e-6
+    a.ldh = a.ldx = a.ldg = a.ldx_new = a.ldy = D
+    _lib.check(_lib.load().adcdiff_residual_norm(C.byref(a), torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(s["x"], want[0]) and torch.equal(s["h"], want[1])
+
+
 def test_other_stream_and_graphs():
     s = _inputs(257, 1024, BF, F, F, 1, "rms", "rms")
     args = [s[k] for k in NAMES]
