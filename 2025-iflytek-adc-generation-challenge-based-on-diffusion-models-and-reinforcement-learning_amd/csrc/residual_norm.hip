@@ -74,14 +74,6 @@ __device__ __forceinline__ void load_vector(const float* p, float absent, int t,
     for (int e = 0; e < 8; ++e) v[e] = p ? v[e] : absent;
 }
 
-// A thread's team: the same for a whole wave unless teams are narrower, which keeps row addresses out of the vector registers
-template <int TPR>
-__device__ __forceinline__ int team_of(int tid) {
-    if constexpr (TPR >= kThreads) return 0;
-    else if constexpr (TPR >= 64) return __builtin_amdgcn_readfirstlane(tid / TPR);
-    else return tid / TPR;
-}
-
 // bit e: element e of the thread lies inside the row
 template <bool VEC, int TPR>
 __device__ __forceinline__ unsigned inside(int t, int D) {
@@ -119,7 +111,7 @@ template <typename T, typename R, bool VEC, int TPR>
 __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_kernel(const ResNormParams p) {
     constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
     __shared__ float red[2 * (THREADS / 64)];
-    const int tid = threadIdx.x, t = TEAMS == 1 ? tid : tid % TPR, team = team_of<TPR>(tid), D = p.D;
+    const int tid = threadIdx.x, t = TEAMS == 1 ? tid : tid % TPR, team = TEAMS == 1 ? 0 : tid / TPR, D = p.D;
     const unsigned in = inside<VEC, TPR>(t, D);
     const bool one_gate = p.gate && p.gate_share >= p.M, row_gate = p.gate && !one_gate;
     RawRow<R, VEC, TPR> rx;
@@ -247,7 +239,7 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
     __shared__ float joined[TEAMS > 1 ? THREADS / 64 * TPW * 8 : 1];
     extern __shared__ __attribute__((aligned(16))) float wide[];     // kWideSums bytes where WIDE
     const ResNormParams& p = q.f;
-    const int tid = threadIdx.x, t = TEAMS == 1 ? tid : tid % TPR, team = team_of<TPR>(tid), D = p.D;
+    const int tid = threadIdx.x, t = TEAMS == 1 ? tid : tid % TPR, team = TEAMS == 1 ? 0 : tid / TPR, D = p.D;
     const unsigned in = inside<VEC, TPR>(t, D);
     TeamSum<TPR, 2> sum(red);
     ColumnSums<WIDE> a_pre_w, a_pre_b, a_post_w, a_post_b;
@@ -497,7 +489,7 @@ int check_args(const char* who, const adcdiff_residual_norm_args* a) {
         return fail(ADCDIFF_E_BADARG, "%s: a gate, a post norm or a residual scale without h", who);
     if ((!a->post_norm && (a->post_weight || a->post_bias)) || (!a->pre_norm && (a->pre_weight || a->pre_bias)))
         return fail(ADCDIFF_E_BADARG, "%s: a weight or bias without its norm", who);
-    if (a->gate && (a->gate_rows < 1 || a->M % a->gate_rows != 0) && a->M > 0)
+    if (a->gate && (a->gate_rows < (a->M > 0) || (a->M > 0 && a->M % a->gate_rows != 0)))
         return fail(ADCDIFF_E_BADARG, "%s: %d gate rows do not divide %d rows", who, a->gate_rows, a->M);
     if ((a->h && a->ldh < a->D) || (a->x && a->ldx < a->D) || (a->gate && a->gate_rows > 1 && a->ldg != 0 && a->ldg < a->D))
         return fail(ADCDIFF_E_BADARG, "%s: a row pitch below %d columns", who, a->D);
@@ -523,26 +515,35 @@ bool vector_inputs(const adcdiff_residual_norm_args& a) {
            vector_rows(a.post_weight, 0, 4) && vector_rows(a.post_bias, 0, 4) && vector_rows(a.pre_weight, 0, 4) && vector_rows(a.pre_bias, 0, 4);
 }
 
-// Threads for a row of D columns, eight each.  Rows that are read in single elements take the next power of two.
-int team_width(int D, bool vec) {
+// Threads for a row of D columns, eight each.  Rows that are read in single elements take the next power of two.  Vector rows have more sizes
+// where both sides were measured (67 M elements, bfloat16): 32 instead of 64 threads at D = 136 (forward 36.8 -> 21.6 us, backward 75 -> 52 us),
+// 768 instead of 1024 at D = 6000 (148 -> 131 us, 970 -> 230 us).  192, 320 and 384 belong to the backward pass: fewer idle threads hold
+// registers there (D = 2056: 298 with 512 threads -> 266 us, D = 1032: 288 -> 283, float32 335 -> 319), while the forward pass gains nothing
+// from them (D = 2056: 166 -> 176 us; D = 3000: 124 -> 139 us).
+int team_width(int D, bool vec, bool backward) {
     const int waves = (D + 511) / 512;
     if (vec && D <= 128) return 16;
     if (vec && D <= 256) return 32;
-    if (!vec) return waves <= 1 ? 64 : waves <= 2 ? 128 : waves <= 4 ? 256 : waves <= 8 ? 512 : 1024;
-    return 64 * (waves <= 6 ? waves : waves <= 8 ? 8 : waves <= 12 ? 12 : 16);
+    if (vec && backward && waves <= 6) return 64 * waves;
+    if (vec && waves > 8 && waves <= 12) return 768;
+    return waves <= 1 ? 64 : waves <= 2 ? 128 : waves <= 4 ? 256 : waves <= 8 ? 512 : 1024;
 }
 
 // Calls f(std::integral_constant<int, threads>) for the team of a row
-template <bool VEC, typename F>
+template <bool VEC, bool BACKWARD, typename F>
 void for_width(int tpr, F f) {
     if constexpr (VEC) {
         switch (tpr) {
             case 16: return f(std::integral_constant<int, 16>());
             case 32: return f(std::integral_constant<int, 32>());
+            case 768: return f(std::integral_constant<int, 768>());
+        }
+    }
+    if constexpr (VEC && BACKWARD) {
+        switch (tpr) {
             case 192: return f(std::integral_constant<int, 192>());
             case 320: return f(std::integral_constant<int, 320>());
             case 384: return f(std::integral_constant<int, 384>());
-            case 768: return f(std::integral_constant<int, 768>());
         }
     }
     switch (tpr) {
@@ -563,7 +564,7 @@ void launch_forward(const ResNormParams& p, hipStream_t stream) {
 
 template <typename T, typename R, bool VEC>
 void forward_by_width(const ResNormParams& p, hipStream_t stream) {
-    for_width<VEC>(team_width(p.D, VEC), [&](auto tpr) { launch_forward<T, R, VEC, decltype(tpr)::value>(p, stream); });
+    for_width<VEC, false>(team_width(p.D, VEC, false), [&](auto tpr) { launch_forward<T, R, VEC, decltype(tpr)::value>(p, stream); });
 }
 
 template <bool VEC>
@@ -587,7 +588,7 @@ constexpr int kMaxGroups = 512;
 
 Cut cut_rows(int M, int D, bool vec, int gate_rows, bool gate_grad, int vectors) {
     Cut c{};
-    c.tpr = team_width(D, vec);
+    c.tpr = team_width(D, vec, true);
     c.teams = c.tpr >= kThreads ? 1 : kThreads / c.tpr;
     c.vectors = vectors;
     c.gate_sum = gate_grad && gate_rows > 0 && M / std::max(gate_rows, 1) != 1;
@@ -615,7 +616,7 @@ size_t workspace_floats(const Cut& c, int D) {
 template <typename T, typename R, bool VEC>
 int backward_by_width(const ResNormGradParams& q, const Cut& c, hipStream_t stream) {
     int rc = ADCDIFF_OK;
-    for_width<VEC>(c.tpr, [&](auto tpr) {
+    for_width<VEC, true>(c.tpr, [&](auto tpr) {
         constexpr int TPR = decltype(tpr)::value;
         const auto kernel = &residual_norm_grad_kernel<T, R, VEC, TPR>;
         constexpr int lds = TPR == 1024 ? kWideSums : 0;
