@@ -247,7 +247,8 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
     a_pre_b.init(wide + 8192, tid);
     a_post_w.init(wide + 2 * 8192, tid);
     a_post_b.init(wide + 3 * 8192, tid);
-    // Teams of 768 and 1024 have 168 and 128 registers per thread: they load the weights where they are used, and no row ahead.
+    // Teams of 768 and 1024 threads have 168 and 128 registers per thread.  They load weights where they are used and no row ahead, and a row's raw
+    // values end with its turn (kept over turns they spilled: 8192 x 8192 bfloat16 461 us against 223 us).
     constexpr bool LEAN = TPR > 512;
     float post_w[8], post_b[8], pre_w[8];
     if constexpr (!LEAN) {
@@ -278,7 +279,7 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
                 if (q.d_y) ry.load(static_cast<const T*>(q.d_y) + row * q.ld_dy, t, D);
                 if (p.gate) {
                     const long long g = row_gate ? row : row / p.gate_share;
-                    if (g != gate_row) rg.load(p.gate, p.gate_bf16, g * p.ldg, t, D);
+                    if (LEAN || g != gate_row) rg.load(p.gate, p.gate_bf16, g * p.ldg, t, D);
                     gate_row = g;
                 }
             }
@@ -291,7 +292,10 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
             const long long row = first + r;
             const bool live = row < last;
             float d[8], v[8], u[8], uhat[8], g[8], s[2];
-            if constexpr (LEAN) fetch(row);
+            if constexpr (LEAN) {
+                rx.clear(); rd.clear(); rh.clear(); ry.clear(); rg.clear();
+                fetch(row);
+            }
             const f32x4 st = rs;
             rd.get(d);
             rx.get(v);
@@ -515,18 +519,17 @@ bool vector_inputs(const adcdiff_residual_norm_args& a) {
            vector_rows(a.post_weight, 0, 4) && vector_rows(a.post_bias, 0, 4) && vector_rows(a.pre_weight, 0, 4) && vector_rows(a.pre_bias, 0, 4);
 }
 
-// Threads for a row of D columns, eight each.  Rows that are read in single elements take the next power of two.  Vector rows have more sizes
-// where both sides were measured (67 M elements, bfloat16): 32 instead of 64 threads at D = 136 (forward 36.8 -> 21.6 us, backward 75 -> 52 us),
-// 768 instead of 1024 at D = 6000 (148 -> 131 us, 970 -> 230 us).  192, 320 and 384 belong to the backward pass: fewer idle threads hold
-// registers there (D = 2056: 298 with 512 threads -> 266 us, D = 1032: 288 -> 283, float32 335 -> 319), while the forward pass gains nothing
-// from them (D = 2056: 166 -> 176 us; D = 3000: 124 -> 139 us).
+// Threads for a row of D columns, eight each: a power of two, and more sizes where both sides were measured (67 M elements, bfloat16; f / b: forward,
+// backward).  768 instead of 1024: D = 6000 f 148 -> 131 us, b 970 -> 230 us, single elements D = 5001 f 219 -> 209, b 534 -> 335.  Rows read in
+// vectors: 32 instead of 64 at D = 136, f 36.8 -> 21.6, b 75 -> 52; and in the backward pass 192, 320 and 384, where fewer idle threads hold
+// registers (D = 2056: b 298 -> 266 us, D = 1032: 288 -> 283, in float32 335 -> 319), while the forward pass loses with them (D = 2056: 166 -> 176 us,
+// D = 3000: 124 -> 139 us).
 int team_width(int D, bool vec, bool backward) {
     const int waves = (D + 511) / 512;
     if (vec && D <= 128) return 16;
     if (vec && D <= 256) return 32;
     if (vec && backward && waves <= 6) return 64 * waves;
-    if (vec && waves > 8 && waves <= 12) return 768;
-    return waves <= 1 ? 64 : waves <= 2 ? 128 : waves <= 4 ? 256 : waves <= 8 ? 512 : 1024;
+    return waves <= 1 ? 64 : waves <= 2 ? 128 : waves <= 4 ? 256 : waves <= 8 ? 512 : waves <= 12 ? 768 : 1024;
 }
 
 // Calls f(std::integral_constant<int, threads>) for the team of a row
@@ -536,7 +539,6 @@ void for_width(int tpr, F f) {
         switch (tpr) {
             case 16: return f(std::integral_constant<int, 16>());
             case 32: return f(std::integral_constant<int, 32>());
-            case 768: return f(std::integral_constant<int, 768>());
         }
     }
     if constexpr (VEC && BACKWARD) {
@@ -551,6 +553,7 @@ void for_width(int tpr, F f) {
         case 128: return f(std::integral_constant<int, 128>());
         case 256: return f(std::integral_constant<int, 256>());
         case 512: return f(std::integral_constant<int, 512>());
+        case 768: return f(std::integral_constant<int, 768>());
         default: return f(std::integral_constant<int, 1024>());
     }
 }
