@@ -220,45 +220,63 @@ __device__ __forceinline__ i32x4 load_chunk(const int8_t* __restrict__ row, int 
     return v;
 }
 
-// Eight consecutive outputs of row m from column n on (fewer at the right edge)
+// Eight consecutive outputs of row m from column n on (fewer at the right edge): their scales, biases and residual (which the few-row kernel loads before
+// the sums are there), and the outputs
 template <typename Out>
-__device__ __forceinline__ void finish8(const I8Params& p, int m, int n, const i32x4& lo, const i32x4& hi) {
-    const float sa = p.a_scale[m];
-    const Out* res = static_cast<const Out*>(p.residual) + (long long)m * p.ldr + n;
-    Out* out = static_cast<Out*>(p.out) + (long long)m * p.ldo + n;
+struct Finish8 {
     typedef Out Eight __attribute__((ext_vector_type(8)));
     typedef Eight EightAt16 __attribute__((aligned(16)));
-    if (p.vec) {   // N is a multiple of 8 and rows of out and residual lie on 16-byte boundaries
-        float w[8], b[8] = {};
-        Eight r, o;
-        const f32x4_any* pw = reinterpret_cast<const f32x4_any*>(p.w_scale + n);
+    f32x4 w0, w1, b0, b1;
+    float sa;
+    Eight r;
+    __device__ __forceinline__ void load(const I8Params& p, int m, int n) {
+        const Out* res = static_cast<const Out*>(p.residual) + (long long)m * p.ldr + n;
+        sa = p.a_scale[m];
+        b0 = b1 = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.vec) {   // N is a multiple of 8 and rows of out and residual lie on 16-byte boundaries
+            const f32x4_any* pw = reinterpret_cast<const f32x4_any*>(p.w_scale + n);
+            w0 = pw[0];
+            w1 = pw[1];
+            if (p.bias) {
+                const f32x4_any* pb = reinterpret_cast<const f32x4_any*>(p.bias + n);
+                b0 = pb[0];
+                b1 = pb[1];
+            }
+            if (p.residual) r = *reinterpret_cast<const EightAt16*>(res);
+        } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) { w[c] = pw[0][c]; w[4 + c] = pw[1][c]; }
-        if (p.bias) {
-            const f32x4_any* pb = reinterpret_cast<const f32x4_any*>(p.bias + n);
+            for (int c = 0; c < 4; ++c) {
+                const bool in = n + c < p.N, in4 = n + 4 + c < p.N;
+                w0[c] = in ? p.w_scale[n + c] : 0.0f;
+                w1[c] = in4 ? p.w_scale[n + 4 + c] : 0.0f;
+                b0[c] = in && p.bias ? p.bias[n + c] : 0.0f;
+                b1[c] = in4 && p.bias ? p.bias[n + 4 + c] : 0.0f;
+            }
+            if (p.residual) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) { b[c] = pb[0][c]; b[4 + c] = pb[1][c]; }
+                for (int c = 0; c < 8; ++c) r[c] = n + c < p.N ? res[c] : (Out)0.0f;
+            }
         }
-        if (p.residual) r = *reinterpret_cast<const EightAt16*>(res);
+    }
+    __device__ __forceinline__ void store(const I8Params& p, int m, int n, const i32x4& lo, const i32x4& hi) const {
+        Out* out = static_cast<Out*>(p.out) + (long long)m * p.ldo + n;
+        Eight o;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            float v = fmaf((float)(c < 4 ? lo[c & 3] : hi[c & 3]) * sa, w[c], b[c]);
+            float v = c < 4 ? fmaf((float)lo[c & 3] * sa, w0[c & 3], b0[c & 3]) : fmaf((float)hi[c & 3] * sa, w1[c & 3], b1[c & 3]);
             if (p.residual) v += (float)r[c];
             if (p.act) v = silu_fast(v);
             o[c] = (Out)v;
         }
-        *reinterpret_cast<EightAt16*>(out) = o;
-    } else {
+        if (p.vec) {
+            *reinterpret_cast<EightAt16*>(out) = o;
+        } else {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            if (n + c >= p.N) break;
-            float v = fmaf((float)(c < 4 ? lo[c & 3] : hi[c & 3]) * sa, p.w_scale[n + c], p.bias ? p.bias[n + c] : 0.0f);
-            if (p.residual) v += (float)res[c];
-            if (p.act) v = silu_fast(v);
-            out[c] = (Out)v;
+            for (int c = 0; c < 8; ++c)
+                if (n + c < p.N) out[c] = o[c];
         }
     }
-}
+};
 
 // ---- BM x BN tile through a ring of LDS stages ------------------------------------------------------------------------------------
 // Eight waves (2 x 4); a stage is 128 columns of the tile's rows, filled by LDS-DMA (64 lanes x 16 bytes = eight rows of 128 bytes per
@@ -349,8 +367,10 @@ __global__ __launch_bounds__(512) void gemm_i8_ring_kernel(const I8Params p) {
 #pragma unroll
     for (int e = tid; e < BM * BN / 8; e += 512) {
         const int r = e / (BN / 8), c = e % (BN / 8) * 8;
-        if (m0 + r < p.M && n0 + c < p.N)
-            finish8<Out>(p, m0 + r, n0 + c, *reinterpret_cast<const i32x4*>(sums + r * PITCH + c), *reinterpret_cast<const i32x4*>(sums + r * PITCH + c + 4));
+        if (m0 + r >= p.M || n0 + c >= p.N) continue;
+        Finish8<Out> finish;
+        finish.load(p, m0 + r, n0 + c);
+        finish.store(p, m0 + r, n0 + c, *reinterpret_cast<const i32x4*>(sums + r * PITCH + c), *reinterpret_cast<const i32x4*>(sums + r * PITCH + c + 4));
     }
 }
 
@@ -358,6 +378,7 @@ __global__ __launch_bounds__(512) void gemm_i8_ring_kernel(const I8Params p) {
 // A unit is 128 columns (a cache line of a row, two MFMA steps).  Wave w takes units w, w + WAVES, ..; its fragments go from memory to
 // registers (no LDS stage, no barrier), DEPTH units in flight.  The partial sums meet in LDS; integer sums do not depend on their
 // order.  Bound by the latency of one or two rounds of loads; the tile is kept small so that enough workgroups share the weights' bytes.
+// 1 x 2048 x 2048 in 4.1 us (the weights' 4 MB at 1.0 TB/s), 32 x 2048 x 4096 in 6.8 us.
 template <typename Out, int BM, int BN, int WAVES, int DEPTH>
 __global__ __launch_bounds__(64 * WAVES) void gemm_i8_split_kernel(const I8Params p) {
     constexpr int TM = BM / 16, TN = BN / 16, PITCH = BN + 4;
@@ -413,6 +434,13 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_i8_split_kernel(const I8Param
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d)
         if (wave + d * WAVES < units) load(d, wave + d * WAVES);
+    // the outputs of this thread, eight of a row, and what they need beside the sums: on its way together with the codes
+    // (1 x 2048 x 2048: 4.30 -> 4.09 us, 64 x 2048 x 2048: 6.02 -> 5.57 us)
+    static_assert(BM * BN / 8 <= 64 * WAVES, "one round of outputs");
+    const int er = tid / (BN / 8), ec = tid % (BN / 8) * 8;
+    const bool mine = er < BM && m0 + er < p.M && n0 + ec < p.N;
+    Finish8<Out> finish;
+    if (mine) finish.load(p, m0 + er, n0 + ec);
     for (int u = wave; u < units; u += DEPTH * WAVES) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
@@ -429,16 +457,14 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_i8_split_kernel(const I8Param
         for (int j = 0; j < TN; ++j)
             *reinterpret_cast<i32x4*>(&part[wave][(16 * i + (lane & 15)) * PITCH + 16 * j + 4 * (lane >> 4)]) = acc[i][j];
     __syncthreads();
-    for (int e = tid; e < BM * BN / 8; e += 64 * WAVES) {
-        const int r = e / (BN / 8), c = e % (BN / 8) * 8;
-        if (m0 + r >= p.M || n0 + c >= p.N) continue;
+    if (mine) {
         i32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-            lo += *reinterpret_cast<const i32x4*>(&part[w][r * PITCH + c]);
-            hi += *reinterpret_cast<const i32x4*>(&part[w][r * PITCH + c + 4]);
+            lo += *reinterpret_cast<const i32x4*>(&part[w][er * PITCH + ec]);
+            hi += *reinterpret_cast<const i32x4*>(&part[w][er * PITCH + ec + 4]);
         }
-        finish8<Out>(p, m0 + r, n0 + c, lo, hi);
+        finish.store(p, m0 + er, n0 + ec, lo, hi);
     }
 }
 

@@ -248,7 +248,7 @@ int check_tensors(const char* who, const adcdiff_grad_tensor* ts, int n, bool cl
             return fail(ADCDIFF_E_BADARG, "%s: tensor %d is not aligned to its elements", who, i);
         *chunks += chunks_of(t.numel);
     }
-    if (*chunks > 0x7fffffffLL) return fail(ADCDIFF_E_BADARG, "%s: too many elements", who);
+    if (*chunks > 0xffffffLL) return fail(ADCDIFF_E_BADARG, "%s: too many elements", who);
     return ADCDIFF_OK;
 }
 

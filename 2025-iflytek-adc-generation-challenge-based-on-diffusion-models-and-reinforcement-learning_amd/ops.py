@@ -397,7 +397,7 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, ou
 
 def quantize_rows(x):
     """(codes int8 [M, K], scale float32 [M]) of the rows of x [M, K] (float32 or bfloat16): scale = max|row| / 127, codes =
-    row / scale rounded half to even, exactly.  For activations (a scale per token) and weights [N, K] (a scale per output channel)
+    row * 127 / max|row| rounded half to even, exactly.  For activations (a scale per token) and weights [N, K] (a scale per output channel)
     alike.  The codes' rows start on 16-byte boundaries, as gemm_int8 reads them.  A row of zeros has scale 0; a row with a NaN or an
     infinity has scale NaN, so that every product with it is NaN."""
     return _call("quantize_rows", x)

@@ -351,7 +351,7 @@ int adcdiff_clip_adamw_step_noalloc(const adcdiff_opt_tensor* tensors, int n_ten
  * norm kinds: 0 none (N(v) = v), 1 rms (no [mean]), 2 layer.  Arithmetic in float32, one rounding per output; y is formed from the
  * unrounded x_new.
  *   h, y           [M, ld >= D] in dtype;  h NULL: x_new = x, only y = N_pre(x) is formed (no gate, no post norm, residual_scale 1)
- *   x, x_new       [M, ld >= D] in stream_dtype; x_new NULL: not written.  x_new may alias x, and y may alias h
+ *   x, x_new       [M, ld >= D] in stream_dtype; x_new NULL: not written.  x_new may alias x, and y may alias h (the same rows)
  *   gate           [gate_rows, ldg] in gate_dtype, or NULL; gate_rows divides M and row r reads gate row r / (M / gate_rows); ldg = 0
  *                  repeats one row
  *   weights, biases [D] float32, each optional
