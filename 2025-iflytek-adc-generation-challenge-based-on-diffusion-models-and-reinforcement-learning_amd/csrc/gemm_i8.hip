@@ -10,7 +10,7 @@ namespace adcdiff {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 u32x4_any __attribute__((aligned(1)));   // global memory takes 16-byte loads at any address
+typedef u32x4 u32x4_byte __attribute__((aligned(1)));   // global memory takes 16-byte loads at any address
 
 // ------------------------------------------------------------------ codes of rows
 // A code is rne(x * 127 / top), exactly.
@@ -48,6 +48,7 @@ struct RowScale {
             }
         }
         if (exact) {
+            asm volatile("");   // a branch to stay: computed in any case and selected, 65536 x 512 takes 38 us instead of 19
 #pragma unroll
             for (int e = 0; e < N; ++e) q[e] = (int)rint((double)x[e] * 127.0 / (double)top);
         }
@@ -56,7 +57,7 @@ struct RowScale {
             for (int e = 0; e < N; ++e) q[e] = 0;
         }
     }
-    __device__ __forceinline__ int code(float x) const {   // of either type
+    __device__ __forceinline__ int code(float x) const {   // of either type (rows of more than 8192)
         const float v[1] = {x};
         int q[1];
         codes<false>(v, q);
@@ -81,44 +82,47 @@ __device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red, int tid)
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-// one row per team, held in registers between the maximum and the codes; bound by HBM (65536 x 2048 bfloat16 79 us, 403 MB at 5.1 TB/s; 4096 x 2048
-// 7.2 us) and by latency below
-template <typename T, bool VEC, int TPR, int V>
+// One row per team, held in registers between the maximum and the codes; bound by HBM (65536 x 2048 bfloat16 79 us, 403 MB at 5.1 TB/s; 4096 x 2048
+// 7.2 us) and by latency below.  PAIRS: rows of q start on 8-byte boundaries and eight codes are one store, those behind K among them.
+template <typename T, RowShape SHAPE, bool PAIRS, int TPR, int V>
 __global__ __launch_bounds__(threads_for<TPR>()) void quantize_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int8_t* __restrict__ q,
-                                                                 long long ldq, float* __restrict__ scale) {
-    constexpr int E = 8 * V, THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
+                                                                           long long ldq, float* __restrict__ scale) {
+    constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
     __shared__ uint32_t red[THREADS / 64];
     const int tid = threadIdx.x, t = tid % TPR;
     // a team wider than a wave is alone in its workgroup, so the barriers of the maximum are met by every thread
     for (long long row = (long long)blockIdx.x * TEAMS + tid / TPR; row < M; row += (long long)gridDim.x * TEAMS) {
-        float v[E];
-        load_row<T, VEC, TPR, E>(x + row * ldx, t, K, v);
+        float v[V][8];
         uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) top = max(top, abs_bits(v[e]));
+        for (int j = 0; j < V; ++j) {
+            RawRow<T, SHAPE> raw;
+            raw.load(x + row * ldx, j * TPR + t, K);
+            raw.get(v[j]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[j][e]));
+        }
         const RowScale s(team_max<TPR>(top, red, tid));
         int8_t* out = q + row * ldq;
-        if constexpr (VEC) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const int c = (j * TPR + t) * 8;
-                if (c < Kp) {
-                    float part[8];
-                    int code[8];
+        for (int j = 0; j < V; ++j) {
+            const int c = (j * TPR + t) * 8;
+            if (c < Kp) {
+                int code[8];
+                s.template codes<sizeof(T) == 2>(v[j], code);
+                uint64_t w = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) part[i] = v[j * 8 + i];
-                    s.template codes<sizeof(T) == 2>(part, code);
-                    uint32_t w[2] = {0, 0};
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)code[i] & 0xffu) << (8 * (i & 3));
-                    *reinterpret_cast<uint2*>(out + c) = uint2{w[0], w[1]};
+                for (int i = 0; i < 8; ++i) w |= (uint64_t)((uint32_t)code[i] & 0xffu) << (8 * i);
+                if constexpr (SHAPE == kMoved) {   // the last thread's own columns are the last of its eight
+                    if (c < K && c + 8 > K) w >>= 8 * (c + 8 - K);
                 }
-            }
-        } else {
+                if constexpr (PAIRS) {
+                    *reinterpret_cast<uint64_t*>(out + c) = w;
+                } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int c = e * TPR + t;
-                if (c < Kp) out[c] = (int8_t)s.code(v[e]);
+                    for (int i = 0; i < 8; ++i)
+                        if (c + i < Kp) out[c + i] = (int8_t)(w >> (8 * i));
+                }
             }
         }
         if (t == 0) scale[row] = s.scale;
@@ -141,23 +145,44 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(const T* __res
     }
 }
 
-template <typename T, bool VEC, int TPR, int V>
-void launch_quantize(const void* x, long long ldx, int M, int K, int Kp, int8_t* q, long long ldq, float* scale, hipStream_t stream) {
+struct QuantizeArgs {
+    const void* x;
+    long long ldx;
+    int M, K, Kp;
+    int8_t* q;
+    long long ldq;
+    float* scale;
+};
+
+template <typename T, RowShape SHAPE, bool PAIRS, int TPR, int V>
+void launch_quantize(const QuantizeArgs& a, hipStream_t stream) {
     constexpr int threads = threads_for<TPR>(), teams = threads / TPR;
-    hipLaunchKernelGGL((quantize_rows_kernel<T, VEC, TPR, V>), dim3((unsigned)std::min(((long long)M + teams - 1) / teams, 1LL << 20)), dim3(threads), 0, stream,
-                       static_cast<const T*>(x), ldx, M, K, Kp, q, ldq, scale);
+    hipLaunchKernelGGL((quantize_rows_kernel<T, SHAPE, PAIRS, TPR, V>), dim3((unsigned)std::min(((long long)a.M + teams - 1) / teams, 1LL << 20)), dim3(threads), 0, stream,
+                       static_cast<const T*>(a.x), a.ldx, a.M, a.K, a.Kp, a.q, a.ldq, a.scale);
 }
 
-template <typename T, bool VEC>
-void quantize_by_width(const void* x, long long ldx, int M, int K, int Kp, int8_t* q, long long ldq, float* scale, hipStream_t stream) {
-    if (Kp <= 128) launch_quantize<T, VEC, 16, 1>(x, ldx, M, K, Kp, q, ldq, scale, stream);
-    else if (Kp <= 512) launch_quantize<T, VEC, 64, 1>(x, ldx, M, K, Kp, q, ldq, scale, stream);
-    // few rows: the latency of one row counts (32 x 2048: 256 threads 2.5 us, 128 threads 2.8); many: the barriers of wide teams (65536 x 2048: 87, 75 us)
-    else if (Kp <= 2048 && M < 2048) launch_quantize<T, VEC, 256, 1>(x, ldx, M, K, Kp, q, ldq, scale, stream);
-    else if (Kp <= 2048) launch_quantize<T, VEC, 128, 2>(x, ldx, M, K, Kp, q, ldq, scale, stream);
-    else if (Kp <= 4096) launch_quantize<T, VEC, 256, 2>(x, ldx, M, K, Kp, q, ldq, scale, stream);
-    else if (Kp <= 8192) launch_quantize<T, VEC, 512, 2>(x, ldx, M, K, Kp, q, ldq, scale, stream);
-    else hipLaunchKernelGGL((quantize_long_rows_kernel<T>), dim3(std::min(M, 1 << 20)), dim3(1024), 0, stream, static_cast<const T*>(x), ldx, M, K, Kp, q, ldq, scale);
+template <typename T, RowShape SHAPE, bool PAIRS>
+void quantize_by_width(const QuantizeArgs& a, hipStream_t stream) {
+    if (a.Kp <= 128) return launch_quantize<T, SHAPE, PAIRS, 16, 1>(a, stream);
+    if constexpr (SHAPE != kTiny) {
+        if (a.Kp <= 512) return launch_quantize<T, SHAPE, PAIRS, 64, 1>(a, stream);
+        // few rows: the latency of one row counts (32 x 2048: 256 threads 2.5 us, 128 threads 2.8); many: the barriers of wide teams (65536 x 2048: 87, 75 us)
+        if (a.Kp <= 2048 && a.M < 2048) return launch_quantize<T, SHAPE, PAIRS, 256, 1>(a, stream);
+        if (a.Kp <= 2048) return launch_quantize<T, SHAPE, PAIRS, 128, 2>(a, stream);
+        if (a.Kp <= 4096) return launch_quantize<T, SHAPE, PAIRS, 256, 2>(a, stream);
+        if (a.Kp <= 8192) return launch_quantize<T, SHAPE, PAIRS, 512, 2>(a, stream);
+        hipLaunchKernelGGL((quantize_long_rows_kernel<T>), dim3(std::min(a.M, 1 << 20)), dim3(1024), 0, stream, static_cast<const T*>(a.x), a.ldx, a.M, a.K, a.Kp, a.q,
+                           a.ldq, a.scale);
+    }
+}
+
+template <typename T, bool PAIRS>
+void quantize_by_shape(const QuantizeArgs& a, hipStream_t stream) {
+    switch (row_shape(a.K)) {
+        case kWhole: return quantize_by_width<T, kWhole, PAIRS>(a, stream);
+        case kMoved: return quantize_by_width<T, kMoved, PAIRS>(a, stream);
+        case kTiny: return quantize_by_width<T, kTiny, PAIRS>(a, stream);
+    }
 }
 
 struct PitchParams {
@@ -177,7 +202,7 @@ __global__ __launch_bounds__(256) void pitch_rows_kernel(const PitchParams p) {
     const int n = (int)min(16LL, max(0LL, (long long)c.K - col));
     u32x4 w = {0, 0, 0, 0};
     if (n == 16) {
-        w = *reinterpret_cast<const u32x4_any*>(s);
+        w = *reinterpret_cast<const u32x4_byte*>(s);
     } else {
 #pragma unroll
         for (int b = 0; b < 15; ++b)
@@ -187,8 +212,6 @@ __global__ __launch_bounds__(256) void pitch_rows_kernel(const PitchParams p) {
 }
 
 // ------------------------------------------------------------------ product
-typedef f32x4 f32x4_any __attribute__((aligned(4)));   // vectors of scales and biases start at any element
-
 struct I8Params {
     const int8_t *a, *w;
     const float *a_scale, *w_scale, *bias;
@@ -694,13 +717,14 @@ extern "C" int adcdiff_quantize_rows(const void* x, long long ldx, int dtype, in
     hipStream_t stream = as_stream(stream_);
     const int Kp = (int)std::min<long long>(ldq, ((long long)K + 15) / 16 * 16);
     TimingScope timing(ADCDIFF_KIND_OTHER, M, K, 0, 0.0, (double)M * K * (type_size(dtype) + 1), stream);
-    const bool vec = K % 8 == 0 && Kp % 8 == 0 && vector_rows(x, ldx, type_size(dtype)) && reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
+    const bool pairs = Kp % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0;
+    const QuantizeArgs a{x, ldx, M, K, Kp, q, ldq, scale};
     if (dtype == ADCDIFF_BF16) {
-        if (vec) quantize_by_width<bf16_t, true>(x, ldx, M, K, Kp, q, ldq, scale, stream);
-        else quantize_by_width<bf16_t, false>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+        if (pairs) quantize_by_shape<bf16_t, true>(a, stream);
+        else quantize_by_shape<bf16_t, false>(a, stream);
     } else {
-        if (vec) quantize_by_width<float, true>(x, ldx, M, K, Kp, q, ldq, scale, stream);
-        else quantize_by_width<float, false>(x, ldx, M, K, Kp, q, ldq, scale, stream);
+        if (pairs) quantize_by_shape<float, true>(a, stream);
+        else quantize_by_shape<float, false>(a, stream);
     }
     return check_launch("quantize_rows");
 }

@@ -41,8 +41,6 @@ __device__ __forceinline__ int find_entry(const GradTable& g, int chunk) {
 }
 
 // Gradients are aligned to their element only (views into an arena); the memory system takes 16-byte accesses at any address.
-typedef f32x4 f32x4_any __attribute__((aligned(4)));
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 struct SumSquares {   // float64: any float32 gradient squares without overflow or underflow, and the sum is exact to 2^-53
     typedef double Acc;

@@ -3,7 +3,7 @@
 // The bracketed mean belongs to the layer norm; the rms norm has none.  All arithmetic is float32; h, y share one type, x, x' another,
 // the gate has its own, and each output is rounded once.  y is formed from the unrounded x'.
 //
-// A team of TPR threads owns a row and holds it in registers (V vectors of 8 columns per thread), so every pass over the row after the
+// A team of TPR threads owns a row and holds it in registers (8 columns per thread), so every pass over the row after the
 // first load is free; both kernels are bound by HBM.  Statistics are two-pass (mean, then centred squares) on those registers.
 #include <algorithm>
 #include <atomic>
@@ -21,6 +21,7 @@ struct ResNormParams {
     float* stats;                 // [M, 4]: post mean, 1 / post deviation, pre mean, 1 / pre deviation
     long long ldh, ldx, ldg, ldxn, ldy;
     int M, D, post, pre, gate_bf16, gate_share;   // gate_share: rows per gate row
+    int crossing;                 // x is overwritten in place and a row's last thread moves back over a wave's end
     float scale, eps, inv_d;
 };
 
@@ -37,25 +38,25 @@ struct ResNormGradParams {
 };
 
 // A gate row of either type
-template <bool VEC, int TPR>
+template <RowShape SHAPE>
 struct RawGate {
-    RawRow<float, VEC, TPR> f;
+    RawRow<float, SHAPE> f;
     __device__ __forceinline__ void clear() { f.clear(); }
     __device__ __forceinline__ void load(const void* gate, int bf16, long long offset, int t, int D) {
         if (bf16) {
-            RawRow<bf16_t, VEC, TPR> b;
+            RawRow<bf16_t, SHAPE> b;
             b.load(static_cast<const bf16_t*>(gate) + offset, t, D);
 #pragma unroll
-            for (int i = 0; i < RawRow<bf16_t, VEC, TPR>::N; ++i) f.r[i] = b.r[i];
+            for (int i = 0; i < RawRow<bf16_t, SHAPE>::N; ++i) f.r[i] = b.r[i];
         } else {
             f.load(static_cast<const float*>(gate) + offset, t, D);
         }
     }
     __device__ __forceinline__ void get(int bf16, float (&v)[8]) const {
         if (bf16) {
-            RawRow<bf16_t, VEC, TPR> b;
+            RawRow<bf16_t, SHAPE> b;
 #pragma unroll
-            for (int i = 0; i < RawRow<bf16_t, VEC, TPR>::N; ++i) b.r[i] = f.r[i];
+            for (int i = 0; i < RawRow<bf16_t, SHAPE>::N; ++i) b.r[i] = f.r[i];
             b.get(v);
         } else {
             f.get(v);
@@ -64,9 +65,9 @@ struct RawGate {
 };
 
 // a weight or bias, or what it is without one
-template <bool VEC, int TPR>
+template <RowShape SHAPE>
 __device__ __forceinline__ void load_vector(const float* p, float absent, int t, int D, float (&v)[8]) {
-    RawRow<float, VEC, TPR> r;
+    RawRow<float, SHAPE> r;
     r.clear();
     if (p) r.load(p, t, D);
     r.get(v);
@@ -74,17 +75,7 @@ __device__ __forceinline__ void load_vector(const float* p, float absent, int t,
     for (int e = 0; e < 8; ++e) v[e] = p ? v[e] : absent;
 }
 
-// bit e: element e of the thread lies inside the row
-template <bool VEC, int TPR>
-__device__ __forceinline__ unsigned inside(int t, int D) {
-    if constexpr (VEC) return t * 8 < D ? 0xffu : 0u;
-    unsigned m = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m |= e * TPR + t < D ? 1u << e : 0u;
-    return m;
-}
-
-// mean and 1 / sqrt(variance + eps) of the row in v (mean = 0 for the rms norm); elements outside the row are left out
+// mean and 1 / sqrt(variance + eps) of the row in v (mean = 0 for the rms norm); `in`: the elements that count
 template <typename Sum>
 __device__ __forceinline__ void row_stats(const float (&v)[8], int kind, unsigned in, int tid, float inv_d, float eps, Sum& sum, float& mean, float& inv) {
     float s[1] = {0.0f};
@@ -108,16 +99,16 @@ __device__ __forceinline__ void row_stats(const float (&v)[8], int kind, unsigne
 // A team of TPR threads per row, eight columns per thread; weights, biases and a gate shared by all rows stay in registers over the rows of a
 // workgroup, and the next row is on its way while the one in hand is reduced.
 // Bound by HBM: 65536 x 2048 bfloat16 with a gate for each row 267 us (1.34 GB at 5.0 TB/s), 4096 x 1024 float32 17 us; 32 x 512: 3.8 us, a latency.
-template <typename T, typename R, bool VEC, int TPR>
+template <typename T, typename R, RowShape SHAPE, int TPR>
 __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_kernel(const ResNormParams p) {
     constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
     __shared__ float red[2 * (THREADS / 64)];
     const int tid = threadIdx.x, t = TEAMS == 1 ? tid : tid % TPR, team = TEAMS == 1 ? 0 : tid / TPR, D = p.D;
-    const unsigned in = inside<VEC, TPR>(t, D);
+    const unsigned in = own_columns<SHAPE>(t, D);
     const bool one_gate = p.gate && p.gate_share >= p.M, row_gate = p.gate && !one_gate;
-    RawRow<R, VEC, TPR> rx;
-    RawRow<T, VEC, TPR> rh;
-    RawGate<VEC, TPR> rg;
+    RawRow<R, SHAPE> rx;
+    RawRow<T, SHAPE> rh;
+    RawGate<SHAPE> rg;
     rx.clear(); rh.clear(); rg.clear();
     auto fetch = [&](long long row) __attribute__((always_inline)) {
         if (row < p.M) {
@@ -129,14 +120,14 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_kernel(const
     const long long step = (long long)gridDim.x * TEAMS;
     fetch((long long)blockIdx.x * TEAMS + team);
     float post_w[8], post_b[8], pre_w[8], pre_b[8], gate[8];
-    load_vector<VEC, TPR>(p.post_w, 1.0f, t, D, post_w);
-    load_vector<VEC, TPR>(p.post_b, 0.0f, t, D, post_b);
-    load_vector<VEC, TPR>(p.pre_w, 1.0f, t, D, pre_w);
-    load_vector<VEC, TPR>(p.pre_b, 0.0f, t, D, pre_b);
+    load_vector<SHAPE>(p.post_w, 1.0f, t, D, post_w);
+    load_vector<SHAPE>(p.post_b, 0.0f, t, D, post_b);
+    load_vector<SHAPE>(p.pre_w, 1.0f, t, D, pre_w);
+    load_vector<SHAPE>(p.pre_b, 0.0f, t, D, pre_b);
 #pragma unroll
     for (int e = 0; e < 8; ++e) gate[e] = 1.0f;
     if (one_gate) {
-        RawGate<VEC, TPR> g;
+        RawGate<SHAPE> g;
         g.load(p.gate, p.gate_bf16, 0, t, D);
         g.get(p.gate_bf16, gate);
     }
@@ -160,12 +151,18 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_kernel(const
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = fmaf(p.scale, v[e], gate[e] * u[e]);
         }
-        if (p.xn && live) store_row<R, VEC, TPR, 8>(static_cast<R*>(p.xn) + row * p.ldxn, t, D, v);
+        if constexpr (SHAPE == kMoved) {
+            if (p.crossing) {   // every wave has its part of the row (and of the next one)
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+            }
+        }
+        if (p.xn && live) store_row<R, SHAPE>(static_cast<R*>(p.xn) + row * p.ldxn, t, D, v);
         if (p.pre) {
             row_stats(v, p.pre, in, tid, p.inv_d, p.eps, sum, pre_mean, pre_inv);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = fmaf((v[e] - pre_mean) * pre_inv, pre_w[e], pre_b[e]);
-            if (live) store_row<T, VEC, TPR, 8>(static_cast<T*>(p.y) + row * p.ldy, t, D, v);
+            if (live) store_row<T, SHAPE>(static_cast<T*>(p.y) + row * p.ldy, t, D, v);
         }
         if (p.stats && t == 0 && live) *reinterpret_cast<f32x4*>(p.stats + row * 4) = f32x4{post_mean, post_inv, pre_mean, pre_inv};
     }
@@ -232,8 +229,8 @@ constexpr int kWideSums = 4 * 8 * 1024 * 4;   // bytes of LDS for the four vecto
 // its column sums in registers, so weights cost one partial row per workgroup and the gate one row per chunk.  The partial rows are
 // added in a fixed order by column_sum_kernel: no atomics, results do not change from run to run.
 // Bound by HBM up to 4096 columns: 32768 x 2048 bfloat16 blocks on a float32 stream 250 us (1.21 GB at 4.8 TB/s), 4096 x 1024 float32 24 us; by the
-// rows' latency where a row takes a whole CU (8192 x 8192: 223 us, 3.6 TB/s) or is read in single elements (65536 x 777: 204 us, 3.0 TB/s).
-template <typename T, typename R, bool VEC, int TPR>
+// rows' latency where a row takes a whole CU (8192 x 8192: 223 us, 3.6 TB/s).
+template <typename T, typename R, RowShape SHAPE, int TPR>
 __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(const ResNormGradParams q) {
     constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
     constexpr bool WIDE = TPR == 1024;
@@ -243,7 +240,7 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
     extern __shared__ __attribute__((aligned(16))) float wide[];     // kWideSums bytes where WIDE
     const ResNormParams& p = q.f;
     const int tid = threadIdx.x, t = TEAMS == 1 ? tid : tid % TPR, team = TEAMS == 1 ? 0 : tid / TPR, D = p.D;
-    const unsigned in = inside<VEC, TPR>(t, D);
+    const unsigned in = own_columns<SHAPE>(t, D);
     TeamSum<TPR, 2> sum(red);
     ColumnSums<WIDE> a_pre_w, a_pre_b, a_post_w, a_post_b;
     a_pre_w.init(wide, tid);
@@ -255,9 +252,9 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
     constexpr bool LEAN = TPR > 512;
     float post_w[8], post_b[8], pre_w[8];
     if constexpr (!LEAN) {
-        load_vector<VEC, TPR>(p.post_w, 1.0f, t, D, post_w);
-        load_vector<VEC, TPR>(p.post_b, 0.0f, t, D, post_b);
-        load_vector<VEC, TPR>(p.pre_w, 1.0f, t, D, pre_w);
+        load_vector<SHAPE>(p.post_w, 1.0f, t, D, post_w);
+        load_vector<SHAPE>(p.post_b, 0.0f, t, D, post_b);
+        load_vector<SHAPE>(p.pre_w, 1.0f, t, D, pre_w);
     }
     const bool row_gate = p.gate && p.gate_share == 1;
     const int teams = gridDim.x * TEAMS;
@@ -267,9 +264,9 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
         const int group = c / q.chunks_per_gate;
         const long long first = (long long)group * q.group_rows + (long long)(c % q.chunks_per_gate) * q.chunk_rows;
         const long long last = c < q.chunks ? min(first + q.chunk_rows, (long long)(group + 1) * q.group_rows) : first;
-        RawRow<R, VEC, TPR> rx, rd;
-        RawRow<T, VEC, TPR> rh, ry;
-        RawGate<VEC, TPR> rg;
+        RawRow<R, SHAPE> rx, rd;
+        RawRow<T, SHAPE> rh, ry;
+        RawGate<SHAPE> rg;
         f32x4 rs = {0.0f, 1.0f, 0.0f, 1.0f};
         rx.clear(); rd.clear(); rh.clear(); ry.clear(); rg.clear();
         long long gate_row = -1;
@@ -308,8 +305,8 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
             if constexpr (!LEAN) fetch(row + 1);   // under this row's arithmetic
             if (p.h) {
                 if constexpr (LEAN) {
-                    load_vector<VEC, TPR>(p.post_w, 1.0f, t, D, post_w);
-                    load_vector<VEC, TPR>(p.post_b, 0.0f, t, D, post_b);
+                    load_vector<SHAPE>(p.post_w, 1.0f, t, D, post_w);
+                    load_vector<SHAPE>(p.post_b, 0.0f, t, D, post_b);
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -322,7 +319,7 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
                 }
             }
             if (p.pre) {
-                if constexpr (LEAN) load_vector<VEC, TPR>(p.pre_w, 1.0f, t, D, pre_w);
+                if constexpr (LEAN) load_vector<SHAPE>(p.pre_w, 1.0f, t, D, pre_w);
                 s[0] = s[1] = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -346,7 +343,7 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
                 float o[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o[e] = p.scale * d[e];
-                store_row<R, VEC, TPR, 8>(static_cast<R*>(q.d_x) + row * q.ld_dx, t, D, o);
+                store_row<R, SHAPE>(static_cast<R*>(q.d_x) + row * q.ld_dx, t, D, o);
             }
             if (p.h) {
                 if (q.d_gate && live) {
@@ -354,8 +351,8 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
                         float o[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) o[e] = d[e] * u[e];
-                        if (p.gate_bf16) store_row<bf16_t, VEC, TPR, 8>(static_cast<bf16_t*>(q.d_gate) + row * q.ld_dg, t, D, o);
-                        else store_row<float, VEC, TPR, 8>(static_cast<float*>(q.d_gate) + row * q.ld_dg, t, D, o);
+                        if (p.gate_bf16) store_row<bf16_t, SHAPE>(static_cast<bf16_t*>(q.d_gate) + row * q.ld_dg, t, D, o);
+                        else store_row<float, SHAPE>(static_cast<float*>(q.d_gate) + row * q.ld_dg, t, D, o);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) a_gate[e] = fmaf(d[e], u[e], a_gate[e]);
@@ -364,7 +361,7 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[e] *= gate[e];
                 if (p.post) {
-                    if constexpr (LEAN) load_vector<VEC, TPR>(p.post_w, 1.0f, t, D, post_w);
+                    if constexpr (LEAN) load_vector<SHAPE>(p.post_w, 1.0f, t, D, post_w);
                     if (live) {
                         a_post_w.add_product(d, uhat);
                         a_post_b.add(d);
@@ -380,13 +377,13 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
 #pragma unroll
                     for (int e = 0; e < 8; ++e) d[e] = (d[e] - m0 - uhat[e] * m1) * st[1];
                 }
-                if (q.d_h && live) store_row<T, VEC, TPR, 8>(static_cast<T*>(q.d_h) + row * q.ld_dh, t, D, d);
+                if (q.d_h && live) store_row<T, SHAPE>(static_cast<T*>(q.d_h) + row * q.ld_dh, t, D, d);
             }
         }
         if (q.d_gate && !row_gate && c < q.chunks) {
-            if (q.chunks_per_gate > 1) store_row<float, VEC, TPR, 8>(q.gate_partial + (long long)c * D, t, D, a_gate);
-            else if (p.gate_bf16) store_row<bf16_t, VEC, TPR, 8>(static_cast<bf16_t*>(q.d_gate) + group * q.ld_dg, t, D, a_gate);
-            else store_row<float, VEC, TPR, 8>(static_cast<float*>(q.d_gate) + group * q.ld_dg, t, D, a_gate);
+            if (q.chunks_per_gate > 1) store_row<float, SHAPE>(q.gate_partial + (long long)c * D, t, D, a_gate);
+            else if (p.gate_bf16) store_row<bf16_t, SHAPE>(static_cast<bf16_t*>(q.d_gate) + group * q.ld_dg, t, D, a_gate);
+            else store_row<float, SHAPE>(static_cast<float*>(q.d_gate) + group * q.ld_dg, t, D, a_gate);
         }
     }
     float* out = q.partial + (long long)blockIdx.x * q.vectors * D;
@@ -414,7 +411,7 @@ __global__ __launch_bounds__(threads_for<TPR>()) void residual_norm_grad_kernel(
                     for (int k = WAVES; k < THREADS / 64; k += WAVES) a[e] += joined[((row + k) * 8 + e) * TPW + col];
             }
         }
-        if (team == 0) store_row<float, VEC, TPR, 8>(out + (long long)slot * D, t, D, a);
+        if (team == 0) store_row<float, SHAPE>(out + (long long)slot * D, t, D, a);
     };
     flush(a_pre_w, q.slot_pre_w);
     flush(a_pre_b, q.slot_pre_b);
@@ -512,39 +509,28 @@ ResNormParams forward_params(const adcdiff_residual_norm_args& a) {
     p.M = a.M; p.D = a.D; p.post = a.h ? a.post_norm : 0; p.pre = a.pre_norm;
     p.gate_bf16 = a.gate_dtype == ADCDIFF_BF16;
     p.gate_share = a.gate && a.M > 0 ? a.M / a.gate_rows : 1;
+    p.crossing = a.x_new == a.x && wave_crossing(a.D);
     p.scale = a.residual_scale; p.eps = a.eps; p.inv_d = 1.0f / (float)a.D;
     return p;
 }
 
-bool vector_inputs(const adcdiff_residual_norm_args& a) {
-    const int st = type_size(a.dtype), sr = type_size(a.stream_dtype), sg = type_size(a.gate_dtype);
-    return a.D % 8 == 0 && vector_rows(a.h, a.ldh, st) && vector_rows(a.x, a.ldx, sr) && vector_rows(a.gate, a.ldg, sg) &&
-           vector_rows(a.post_weight, 0, 4) && vector_rows(a.post_bias, 0, 4) && vector_rows(a.pre_weight, 0, 4) && vector_rows(a.pre_bias, 0, 4);
-}
-
 // Threads for a row of D columns, eight each: a power of two, and more sizes where both sides were measured (67 M elements, bfloat16; f / b: forward,
-// backward).  768 instead of 1024: D = 6000 f 148 -> 131 us, b 970 -> 230 us, single elements D = 5001 f 219 -> 209, b 534 -> 335.  Rows read in
-// vectors: 32 instead of 64 at D = 136, f 36.8 -> 21.6, b 75 -> 52; and in the backward pass 192, 320 and 384, where fewer idle threads hold
-// registers (D = 2056: b 298 -> 266 us, D = 1032: 288 -> 283, in float32 335 -> 319), while the forward pass loses with them (D = 2056: 166 -> 176 us,
-// D = 3000: 124 -> 139 us).
-int team_width(int D, bool vec, bool backward) {
+// backward).  768 instead of 1024 at D = 6000, f 148 -> 131 us, b 970 -> 230 us; 32 instead of 64 at D = 136, f 36.8 -> 21.6, b 75 -> 52; and in the
+// backward pass 192, 320 and 384, where fewer idle threads hold registers (D = 2056: b 298 -> 266 us, D = 1032: 288 -> 283, in float32 335 -> 319), while
+// the forward pass loses with them (D = 2056: 166 -> 176 us, D = 3000: 124 -> 139 us).
+int team_width(int D, bool backward) {
     const int waves = (D + 511) / 512;
-    if (vec && D <= 128) return 16;
-    if (vec && D <= 256) return 32;
-    if (vec && backward && waves <= 6) return 64 * waves;
+    if (D <= 128) return 16;
+    if (D <= 256) return 32;
+    if (backward && waves <= 6) return 64 * waves;
     return waves <= 1 ? 64 : waves <= 2 ? 128 : waves <= 4 ? 256 : waves <= 8 ? 512 : waves <= 12 ? 768 : 1024;
 }
 
 // Calls f(std::integral_constant<int, threads>) for the team of a row
-template <bool VEC, bool BACKWARD, typename F>
+template <RowShape SHAPE, bool BACKWARD, typename F>
 void for_width(int tpr, F f) {
-    if constexpr (VEC) {
-        switch (tpr) {
-            case 16: return f(std::integral_constant<int, 16>());
-            case 32: return f(std::integral_constant<int, 32>());
-        }
-    }
-    if constexpr (VEC && BACKWARD) {
+    if constexpr (SHAPE == kTiny) return f(std::integral_constant<int, 16>());
+    if constexpr (BACKWARD) {
         switch (tpr) {
             case 192: return f(std::integral_constant<int, 192>());
             case 320: return f(std::integral_constant<int, 320>());
@@ -552,6 +538,8 @@ void for_width(int tpr, F f) {
         }
     }
     switch (tpr) {
+        case 16: return f(std::integral_constant<int, 16>());
+        case 32: return f(std::integral_constant<int, 32>());
         case 64: return f(std::integral_constant<int, 64>());
         case 128: return f(std::integral_constant<int, 128>());
         case 256: return f(std::integral_constant<int, 256>());
@@ -561,26 +549,34 @@ void for_width(int tpr, F f) {
     }
 }
 
-template <typename T, typename R, bool VEC, int TPR>
+template <typename T, typename R, RowShape SHAPE, int TPR>
 void launch_forward(const ResNormParams& p, hipStream_t stream) {
     constexpr int threads = threads_for<TPR>(), teams = threads / TPR;
     const long long groups = ((long long)p.M + teams - 1) / teams;
-    hipLaunchKernelGGL((residual_norm_kernel<T, R, VEC, TPR>), dim3((unsigned)std::min<long long>(groups, 2048)), dim3(threads), 0, stream, p);
+    hipLaunchKernelGGL((residual_norm_kernel<T, R, SHAPE, TPR>), dim3((unsigned)std::min<long long>(groups, 2048)), dim3(threads), 0, stream, p);
 }
 
-template <typename T, typename R, bool VEC>
+template <typename T, typename R, RowShape SHAPE>
 void forward_by_width(const ResNormParams& p, hipStream_t stream) {
-    for_width<VEC, false>(team_width(p.D, VEC, false), [&](auto tpr) { launch_forward<T, R, VEC, decltype(tpr)::value>(p, stream); });
+    for_width<SHAPE, false>(team_width(p.D, false), [&](auto tpr) { launch_forward<T, R, SHAPE, decltype(tpr)::value>(p, stream); });
 }
 
-template <bool VEC>
+template <typename T, typename R>
+void forward_by_shape(const ResNormParams& p, hipStream_t stream) {
+    switch (row_shape(p.D)) {
+        case kWhole: return forward_by_width<T, R, kWhole>(p, stream);
+        case kMoved: return forward_by_width<T, R, kMoved>(p, stream);
+        case kTiny: return forward_by_width<T, R, kTiny>(p, stream);
+    }
+}
+
 void forward_by_type(const ResNormParams& p, int dtype, int stream_dtype, hipStream_t stream) {
     if (dtype == ADCDIFF_BF16) {
-        if (stream_dtype == ADCDIFF_BF16) forward_by_width<bf16_t, bf16_t, VEC>(p, stream);
-        else forward_by_width<bf16_t, float, VEC>(p, stream);
+        if (stream_dtype == ADCDIFF_BF16) forward_by_shape<bf16_t, bf16_t>(p, stream);
+        else forward_by_shape<bf16_t, float>(p, stream);
     } else {
-        if (stream_dtype == ADCDIFF_BF16) forward_by_width<float, bf16_t, VEC>(p, stream);
-        else forward_by_width<float, float, VEC>(p, stream);
+        if (stream_dtype == ADCDIFF_BF16) forward_by_shape<float, bf16_t>(p, stream);
+        else forward_by_shape<float, float>(p, stream);
     }
 }
 
@@ -592,9 +588,9 @@ struct Cut {
 
 constexpr int kMaxGroups = 512;
 
-Cut cut_rows(int M, int D, bool vec, int gate_rows, bool gate_grad, int vectors) {
+Cut cut_rows(int M, int D, int gate_rows, bool gate_grad, int vectors) {
     Cut c{};
-    c.tpr = team_width(D, vec, true);
+    c.tpr = team_width(D, true);
     c.teams = c.tpr >= kThreads ? 1 : kThreads / c.tpr;
     c.vectors = vectors;
     c.gate_sum = gate_grad && gate_rows > 0 && M / std::max(gate_rows, 1) != 1;
@@ -619,12 +615,12 @@ size_t workspace_floats(const Cut& c, int D) {
     return n;
 }
 
-template <typename T, typename R, bool VEC>
+template <typename T, typename R, RowShape SHAPE>
 int backward_by_width(const ResNormGradParams& q, const Cut& c, hipStream_t stream) {
     int rc = ADCDIFF_OK;
-    for_width<VEC, true>(c.tpr, [&](auto tpr) {
+    for_width<SHAPE, true>(c.tpr, [&](auto tpr) {
         constexpr int TPR = decltype(tpr)::value;
-        const auto kernel = &residual_norm_grad_kernel<T, R, VEC, TPR>;
+        const auto kernel = &residual_norm_grad_kernel<T, R, SHAPE, TPR>;
         constexpr int lds = TPR == 1024 ? kWideSums : 0;
         if constexpr (lds > 0) {
             static std::atomic<bool> done[64];
@@ -636,21 +632,23 @@ int backward_by_width(const ResNormGradParams& q, const Cut& c, hipStream_t stre
     return rc;
 }
 
-template <bool VEC>
-int backward_by_type(const ResNormGradParams& q, const Cut& c, int dtype, int stream_dtype, hipStream_t stream) {
-    if (dtype == ADCDIFF_BF16) {
-        if (stream_dtype == ADCDIFF_BF16) return backward_by_width<bf16_t, bf16_t, VEC>(q, c, stream);
-        return backward_by_width<bf16_t, float, VEC>(q, c, stream);
-    } else {
-        if (stream_dtype == ADCDIFF_BF16) return backward_by_width<float, bf16_t, VEC>(q, c, stream);
-        return backward_by_width<float, float, VEC>(q, c, stream);
+template <typename T, typename R>
+int backward_by_shape(const ResNormGradParams& q, const Cut& c, hipStream_t stream) {
+    switch (row_shape(q.f.D)) {
+        case kWhole: return backward_by_width<T, R, kWhole>(q, c, stream);
+        case kMoved: return backward_by_width<T, R, kMoved>(q, c, stream);
+        default: return backward_by_width<T, R, kTiny>(q, c, stream);
     }
 }
 
-bool vector_backward(const adcdiff_residual_norm_args& a, const adcdiff_residual_norm_grads& g) {
-    const int st = type_size(a.dtype), sr = type_size(a.stream_dtype), sg = type_size(a.gate_dtype);
-    return vector_inputs(a) && vector_rows(g.d_x_new, g.ld_d_x_new, sr) && vector_rows(g.d_y, g.ld_d_y, st) && vector_rows(g.h, g.ld_h, st) &&
-           vector_rows(g.x, g.ld_x, sr) && vector_rows(g.gate, a.gate_rows > 1 ? g.ld_gate : 0, sg);
+int backward_by_type(const ResNormGradParams& q, const Cut& c, int dtype, int stream_dtype, hipStream_t stream) {
+    if (dtype == ADCDIFF_BF16) {
+        if (stream_dtype == ADCDIFF_BF16) return backward_by_shape<bf16_t, bf16_t>(q, c, stream);
+        return backward_by_shape<bf16_t, float>(q, c, stream);
+    } else {
+        if (stream_dtype == ADCDIFF_BF16) return backward_by_shape<float, bf16_t>(q, c, stream);
+        return backward_by_shape<float, float>(q, c, stream);
+    }
 }
 
 int vector_count(const adcdiff_residual_norm_grads& g) { return !!g.post_weight + !!g.post_bias + !!g.pre_weight + !!g.pre_bias; }
@@ -671,15 +669,14 @@ extern "C" int adcdiff_residual_norm(const adcdiff_residual_norm_args* a, adcdif
     const ResNormParams p = forward_params(*a);
     const int st = type_size(a->dtype), sr = type_size(a->stream_dtype);
     TimingScope timing(ADCDIFF_KIND_OTHER, a->M, a->D, 0, 0.0, (double)a->M * a->D * ((a->h ? st : 0) + (a->y ? st : 0) + sr + (a->x_new ? sr : 0)), stream);
-    if (vector_inputs(*a) && vector_rows(a->x_new, a->ldx_new, sr) && vector_rows(a->y, a->ldy, st)) forward_by_type<true>(p, a->dtype, a->stream_dtype, stream);
-    else forward_by_type<false>(p, a->dtype, a->stream_dtype, stream);
+    forward_by_type(p, a->dtype, a->stream_dtype, stream);
     return check_launch("residual_norm");
 }
 
 extern "C" size_t adcdiff_residual_norm_backward_workspace_bytes(const adcdiff_residual_norm_args* a, const adcdiff_residual_norm_grads* g) {
     using namespace adcdiff;
     if (check_args("residual_norm_backward", a) != ADCDIFF_OK || !g) return 0;
-    return std::max<size_t>(16, workspace_floats(cut_rows(a->M, a->D, vector_backward(*a, *g), a->gate ? a->gate_rows : 0, g->gate != nullptr, vector_count(*g)), a->D) * 4);
+    return std::max<size_t>(16, workspace_floats(cut_rows(a->M, a->D, a->gate ? a->gate_rows : 0, g->gate != nullptr, vector_count(*g)), a->D) * 4);
 }
 
 extern "C" int adcdiff_residual_norm_backward(const adcdiff_residual_norm_args* a, const adcdiff_residual_norm_grads* g, void* workspace,
@@ -698,7 +695,7 @@ extern "C" int adcdiff_residual_norm_backward(const adcdiff_residual_norm_args* 
     if ((g->d_x_new && g->ld_d_x_new < a->D) || (g->d_y && g->ld_d_y < a->D) || (g->h && g->ld_h < a->D) || (g->x && g->ld_x < a->D) ||
         (g->gate && a->gate_rows > 1 && g->ld_gate < a->D))
         return fail(ADCDIFF_E_BADARG, "residual_norm_backward: a row pitch below %d columns", a->D);
-    const Cut c = cut_rows(a->M, a->D, vector_backward(*a, *g), a->gate ? a->gate_rows : 0, g->gate != nullptr, vector_count(*g));
+    const Cut c = cut_rows(a->M, a->D, a->gate ? a->gate_rows : 0, g->gate != nullptr, vector_count(*g));
     const size_t need = std::max<size_t>(16, workspace_floats(c, a->D) * 4);
     if (!workspace || !aligned16(workspace) || workspace_bytes < need)
         return fail(ADCDIFF_E_WORKSPACE, "residual_norm_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
@@ -718,7 +715,7 @@ extern "C" int adcdiff_residual_norm_backward(const adcdiff_residual_norm_args* 
     q.slot_pre_w = place(g->pre_weight); q.slot_pre_b = place(g->pre_bias); q.slot_post_w = place(g->post_weight); q.slot_post_b = place(g->post_bias);
     if (a->M > 0) {
         TimingScope timing(ADCDIFF_KIND_OTHER, a->M, a->D, 0, 0.0, (double)a->M * a->D * ((a->h ? 2.0 : 0.0) * st + (g->d_y ? st : 0) + 2.0 * sr + (g->d_x_new ? sr : 0)), stream);
-        rc = vector_backward(*a, *g) ? backward_by_type<true>(q, c, a->dtype, a->stream_dtype, stream) : backward_by_type<false>(q, c, a->dtype, a->stream_dtype, stream);
+        rc = backward_by_type(q, c, a->dtype, a->stream_dtype, stream);
         if (rc != ADCDIFF_OK) return rc;
         rc = check_launch("residual_norm_backward");
         if (rc != ADCDIFF_OK) return rc;

@@ -18,98 +18,84 @@ __device__ __forceinline__ float bf_hi(uint32_t w) { return __builtin_bit_cast(f
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Columns of element e of thread t: vectors of 8 consecutive columns where VEC, else single columns TPR apart.
-template <bool VEC, int TPR>
-__device__ __forceinline__ int column(int t, int e) { return VEC ? ((e >> 3) * TPR + t) * 8 + (e & 7) : e * TPR + t; }
+// Thread t of a team owns the eight columns from 8 t on.  Rows start at any element: the memory system takes 16-byte accesses at any address.
+//   kWhole: D is a multiple of 8
+//   kMoved: it is not, and the last thread with columns moves its eight back to the row's last ones.  It loads and stores what its neighbour does,
+//           with the same bits, and own_columns leaves them to the neighbour in sums.  (65536 x 777 bfloat16: forward 98 us, backward 169; all in single elements 129 and 206;
+//           vectors with a single-element tail 115 and 237: the tail's branch makes the loads of a row ahead wait.)  Where a row is overwritten in place, neighbours in two waves have to
+//           have loaded it before either stores (wave_crossing).
+//   kTiny:  D < 8, the first thread has the row in single elements
+enum RowShape { kWhole, kMoved, kTiny };
+inline RowShape row_shape(int D) { return D % 8 == 0 ? kWhole : D > 8 ? kMoved : kTiny; }
+inline bool wave_crossing(int D) { return D > 512 && D % 512 > 0 && D % 512 < 8; }   // the last thread is a wave's first
 
-// E elements of the row at p; columns >= D read as 0.
-template <typename T, bool VEC, int TPR, int E>
-__device__ __forceinline__ void load_row(const T* __restrict__ p, int t, int D, float (&v)[E]) {
-    if constexpr (VEC) {
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef bf16x8 bf16x8_any __attribute__((aligned(2)));
+
+// first of the eight columns of thread t (8 t < D)
+template <RowShape SHAPE>
+__device__ __forceinline__ int first_column(int t, int D) { return SHAPE == kMoved ? min(t * 8, D - 8) : t * 8; }
+
+// bit e: element e is this thread's in a sum over the row
+template <RowShape SHAPE>
+__device__ __forceinline__ unsigned own_columns(int t, int D) {
+    const int rest = D - t * 8;
+    if (rest <= 0) return 0u;
+    if (SHAPE == kWhole || rest >= 8) return 0xffu;
+    return SHAPE == kMoved ? 0xffu >> (8 - rest) << (8 - rest) : 0xffu >> (8 - rest);
+}
+
+// the eight elements of thread t of the row at p
+template <typename T, RowShape SHAPE>
+__device__ __forceinline__ void store_row(T* __restrict__ p, int t, int D, const float (&v)[8]) {
+    if (t * 8 >= D) return;
+    if constexpr (SHAPE == kTiny) {
 #pragma unroll
-        for (int j = 0; j < E / 8; ++j) {
-            const int c = (j * TPR + t) * 8;
-            if (c < D) {
-                if constexpr (sizeof(T) == 2) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(p + c);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { v[j * 8 + 2 * i] = bf_lo(w[i]); v[j * 8 + 2 * i + 1] = bf_hi(w[i]); }
-                } else {
-                    const f32x4 a = *reinterpret_cast<const f32x4*>(p + c), b = *reinterpret_cast<const f32x4*>(p + c + 4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { v[j * 8 + i] = a[i]; v[j * 8 + 4 + i] = b[i]; }
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[j * 8 + i] = 0.0f;
-            }
-        }
+        for (int e = 0; e < 7; ++e)
+            if (e < D) p[e] = (T)v[e];
     } else {
+        T* const q = p + first_column<SHAPE>(t, D);
+        if constexpr (sizeof(T) == 2) {
+            bf16x8 o;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int c = e * TPR + t;
-            v[e] = c < D ? to_f(p[c]) : 0.0f;
+            for (int i = 0; i < 8; ++i) o[i] = (bf16_t)v[i];
+            *reinterpret_cast<bf16x8_any*>(q) = o;
+        } else {
+            *reinterpret_cast<f32x4_any*>(q) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4_any*>(q + 4) = f32x4{v[4], v[5], v[6], v[7]};
         }
     }
 }
 
-template <typename T, bool VEC, int TPR, int E>
-__device__ __forceinline__ void store_row(T* __restrict__ p, int t, int D, const float (&v)[E]) {
-    if constexpr (VEC) {
-#pragma unroll
-        for (int j = 0; j < E / 8; ++j) {
-            const int c = (j * TPR + t) * 8;
-            if (c < D) {
-                if constexpr (sizeof(T) == 2) {
-                    bf16x8 o;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = (bf16_t)v[j * 8 + i];
-                    *reinterpret_cast<bf16x8*>(p + c) = o;
-                } else {
-                    f32x4 a, b;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { a[i] = v[j * 8 + i]; b[i] = v[j * 8 + 4 + i]; }
-                    *reinterpret_cast<f32x4*>(p + c) = a;
-                    *reinterpret_cast<f32x4*>(p + c + 4) = b;
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int c = e * TPR + t;
-            if (c < D) p[c] = (T)v[e];
-        }
-    }
-}
-
-// Eight elements of a row as they stand in memory: loaded without being looked at, so that the loads of a row ahead stay in flight under the
-// arithmetic of the row in hand.  Columns as in load_row with E = 8; those >= D read as 0.
-template <typename T, bool VEC, int TPR>
+// The eight elements of thread t as they stand in memory: loaded without being looked at, so that the loads of a row ahead stay in flight under
+// the arithmetic of the row in hand.  Elements without a column read as 0.
+template <typename T, RowShape SHAPE>
 struct RawRow {
-    static constexpr int N = VEC && sizeof(T) == 2 ? 4 : 8;
+    static constexpr int N = sizeof(T) == 2 ? 4 : 8;
     uint32_t r[N];
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < N; ++i) r[i] = 0;
     }
     __device__ __forceinline__ void load(const T* __restrict__ p, int t, int D) {
-        if constexpr (VEC) {
-            clear();
-            if (t * 8 < D) {
+        clear();
+        if (t * 8 >= D) return;
+        if constexpr (SHAPE == kTiny) {
 #pragma unroll
-                for (int i = 0; i < N / 4; ++i) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(p + t * 8 + 4 * i);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) r[4 * i + k] = w[k];
+            for (int e = 0; e < 7; ++e) {
+                if (e < D) {
+                    if constexpr (sizeof(T) == 2) r[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
+                    else r[e] = reinterpret_cast<const uint32_t*>(p)[e];
                 }
             }
         } else {
+            const T* const q = p + first_column<SHAPE>(t, D);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = e * TPR + t;
-                if constexpr (sizeof(T) == 2) r[e] = c < D ? reinterpret_cast<const uint16_t*>(p)[c] : 0;
-                else r[e] = c < D ? reinterpret_cast<const uint32_t*>(p)[c] : 0;
+            for (int i = 0; i < N / 4; ++i) {
+                const u32x4 w = *reinterpret_cast<const u32x4_any*>(q + 4 * i);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) r[4 * i + k] = w[k];
             }
         }
     }
@@ -117,12 +103,9 @@ struct RawRow {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = __builtin_bit_cast(float, r[e]);
-        } else if constexpr (VEC) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { v[2 * i] = bf_lo(r[i]); v[2 * i + 1] = bf_hi(r[i]); }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = bf_lo(r[e]);
+            for (int i = 0; i < 4; ++i) { v[2 * i] = bf_lo(r[i]); v[2 * i + 1] = bf_hi(r[i]); }
         }
     }
 };

@@ -356,7 +356,7 @@ int adcdiff_clip_adamw_step_noalloc(const adcdiff_opt_tensor* tensors, int n_ten
  *                  repeats one row
  *   weights, biases [D] float32, each optional
  *   stats          [M, 4] float32 on a 16-byte boundary, or NULL: the row statistics that the backward pass reads
- * D <= 8192, any D and any pitch; rows on 16-byte boundaries with D % 8 == 0 take the vector path. */
+ * D <= 8192, any D, any pitch, pointers on their element's boundary. */
 enum { ADCDIFF_NORM_NONE = 0, ADCDIFF_NORM_RMS = 1, ADCDIFF_NORM_LAYER = 2 };
 typedef struct adcdiff_residual_norm_args {
     int M, D;

@@ -69,6 +69,13 @@ def test_widths_and_types(D, T, R):
         _check(_inputs(9, D, T, R, T, gates, post, pre), post, pre, 0.75, eps=1e-3)
 
 
+@pytest.mark.parametrize("D", [3, 9, 15, 63, 127, 129, 255, 257, 511, 513, 517, 519, 521, 1025, 1535, 1537, 2051, 2561, 4095, 4097, 4103, 6143, 6145, 8191])
+@pytest.mark.parametrize("T, R", [(BF, BF), (F, F)])
+def test_last_columns(D, T, R):
+    """rows whose last thread has fewer than eight columns of its own, behind a wave's end among them"""
+    _check(_inputs(37, D, T, R, T, 37, "layer", "rms", pitch=1), "layer", "rms", 0.5)
+
+
 @pytest.mark.parametrize("post, pre", list(itertools.product((None, "rms", "layer"), repeat=2)))
 @pytest.mark.parametrize("gates", [0, 1, 6, 12])
 def test_every_combination_of_parts(post, pre, gates):
@@ -211,7 +218,7 @@ def test_offsets_past_32_bits():
     assert torch.equal(p[0], q[0]) and torch.equal(p[1], q[1])
 
 
-@pytest.mark.parametrize("D", [96, 777, 2048, 8192])
+@pytest.mark.parametrize("D", [5, 96, 513, 777, 1029, 2048, 4097, 8191, 8192])
 def test_stream_in_place(D):
     """x_new over x and y over h (C ABI), with rows enough for every workgroup to take several"""
     import ctypes as C
