@@ -219,7 +219,6 @@ struct I8Params {
     void* out;
     long long lda, ldw, ldr, ldo;
     int M, N, K, act;
-    bool vec;
 };
 
 // v * sigmoid(v) on the hardware's exp2 and reciprocal (each within one unit in the last place): the argument's rounding adds |v| * 2^-24 relative,
@@ -244,12 +243,12 @@ __device__ __forceinline__ i32x4 load_chunk(const int8_t* __restrict__ row, int 
     return v;
 }
 
-// Eight consecutive outputs of row m from column n on (fewer at the right edge): their scales, biases and residual (which the few-row kernel loads before
-// the sums are there), and the outputs
+// Eight consecutive outputs of row m from column n on (single elements where the row ends before): their scales, biases and residual (which the
+// few-row kernel loads before the sums are there), and the outputs.  Rows may start at any element.
 template <typename Out>
 struct Finish8 {
     typedef Out Eight __attribute__((ext_vector_type(8)));
-    typedef Eight EightAt16 __attribute__((aligned(16)));
+    typedef Eight EightAny __attribute__((aligned(sizeof(Out))));
     f32x4 w0, w1, b0, b1;
     float sa;
     Eight r;
@@ -257,7 +256,7 @@ struct Finish8 {
         const Out* res = static_cast<const Out*>(p.residual) + (long long)m * p.ldr + n;
         sa = p.a_scale[m];
         b0 = b1 = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (p.vec) {   // N is a multiple of 8 and rows of out and residual lie on 16-byte boundaries
+        if (n + 8 <= p.N) {
             const f32x4_any* pw = reinterpret_cast<const f32x4_any*>(p.w_scale + n);
             w0 = pw[0];
             w1 = pw[1];
@@ -266,7 +265,7 @@ struct Finish8 {
                 b0 = pb[0];
                 b1 = pb[1];
             }
-            if (p.residual) r = *reinterpret_cast<const EightAt16*>(res);
+            if (p.residual) r = *reinterpret_cast<const EightAny*>(res);
         } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -292,8 +291,8 @@ struct Finish8 {
             if (p.act) v = silu_fast(v);
             o[c] = (Out)v;
         }
-        if (p.vec) {
-            *reinterpret_cast<EightAt16*>(out) = o;
+        if (n + 8 <= p.N) {
+            *reinterpret_cast<EightAny*>(out) = o;
         } else {
 #pragma unroll
             for (int c = 0; c < 8; ++c)
@@ -501,11 +500,10 @@ __global__ __launch_bounds__(64 * WAVES) void gemm_i8_split_kernel(const I8Param
 // against the epilogue's stores.
 #include "w4_mainloop_i8.inc"
 
-// SIDE: bit 0 residual, bit 1 SiLU, known at compile time so that loads and stores are counted exactly and no wait covers the stores; -1: asked
-// for at run time, together with single-element accesses (outputs whose rows are not on 16-byte boundaries).
-template <typename Out, int SIDE>
+// SIDE: bit 0 residual, bit 1 SiLU, known at compile time so that loads and stores are counted exactly and no wait covers the stores.
+// WHOLE: N is a multiple of 8; else eight outputs at the edge of a tile that moved back may belong to two tiles and are stored one by one.
+template <typename Out, int SIDE, bool WHOLE>
 __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(const I8Params p) {
-    constexpr bool VEC = SIDE >= 0;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -588,8 +586,8 @@ __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(const I8Params p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) sa[i] = p.a_scale[mw + 16 * i + frow];
     typedef Out Side __attribute__((ext_vector_type(8)));
-    typedef Side SideAny __attribute__((aligned(VEC ? 16 : sizeof(Out))));
-    const bool residual = SIDE >= 0 ? (SIDE & 1) != 0 : p.residual != nullptr, act = SIDE >= 0 ? (SIDE & 2) != 0 : p.act != 0;
+    typedef Side SideAny __attribute__((aligned(sizeof(Out))));   // rows start at any element
+    constexpr bool residual = (SIDE & 1) != 0, act = (SIDE & 2) != 0;
     const Out* const res = static_cast<const Out*>(p.residual) + (long long)(mw + frow) * p.ldr + nl;
     Side side[2][4];
     auto fetch = [&](int i) __attribute__((always_inline)) {
@@ -628,7 +626,7 @@ __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(const I8Params p) {
             if (m >= m_lo) {
                 if (n >= n_lo) {
                     *reinterpret_cast<SideAny*>(out) = o;
-                } else if constexpr (!VEC) {
+                } else if constexpr (!WHOLE) {
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
                         if (n + c >= n_lo) out[c] = o[c];
@@ -638,23 +636,27 @@ __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(const I8Params p) {
     }
 }
 
-template <typename Out, int SIDE>
+template <typename Out, int SIDE, bool WHOLE>
 int launch_w4(const I8Params& p, hipStream_t stream) {
     constexpr int smem = 2 * 65536;
     static std::atomic<bool> done[64];
-    const int rc = allow_lds("gemm_i8", reinterpret_cast<const void*>(&gemm_i8_w4_kernel<Out, SIDE>), smem, done);
+    const int rc = allow_lds("gemm_i8", reinterpret_cast<const void*>(&gemm_i8_w4_kernel<Out, SIDE, WHOLE>), smem, done);
     if (rc != ADCDIFF_OK) return rc;
     const long long tiles = (((long long)p.M + 255) / 256) * (((long long)p.N + 255) / 256);
     if (tiles > 0xffffff) return fail(ADCDIFF_E_BADARG, "gemm_i8: %d x %d outputs are too many for one call", p.M, p.N);
-    hipLaunchKernelGGL((gemm_i8_w4_kernel<Out, SIDE>), dim3((unsigned)tiles), dim3(256), smem, stream, p);
+    hipLaunchKernelGGL((gemm_i8_w4_kernel<Out, SIDE, WHOLE>), dim3((unsigned)tiles), dim3(256), smem, stream, p);
     return check_launch("gemm_i8");
+}
+
+template <typename Out, int SIDE>
+int launch_w4_shape(const I8Params& p, hipStream_t stream) {
+    return p.N % 8 == 0 ? launch_w4<Out, SIDE, true>(p, stream) : launch_w4<Out, SIDE, false>(p, stream);
 }
 
 template <typename Out>
 int launch_w4_side(const I8Params& p, hipStream_t stream) {
-    if (!p.vec) return launch_w4<Out, -1>(p, stream);
-    if (p.act) return p.residual ? launch_w4<Out, 3>(p, stream) : launch_w4<Out, 2>(p, stream);
-    return p.residual ? launch_w4<Out, 1>(p, stream) : launch_w4<Out, 0>(p, stream);
+    if (p.act) return p.residual ? launch_w4_shape<Out, 3>(p, stream) : launch_w4_shape<Out, 2>(p, stream);
+    return p.residual ? launch_w4_shape<Out, 1>(p, stream) : launch_w4_shape<Out, 0>(p, stream);
 }
 
 template <typename Out, int BM, int BN, int WAVES, int DEPTH>
@@ -774,9 +776,8 @@ extern "C" int adcdiff_gemm_i8(const adcdiff_gemm_i8_args* a, adcdiff_stream_t s
     const int rc = check_gemm(a);
     if (rc != ADCDIFF_OK || a->M == 0) return rc;
     hipStream_t stream = as_stream(stream_);
-    I8Params p{a->a, a->w, a->a_scale, a->w_scale, a->bias, a->residual, a->out, a->lda, a->ldw, a->ldr, a->ldo, a->M, a->N, a->K, a->act, false};
+    I8Params p{a->a, a->w, a->a_scale, a->w_scale, a->bias, a->residual, a->out, a->lda, a->ldw, a->ldr, a->ldo, a->M, a->N, a->K, a->act};
     const int so = type_size(a->out_dtype);
-    p.vec = a->N % 8 == 0 && vector_rows(a->out, a->ldo, so) && vector_rows(a->residual, a->ldr, so);
     TimingScope timing(ADCDIFF_KIND_OTHER, a->M, a->N, a->K, 2.0 * a->M * a->N * a->K,
                        (double)a->M * a->K + (double)a->N * a->K + (double)a->M * a->N * so * (a->residual ? 2 : 1), stream);
     return a->out_dtype == ADCDIFF_BF16 ? launch_gemm<bf16_t>(p, stream) : launch_gemm<float>(p, stream);

@@ -145,9 +145,6 @@ struct TeamSum {
 inline bool type_ok(int dtype) { return dtype == ADCDIFF_F32 || dtype == ADCDIFF_BF16; }
 inline int type_size(int dtype) { return dtype == ADCDIFF_BF16 ? 2 : 4; }
 
-// rows on 16-byte boundaries (vector accesses), or absent
-inline bool vector_rows(const void* p, long long ld, int size) { return !p || (aligned16(p) && (ld * size & 15) == 0); }
-
 // Lets a kernel use `bytes` of dynamic LDS on the current device; done[device] remembers that it was said
 inline int allow_lds(const char* who, const void* kernel, int bytes, std::atomic<bool> (&done)[64]) {
     int dev = 0;
