@@ -358,9 +358,9 @@ def _norm_type(norm_type):
 
 def _as_list(tensors):
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    for t in tensors:
-        if not torch.is_tensor(t):
-            raise TypeError("gradients must be tensors, got %s" % type(t).__name__)
+    for kind in set(map(type, tensors)):     # a look at each type, not at each of hundreds of tensors
+        if not issubclass(kind, torch.Tensor):
+            raise TypeError("gradients must be tensors, got %s" % kind.__name__)
     return tensors
 
 
