@@ -98,6 +98,22 @@ def test_codes_of_strided_rows():
     assert ops.quantize_rows(held[:0])[0].shape == (0, 700)
 
 
+@pytest.mark.parametrize("dtype", [F, BF])
+@pytest.mark.parametrize("K, ldq", [(5, 5), (5, 8), (7, 16), (9, 9), (21, 23), (21, 24), (100, 101), (129, 144), (515, 515), (2047, 2048), (4097, 4099), (8195, 8197)])
+def test_code_rows_of_any_pitch(K, ldq, dtype):
+    """codes at any pitch (C ABI) from rows at odd addresses; zeros up to the next multiple of 16 inside the pitch, the rest untouched"""
+    from adcdiff import _lib
+    M = 11
+    x = torch.randn(M * (K + 3) + 1, device="cuda").to(dtype)[1:].view(M, K + 3)[:, :K]
+    want, scale = ops.quantize_rows(x)
+    q, got = torch.full((M * ldq + 40,), 99, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    _lib.check(_lib.load().adcdiff_quantize_rows(x.data_ptr(), K + 3, int(dtype == BF), M, K, q.data_ptr(), ldq, got.data_ptr(),
+                                                 torch.cuda.current_stream().cuda_stream))
+    rows, end = q[:M * ldq].view(M, ldq), min(ldq, (K + 15) // 16 * 16)
+    assert torch.equal(rows[:, :K], want) and torch.equal(got, scale)
+    assert not rows[:, K:end].any() and bool((rows[:, end:] == 99).all()) and bool((q[M * ldq:] == 99).all())
+
+
 def test_codes_past_32_bits():
     pitch = (1 << 30) + 16
     held = torch.empty(2 * pitch + 512, device="cuda", dtype=BF)
@@ -174,6 +190,27 @@ def test_residual_in_place():
         p.a, p.w, p.a_scale, p.w_scale, p.residual, p.out = (t.data_ptr() for t in (a, w, sa, sw, res, res))
         _lib.check(_lib.load().adcdiff_gemm_i8(C.byref(p), torch.cuda.current_stream().cuda_stream))
         assert torch.equal(res, want)
+
+
+@pytest.mark.parametrize("out", ["fp32", "bf16"])
+@pytest.mark.parametrize("M, N, K, act", [(8200, 2051, 300, 0), (8200, 2051, 300, 1), (3000, 1003, 200, 1), (90, 77, 600, 0), (20, 301, 700, 1), (3, 5, 40, 0)])
+def test_outputs_at_any_element(M, N, K, act, out):
+    """odd widths, pitches and offsets of the residual and the output, in place (C ABI); nothing between the rows is written"""
+    import ctypes as C
+    from adcdiff import _lib
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    a, w = _rows16(_codes(gen, M, K)), _rows16(_codes(gen, N, K))
+    sa, sw = torch.rand(M, generator=gen, device="cuda"), torch.rand(N, generator=gen, device="cuda")
+    pitch = N + 3
+    held = torch.randn(M * pitch + 1, generator=gen, device="cuda").to(TYPES[out])
+    before, rows = held.clone(), held[1:].view(M, pitch)[:, :N]
+    want = ops.gemm_int8(a, sa, w, sw, residual=rows.contiguous(), act=act, out_dtype=out)
+    p = _lib.GemmI8Args()
+    p.M, p.N, p.K, p.act, p.out_dtype, p.lda, p.ldw, p.ldr, p.ldo = M, N, K, act, int(out == "bf16"), a.stride(0), w.stride(0), pitch, pitch
+    p.a, p.w, p.a_scale, p.w_scale, p.residual, p.out = (t.data_ptr() for t in (a, w, sa, sw, rows, rows))
+    _lib.check(_lib.load().adcdiff_gemm_i8(C.byref(p), torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(rows, want)
+    assert torch.equal(held[1:].view(M, pitch)[:, N:], before[1:].view(M, pitch)[:, N:]) and held[0] == before[0]
 
 
 @pytest.mark.parametrize("M, N, K", [(1, 64, 1003), (50, 33, 77), (300, 1001, 515)])

@@ -218,6 +218,27 @@ def test_offsets_past_32_bits():
     assert torch.equal(p[0], q[0]) and torch.equal(p[1], q[1])
 
 
+@pytest.mark.parametrize("D", [3, 8, 9, 96, 513, 777, 1024, 4097, 8191])
+@pytest.mark.parametrize("T, R", [(BF, F), (F, BF)])
+def test_output_rows_with_gaps(D, T, R):
+    """x_new and y at an odd pitch and offset (C ABI): the same values, and nothing between the rows is written"""
+    import ctypes as C
+    from adcdiff import _lib
+    M, pitch = 61, D + 3
+    s = _inputs(M, D, T, R, F, 1, "rms", "layer", pitch=1, offset=1)
+    want = ops.residual_norm(s["h"], s["x"], gate=s["gate"], post_norm="rms", pre_norm="layer", residual_scale=0.5)
+    held = [torch.full((M * pitch + 1,), 7.0, device="cuda", dtype=t) for t in (R, T)]
+    xn, y = (t[1:].view(M, pitch) for t in held)
+    a = _lib.ResidualNormArgs()
+    a.M, a.D, a.dtype, a.stream_dtype, a.gate_dtype, a.post_norm, a.pre_norm, a.gate_rows = M, D, int(T == BF), int(R == BF), 0, 1, 2, 1
+    a.h, a.x, a.x_new, a.y = s["h"].data_ptr(), s["x"].data_ptr(), xn.data_ptr(), y.data_ptr()
+    a.gate, a.residual_scale, a.eps = s["gate"].data_ptr(), 0.5, 1e-6
+    a.ldh, a.ldx, a.ldg, a.ldx_new, a.ldy = s["h"].stride(0), s["x"].stride(0), D, pitch, pitch
+    _lib.check(_lib.load().adcdiff_residual_norm(C.byref(a), torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(xn[:, :D], want[0]) and torch.equal(y[:, :D], want[1])
+    assert bool((xn[:, D:] == 7.0).all()) and bool((y[:, D:] == 7.0).all()) and all(float(t[0]) == 7.0 for t in held)
+
+
 @pytest.mark.parametrize("D", [5, 96, 513, 777, 1029, 2048, 4097, 8191, 8192])
 def test_stream_in_place(D):
     """x_new over x and y over h (C ABI), with rows enough for every workgroup to take several"""
