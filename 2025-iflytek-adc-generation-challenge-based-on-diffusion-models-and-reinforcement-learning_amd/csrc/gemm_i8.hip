@@ -84,10 +84,13 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cas
 
 // One row per team, held in registers between the maximum and the codes; bound by HBM (65536 x 2048 bfloat16 79 us, 403 MB at 5.1 TB/s; 4096 x 2048
 // 7.2 us) and by latency below.  PAIRS: rows of q start on 8-byte boundaries and eight codes are one store, those behind K among them.
+template <int TPR>
+constexpr int quantize_threads() { return TPR > 64 ? TPR : threads_for<TPR>(); }
+
 template <typename T, RowShape SHAPE, bool PAIRS, int TPR, int V>
-__global__ __launch_bounds__(threads_for<TPR>()) void quantize_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int8_t* __restrict__ q,
+__global__ __launch_bounds__(quantize_threads<TPR>()) void quantize_rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, int Kp, int8_t* __restrict__ q,
                                                                            long long ldq, float* __restrict__ scale) {
-    constexpr int THREADS = threads_for<TPR>(), TEAMS = THREADS / TPR;
+    constexpr int THREADS = quantize_threads<TPR>(), TEAMS = THREADS / TPR;
     __shared__ uint32_t red[THREADS / 64];
     const int tid = threadIdx.x, t = tid % TPR;
     // a team wider than a wave is alone in its workgroup, so the barriers of the maximum are met by every thread
@@ -156,7 +159,7 @@ struct QuantizeArgs {
 
 template <typename T, RowShape SHAPE, bool PAIRS, int TPR, int V>
 void launch_quantize(const QuantizeArgs& a, hipStream_t stream) {
-    constexpr int threads = threads_for<TPR>(), teams = threads / TPR;
+    constexpr int threads = quantize_threads<TPR>(), teams = threads / TPR;
     hipLaunchKernelGGL((quantize_rows_kernel<T, SHAPE, PAIRS, TPR, V>), dim3((unsigned)std::min(((long long)a.M + teams - 1) / teams, 1LL << 20)), dim3(threads), 0, stream,
                        static_cast<const T*>(a.x), a.ldx, a.M, a.K, a.Kp, a.q, a.ldq, a.scale);
 }
