@@ -355,6 +355,18 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
     return false;
 }
 
+// No operator here has a forward-mode derivative.  A tangent is refused: below autograd it would be dropped, and a result without one counts as constant.
+void no_tangent(const char* name, const Tensor& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name, " has no forward-mode derivative");
+}
+void no_tangents(const char* name, std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        if (t) no_tangent(name, *t);
+}
+void no_tangents(const char* name, at::TensorList tensors) {
+    for (const Tensor& t : tensors) no_tangent(name, t);
+}
+
 // A result without a gradient of its own: asking for one raises instead of leaving it out.  `call` makes the outputs.
 struct Ungraded : torch::autograd::Function<Ungraded> {
     static variable_list forward(AutogradContext* ctx, at::TensorList inputs, const std::function<variable_list()>& call, const std::string& message) {
@@ -388,6 +400,7 @@ std::vector<Tensor> residual_norm_backward_autograd(const OptTensor& h, const Te
     static const auto op = below_autograd("adcdiff::residual_norm_backward", &residual_norm_backward);
     auto call = [&] { return op.call(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, stats, d_x_new, d_y, post_norm, pre_norm, residual_scale, eps, need); };
     const std::initializer_list<const Tensor*> inputs = {&x, ptr(h), ptr(gate), ptr(post_weight), ptr(post_bias), ptr(pre_weight), ptr(pre_bias), ptr(d_x_new), ptr(d_y)};
+    no_tangents("residual_norm_backward", inputs);
     if (wants_grad(inputs)) return ungraded(inputs, call, "residual_norm is differentiable once");
     at::AutoDispatchBelowADInplaceOrView below;
     return call();
@@ -436,7 +449,9 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
 std::vector<Tensor> residual_norm_autograd(const OptTensor& h, const Tensor& x, const OptTensor& gate, const OptTensor& post_weight, const OptTensor& post_bias,
                                            const OptTensor& pre_weight, const OptTensor& pre_bias, int64_t post_norm, int64_t pre_norm,
                                            double residual_scale, double eps, bool with_x, bool with_stats) {
-    if (wants_grad({&x, ptr(h), ptr(gate), ptr(post_weight), ptr(post_bias), ptr(pre_weight), ptr(pre_bias)}))
+    const std::initializer_list<const Tensor*> inputs = {&x, ptr(h), ptr(gate), ptr(post_weight), ptr(post_bias), ptr(pre_weight), ptr(pre_bias)};
+    no_tangents("residual_norm", inputs);
+    if (wants_grad(inputs))
         return ResidualNorm::apply(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x, with_stats);
     static const auto op = below_autograd("adcdiff::residual_norm", &residual_norm);
     at::AutoDispatchBelowADInplaceOrView below;
@@ -446,22 +461,27 @@ std::vector<Tensor> residual_norm_autograd(const OptTensor& h, const Tensor& x, 
 // the norm of gradients that themselves require one (create_graph) is not differentiated
 Tensor grad_norm_autograd(at::TensorList grads, int64_t norm_type) {
     static const auto op = below_autograd("adcdiff::grad_norm", &grad_norm);
+    no_tangents("grad_norm", grads);
     at::AutoDispatchBelowADInplaceOrView below;
     return op.call(grads, norm_type);
 }
 Tensor clip_grad_norm_autograd_(at::TensorList grads, double max_norm, int64_t norm_type) {
     static const auto op = below_autograd("adcdiff::clip_grad_norm_", &clip_grad_norm_);
+    no_tangents("clip_grad_norm_", grads);
     at::AutoDispatchBelowADInplaceOrView below;
     return op.call(grads, max_norm, norm_type);
 }
 Tensor clip_grad_norm_out_autograd(at::TensorList grads, double max_norm, int64_t norm_type, at::TensorList out) {
     static const auto op = below_autograd("adcdiff::clip_grad_norm_out", &clip_grad_norm_out);
+    no_tangents("clip_grad_norm_out", grads);
+    no_tangents("clip_grad_norm_out", out);
     at::AutoDispatchBelowADInplaceOrView below;
     return op.call(grads, max_norm, norm_type, out);
 }
 
 std::tuple<Tensor, Tensor> quantize_rows_autograd(const Tensor& x) {
     static const auto op = below_autograd("adcdiff::quantize_rows", &quantize_rows);
+    no_tangents("quantize_rows", {&x});
     if (wants_grad({&x})) {
         const variable_list outs = ungraded({&x}, [&] { auto r = op.call(x); return variable_list{std::get<0>(r), std::get<1>(r)}; }, kNoLayerGradient);
         return {outs[0], outs[1]};
@@ -473,6 +493,7 @@ Tensor gemm_int8_autograd(const Tensor& a, const Tensor& a_scale, const Tensor& 
                           int64_t act, int64_t out_dtype) {
     static const auto op = below_autograd("adcdiff::gemm_int8", &gemm_int8);
     const std::initializer_list<const Tensor*> inputs = {&a_scale, &w_scale, ptr(bias), ptr(residual)};
+    no_tangents("gemm_int8", inputs);
     if (wants_grad(inputs))
         return ungraded(inputs, [&] { return variable_list{op.call(a, a_scale, w, w_scale, bias, residual, act, out_dtype)}; }, kNoLayerGradient)[0];
     at::AutoDispatchBelowADInplaceOrView below;
@@ -482,6 +503,7 @@ Tensor linear_int8_autograd(const Tensor& x, const Tensor& w, const Tensor& w_sc
                             int64_t out_dtype) {
     static const auto op = below_autograd("adcdiff::linear_int8", &linear_int8);
     const std::initializer_list<const Tensor*> inputs = {&x, &w_scale, ptr(bias), ptr(residual)};
+    no_tangents("linear_int8", inputs);
     if (wants_grad(inputs))
         return ungraded(inputs, [&] { return variable_list{op.call(x, w, w_scale, bias, residual, act, out_dtype)}; }, kNoLayerGradient)[0];
     at::AutoDispatchBelowADInplaceOrView below;

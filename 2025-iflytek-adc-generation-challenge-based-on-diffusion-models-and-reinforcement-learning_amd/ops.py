@@ -331,7 +331,7 @@ def residual_norm(h, x, gate=None, post_norm=None, post_weight=None, post_bias=N
     group of consecutive rows, one for each row).  Types float32 and bfloat16; x_new has x's type, y has h's; float32 inside, one
     rounding per output.  Any row pitch and any D from 1 to 8192.
 
-    Differentiable once in every tensor; gradients of a shared gate and of the weights are summed in a fixed order.  Works under
+    Differentiable once in every tensor, in reverse mode (a tangent raises); gradients of a shared gate and of the weights are summed in a fixed order.  Works under
     graph capture; where a backward pass is captured, no other graph of the same leaves may be alive on another stream (autograd's
     accumulation belongs to the stream of a leaf's first use), or torch.ops.adcdiff.residual_norm_backward is called directly."""
     if gate is not None and gate.dim() == 1:
