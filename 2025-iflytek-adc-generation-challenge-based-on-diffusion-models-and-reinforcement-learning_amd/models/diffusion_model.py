@@ -491,6 +491,7 @@ class UNetModel(nn.Module):
 
     def forward(self, x: torch.Tensor, t: torch.Tensor, condition: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Predicted noise for x [B, input_dim], per-row timesteps t [B] (diffusion_model.py:749-789)."""
+        ops._no_tangents("UNetModel", x, condition)
         dev = self._device()
         ops._need_gpu(x, t, condition)
         eng = self.engine()

@@ -11,6 +11,7 @@ the PyTorch dispatcher: they call the custom operators ``torch.ops.adcdiff.*`` r
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import BF16, F32, AdcdiffError, check
@@ -28,6 +29,14 @@ def _need_gpu(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise AdcdiffError("adcdiff kernels run on an MI355X only; got a %s tensor (no CPU fallback exists)" % t.device)
+
+
+def _no_tangents(name, *tensors):
+    """A custom operator drops a forward-mode tangent without a word where no input requires a gradient: refused before the dispatcher."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("%s has no forward-mode derivative" % name)
 
 
 def dtype_code(name):
@@ -242,6 +251,7 @@ class timing:
 def gemm(a_list, w, bias=None, rowbias=None, rowbias_idx=None, residual=None, act=0, out_f32=True, out_op=False, gn=(),
          m_valid=None, dtype="fp32", eps=1e-5, tile_hint=0, split_k=0):
     """adcdiff_gemm through the dispatcher; arguments and results as _raw_gemm."""
+    _no_tangents("gemm", *a_list, w, bias, rowbias, residual, *(v for g in gn for v in g[:2]))
     from . import torch_ops  # noqa: F401  (registers the operators)
     outs = torch.ops.adcdiff.gemm(list(a_list), w, bias, rowbias, rowbias_idx, residual, int(act), bool(out_f32), bool(out_op),
                                   [g[0] for g in gn], [g[1] for g in gn], [int(g[2]) for g in gn], 0 if m_valid is None else int(m_valid),
@@ -250,6 +260,7 @@ def gemm(a_list, w, bias=None, rowbias=None, rowbias_idx=None, residual=None, ac
 
 
 def groupnorm_silu(x, groups, gamma, beta, eps=1e-5, out_dtype="fp32", with_raw=False):
+    _no_tangents("groupnorm_silu", x, gamma, beta)
     from . import torch_ops  # noqa: F401
     outs = torch.ops.adcdiff.groupnorm_silu(x, int(groups), gamma, beta, float(eps), dtype_code(out_dtype), bool(with_raw))
     return (outs[0], outs[1]) if with_raw else outs[0]
@@ -261,6 +272,7 @@ def philox_normal(rows, cols, seed, stream_id, step, row_offset=0, device="cuda"
 
 
 def ddpm_step(x, eps, coef, noise=None, seed=0, step=0, row_offset=0, out=None):
+    _no_tangents("ddpm_step", x, eps, noise)
     from . import torch_ops  # noqa: F401
     c = [float(v) for v in coef]
     res = torch.ops.adcdiff.ddpm_step(x, eps, noise, c[0], c[1], c[2], c[3], int(seed), int(step), int(row_offset))
@@ -271,6 +283,7 @@ def ddpm_step(x, eps, coef, noise=None, seed=0, step=0, row_offset=0, out=None):
 
 
 def ddim_step(x, eps, coef, noise=None, seed=0, step=0, row_offset=0, out=None):
+    _no_tangents("ddim_step", x, eps, noise)
     from . import torch_ops  # noqa: F401
     c = [float(v) for v in coef]
     res = torch.ops.adcdiff.ddim_step(x, eps, noise, c[0], c[1], c[2], c[3], c[4], int(seed), int(step), int(row_offset))
@@ -281,6 +294,7 @@ def ddim_step(x, eps, coef, noise=None, seed=0, step=0, row_offset=0, out=None):
 
 
 def q_sample(x0, t, sqrt_ac, sqrt_1mac, noise=None, seed=0, step=0, row_offset=0, return_noise=False):
+    _no_tangents("q_sample", x0, sqrt_ac, sqrt_1mac, noise)
     from . import torch_ops  # noqa: F401
     out, used = torch.ops.adcdiff.q_sample(x0, t, sqrt_ac, sqrt_1mac, noise, int(seed), int(step), int(row_offset))
     return (out, used) if return_noise else out
@@ -288,6 +302,7 @@ def q_sample(x0, t, sqrt_ac, sqrt_1mac, noise=None, seed=0, step=0, row_offset=0
 
 def latent_summary(x):
     """[B, D] float32 latents -> [B, 5] float32 (mean, sum, x[:, 3], x[:, 5], x[:, 8]) with numpy's float32 summation order."""
+    _no_tangents("latent_summary", x)
     from . import torch_ops  # noqa: F401
     if x.dtype != torch.float32 or x.dim() != 2 or x.stride(1) != 1:
         raise ValueError("latent_summary expects a [B, D] float32 tensor with contiguous rows")

@@ -1,11 +1,11 @@
-"""Derivatives that the operators around a residual block do not have are refused, never left out: a result without a tangent counts as
+"""Derivatives that an operator does not have are refused, never left out: a result without a tangent counts as
 constant.  On fake tensors: the refusals come before any kernel."""
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
 
-import adcdiff  # noqa: F401
+import adcdiff
 from adcdiff import ops
 
 
@@ -59,3 +59,30 @@ def test_forward_mode_is_refused(name):
                 call(dual)
         with pytest.raises(NotImplementedError, match="forward"):
             torch.func.jvp(lambda v: (call(v), v)[1], (_gpu(4, 32),), (_gpu(4, 32),))
+
+
+# functions of the sampling path, on the CPU: the refusal comes before the one of CPU tensors
+PATH_CALLS = {
+    "gemm a": lambda d: ops.gemm([d], torch.empty(16, 32)),
+    "gemm w": lambda d: ops.gemm([torch.empty(4, 32)], d),
+    "gemm residual": lambda d: ops.gemm([torch.empty(4, 8)], torch.empty(32, 8), residual=d),
+    "groupnorm_silu x": lambda d: ops.groupnorm_silu(d, 4, torch.ones(32), torch.zeros(32)),
+    "groupnorm_silu gamma": lambda d: ops.groupnorm_silu(torch.ones(4, 128), 4, d.reshape(128), torch.zeros(128)),
+    "ddpm_step": lambda d: ops.ddpm_step(d, torch.empty(4, 32), (1.0, 0.1, 0.5, 0.2)),
+    "ddim_step": lambda d: ops.ddim_step(torch.empty(4, 32), d, (1.0, 0.1, 0.5, 0.2, 0.1)),
+    "q_sample": lambda d: ops.q_sample(d, torch.zeros(4, dtype=torch.int64), torch.ones(10), torch.ones(10)),
+    "latent_summary": lambda d: ops.latent_summary(d),
+    "model": lambda d: adcdiff.UNetModel(32, 32, 32, 10, strict_shapes=False)(d, torch.zeros(4, dtype=torch.int64)),
+}
+
+
+@pytest.mark.parametrize("name", list(PATH_CALLS))
+def test_forward_mode_of_the_path_is_refused(name):
+    call = PATH_CALLS[name]
+    with forward_ad.dual_level():
+        with pytest.raises(adcdiff.AdcdiffError):     # as without forward mode: no CPU path
+            call(torch.zeros(4, 32))
+        with pytest.raises(NotImplementedError, match="forward"):
+            call(forward_ad.make_dual(torch.zeros(4, 32), torch.zeros(4, 32)))
+    with pytest.raises(NotImplementedError, match="forward"):
+        torch.func.jvp(call, (torch.zeros(4, 32),), (torch.zeros(4, 32),))
