@@ -230,6 +230,11 @@ __device__ __forceinline__ float silu_fast(float v) {
     return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896f));
 }
 
+// The sum times both scales, |sum| < 2^31.  The row's scale first stays finite below 2^96, and a sum is at least 1, so nothing is lost below either (a
+// subnormal scale times a whole number is exact until it is normal).  From 2^96 on the output's scale comes first: where that overflows, so does the value.
+__device__ __forceinline__ bool far_scale(float sa) { return fabsf(sa) >= 0x1p96f; }
+__device__ __forceinline__ float scaled(int sum, float sa, float w, float b, bool far) { return fmaf((float)sum * (far ? w : sa), far ? sa : w, b); }
+
 // 16 bytes of a row from column k on, with the bytes at columns >= K cleared.  Rows start on 16-byte boundaries, so a chunk that holds a
 // valid byte never leaves the page of that byte: the bytes behind K may be read, and count for nothing.
 __device__ __forceinline__ i32x4 load_chunk(const int8_t* __restrict__ row, int k, int K) {
@@ -286,10 +291,11 @@ struct Finish8 {
     }
     __device__ __forceinline__ void store(const I8Params& p, int m, int n, const i32x4& lo, const i32x4& hi) const {
         Out* out = static_cast<Out*>(p.out) + (long long)m * p.ldo + n;
+        const bool far = far_scale(sa);
         Eight o;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            float v = c < 4 ? fmaf((float)lo[c & 3] * sa, w0[c & 3], b0[c & 3]) : fmaf((float)hi[c & 3] * sa, w1[c & 3], b1[c & 3]);
+            float v = c < 4 ? scaled(lo[c & 3], sa, w0[c & 3], b0[c & 3], far) : scaled(hi[c & 3], sa, w1[c & 3], b1[c & 3], far);
             if (p.residual) v += (float)r[c];
             if (p.act) v = silu_fast(v);
             o[c] = (Out)v;
@@ -600,18 +606,30 @@ __global__ __launch_bounds__(256, 1) void gemm_i8_w4_kernel(const I8Params p) {
         }
     };
     fetch(0);
+    bool far = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) far |= far_scale(sa[i]);
+    const bool any_far = __any(far);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const long long m = mw + 16 * i + frow;
         if (i < 7) fetch(i + 1);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float v[8];
+            float v[8], sum[8];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const auto s = __builtin_amdgcn_permlane16_swap((unsigned)acc[i][2 * j][c], (unsigned)acc[i][2 * j + 1][c], false, false);
-                v[c] = fmaf((float)(int)s[0] * sa[i], w[j][c], b[j][c]);
-                v[4 + c] = fmaf((float)(int)s[1] * sa[i], w[j][4 + c], b[j][4 + c]);
+                sum[c] = (float)(int)s[0];
+                sum[4 + c] = (float)(int)s[1];
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] = fmaf(sum[c] * sa[i], w[j][c], b[j][c]);
+            if (__builtin_expect(any_far, 0)) {   // (selecting both factors in every output, or the loop twice, cost up to 3 %)
+                if (far_scale(sa[i])) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) v[c] = fmaf(sum[c] * w[j][c], sa[i], b[j][c]);
+                }
             }
             if (residual) {
 #pragma unroll
