@@ -36,7 +36,8 @@ def build_library(force=False, verbose=False):
     inc_i8 = os.path.join(CSRC, "w4_mainloop_i8.inc")
     if force or _stale(inc_i8, [gen]):
         subprocess.run([sys.executable, gen, "--i8", inc_i8], check=True)
-    headers = [inc_i8, os.path.join(CSRC, "common.h"), os.path.join(CSRC, "row_access.h"), os.path.join(CSRC, "unet_plan.h"), inc, os.path.join(os.path.dirname(HERE), "include", "adcdiff.h")]
+    # this file among them: it holds the flags, and objects of other flags must not be linked
+    headers = [os.path.abspath(__file__), inc_i8, os.path.join(CSRC, "common.h"), os.path.join(CSRC, "row_access.h"), os.path.join(CSRC, "unet_plan.h"), inc, os.path.join(os.path.dirname(HERE), "include", "adcdiff.h")]
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
     objs, cmds = [], []
@@ -65,7 +66,7 @@ def build_binding(force=False, verbose=False):
     src = os.path.join(CSRC, "torch_binding.cpp")
     import torch
     from torch.utils import cpp_extension
-    deps = [src, os.path.join(os.path.dirname(HERE), "include", "adcdiff.h"), torch.__file__]
+    deps = [os.path.abspath(__file__), src, os.path.join(os.path.dirname(HERE), "include", "adcdiff.h"), torch.__file__]
     if force or _stale(BINDING, deps):
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
                "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I/opt/rocm/include"]
