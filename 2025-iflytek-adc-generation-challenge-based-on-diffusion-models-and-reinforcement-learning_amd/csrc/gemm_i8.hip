@@ -233,7 +233,6 @@ __device__ __forceinline__ float silu_fast(float v) {
 // The sum times both scales, |sum| < 2^31.  The row's scale first stays finite below 2^96, and a sum is at least 1, so nothing is lost below either (a
 // subnormal scale times a whole number is exact until it is normal).  From 2^96 on the output's scale comes first: where that overflows, so does the value.
 __device__ __forceinline__ bool far_scale(float sa) { return fabsf(sa) >= 0x1p96f; }
-__device__ __forceinline__ float scaled(int sum, float sa, float w, float b, bool far) { return fmaf((float)sum * (far ? w : sa), far ? sa : w, b); }
 
 // 16 bytes of a row from column k on, with the bytes at columns >= K cleared.  Rows start on 16-byte boundaries, so a chunk that holds a
 // valid byte never leaves the page of that byte: the bytes behind K may be read, and count for nothing.
@@ -291,14 +290,22 @@ struct Finish8 {
     }
     __device__ __forceinline__ void store(const I8Params& p, int m, int n, const i32x4& lo, const i32x4& hi) const {
         Out* out = static_cast<Out*>(p.out) + (long long)m * p.ldo + n;
+        float v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = c < 4 ? fmaf((float)lo[c & 3] * sa, w0[c & 3], b0[c & 3]) : fmaf((float)hi[c & 3] * sa, w1[c & 3], b1[c & 3]);
         const bool far = far_scale(sa);
+        if (__builtin_expect(__any(far), 0)) {
+            if (far) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[c] = c < 4 ? fmaf((float)lo[c & 3] * w0[c & 3], sa, b0[c & 3]) : fmaf((float)hi[c & 3] * w1[c & 3], sa, b1[c & 3]);
+            }
+        }
         Eight o;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            float v = c < 4 ? scaled(lo[c & 3], sa, w0[c & 3], b0[c & 3], far) : scaled(hi[c & 3], sa, w1[c & 3], b1[c & 3], far);
-            if (p.residual) v += (float)r[c];
-            if (p.act) v = silu_fast(v);
-            o[c] = (Out)v;
+            if (p.residual) v[c] += (float)r[c];
+            if (p.act) v[c] = silu_fast(v[c]);
+            o[c] = (Out)v[c];
         }
         if (n + 8 <= p.N) {
             *reinterpret_cast<EightAny*>(out) = o;
