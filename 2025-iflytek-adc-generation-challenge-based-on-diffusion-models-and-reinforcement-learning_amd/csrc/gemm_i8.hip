@@ -714,22 +714,38 @@ int launch_ring(const I8Params& p, hipStream_t stream) {
 //     64 x 64 ring     2.0 + 0.65 r + (0.09 + 0.25 r) kt:   512 x 2048 x 2048 8.6 (128 x 128: 15.0, 256 x 256: 25.6), 1024 x 2048 x 2048 11.2 (15.9, 26.0)
 //     128 x 128 ring   3.7 + 2.9 r + (0.23 + 0.42 r) kt:    2048 x 2048 x 2048 16.8 (20.6, 27.3), 4096 x 2048 x 2048 26.0 (37.9, 29.4)
 //     256 x 256        a round of 256 workgroups 10.9 + 1.45 kt, one of at most 128 11 + 1.1 kt:  8192 x 2048 x 2048 34.1 (66.9, 46.1), 65536 x 512 x 512 33.4 (52.8, 41.9)
-template <typename Out>
-int launch_gemm(const I8Params& p, hipStream_t stream) {
+// The result names the tile: 16 (16 x 16), 3216 (32 x 16), 32 (32 x 32), 64, 128, 256.
+int choose_kernel(const I8Params& p, bool whole256) {
     auto tiles = [&](int bm, int bn) { return (((long long)p.M + bm - 1) / bm) * (((long long)p.N + bn - 1) / bn); };
-    if (p.M <= 16 || tiles(16, 16) <= 256) return launch_split<Out, 16, 16, 8, 4>(p, stream);
-    if (tiles(32, 16) <= 256) return launch_split<Out, 32, 16, 8, 4>(p, stream);
-    if (tiles(32, 32) <= 256) return launch_split<Out, 32, 32, 8, 2>(p, stream);
+    if (p.M <= 16 || tiles(16, 16) <= 256) return 16;
+    if (tiles(32, 16) <= 256) return 3216;
+    if (tiles(32, 32) <= 256) return 32;
     const double kt = (p.K + 127) / 128;
     const double r64 = std::max(1.0, tiles(64, 64) / 256.0), r128 = std::max(1.0, tiles(128, 128) / 256.0);
     const double t64 = 2.0 + 0.65 * r64 + (0.09 + 0.25 * r64) * kt, t128 = 3.7 + 2.9 * r128 + (0.23 + 0.42 * r128) * kt;
-    // the 256 x 256 kernel needs whole tiles in every direction and 32-bit offsets inside them
-    if (p.M >= 256 && p.N >= 256 && p.K >= 256 && p.lda < (1 << 23) && p.ldw < (1 << 23)) {
+    if (whole256) {
         const long long n = tiles(256, 256), last = n % 256;
         const double t256 = (double)((n + 127) / 256) * (10.9 + 1.45 * kt) + (last > 0 && last <= 128 ? 11.0 + 1.1 * kt : 0.0);
-        if (t256 < std::min(t64, t128)) return launch_w4_side<Out>(p, stream);
+        if (t256 < std::min(t64, t128)) return 256;
     }
-    return t64 < t128 ? launch_ring<Out, 64, 64, 3>(p, stream) : launch_ring<Out, 128, 128, 2>(p, stream);
+    return t64 < t128 ? 64 : 128;
+}
+
+template <typename Out>
+int launch_gemm(const I8Params& p, hipStream_t stream) {
+    // the 256 x 256 kernel needs whole tiles in every direction and 32-bit offsets inside them
+    const bool whole256 = p.M >= 256 && p.N >= 256 && p.K >= 256 && p.lda < (1 << 23) && p.ldw < (1 << 23);
+    const long long forced = debug_value(DBG_GEMM_I8_KERNEL);
+    if (forced == 256 && !whole256) return fail(ADCDIFF_E_BADARG, "gemm_i8: gemm_i8_kernel = 256 asks for M, N and K of 256 and pitches below 2^23, got %d x %d x %d", p.M, p.N, p.K);
+    switch (forced ? forced : choose_kernel(p, whole256)) {
+        case 16: return launch_split<Out, 16, 16, 8, 4>(p, stream);
+        case 3216: return launch_split<Out, 32, 16, 8, 4>(p, stream);
+        case 32: return launch_split<Out, 32, 32, 8, 2>(p, stream);
+        case 64: return launch_ring<Out, 64, 64, 3>(p, stream);
+        case 128: return launch_ring<Out, 128, 128, 2>(p, stream);
+        case 256: return launch_w4_side<Out>(p, stream);
+    }
+    return fail(ADCDIFF_E_BADARG, "gemm_i8: gemm_i8_kernel = %lld names no kernel", forced);
 }
 
 constexpr int kMaxK = 131071;   // 128 * 128 * K stays below 2^31

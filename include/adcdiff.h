@@ -484,6 +484,8 @@ int adcdiff_pitch_rows_i8(const adcdiff_i8_copy* copies, int n, adcdiff_stream_t
  *                        K tiles of its successor workgroup on the same XCD will read
  *   gemm_splitk (1)      0 = never the few-row kernel that splits K over workgroups (splitk_scratch is ignored): small batches are
  *                        then bit-identical to large ones
+ *   gemm_i8_kernel (0)   16 / 3216 / 32 (few-row tiles of 16 x 16, 32 x 16, 32 x 32), 64 / 128 (square tiles through LDS) or 256 (256 x 256):
+ *                        that kernel for every adcdiff_gemm_i8; calls that it cannot take are rejected (256: M, N, K of at least 256)
  *   step_fold (1)        0 = the reverse step and encoder.0's GroupNorm as launches of their own in the sampling loops
  *   train_transpose (0)  1 = backward products on transposed copies instead of adcdiff_gemm_tr
  *   train_group_dw (1)   0 = every weight-gradient product of adcdiff_unet_backward as a launch of its own (split over the batch,
