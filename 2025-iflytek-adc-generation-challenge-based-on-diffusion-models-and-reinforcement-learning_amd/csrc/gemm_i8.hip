@@ -749,13 +749,14 @@ int launch_gemm(const I8Params& p, hipStream_t stream) {
 }
 
 constexpr int kMaxK = 131071;   // 128 * 128 * K stays below 2^31
+constexpr int kMaxRow = 1 << 30;   // columns of a quantised row: 32-bit counters step 1024 past the last one
 
 }  // namespace
 }  // namespace adcdiff
 
 extern "C" int adcdiff_quantize_rows(const void* x, long long ldx, int dtype, int M, int K, int8_t* q, long long ldq, float* scale, adcdiff_stream_t stream_) {
     using namespace adcdiff;
-    if (M < 0 || K < 1) return fail(ADCDIFF_E_BADARG, "quantize_rows: %d rows of %d columns", M, K);
+    if (M < 0 || K < 1 || K > kMaxRow) return fail(ADCDIFF_E_BADARG, "quantize_rows: %d rows of %d columns (1..%d)", M, K, kMaxRow);
     if (!type_ok(dtype)) return fail(ADCDIFF_E_BADARG, "quantize_rows: type %d", dtype);
     if (M == 0) return ADCDIFF_OK;
     if (!x || !q || !scale) return fail(ADCDIFF_E_BADARG, "quantize_rows: null pointer");

@@ -428,7 +428,7 @@ int adcdiff_clip_grad_norm(const adcdiff_grad_tensor* tensors, int n_tensors, in
 /* Codes of the rows of x [M, K] (dtype): scale[r] = max_k |x[r, k]| / 127 and q[r, k] = x[r, k] * 127 / max|x[r]| rounded half to even,
  * exactly (no second rounding near a tie).  A row of zeros has scale 0 and codes 0; a row with a NaN or an infinity has scale NaN and codes
  * 0, so that what it stands for, and every product with it, is NaN.  q has a pitch of ldq >= K bytes; columns K .. min(ldq, K rounded up to
- * 16) - 1 are written as 0.  Serves activations (a scale for each token) and weights [N, K] (a scale for each channel) alike. */
+ * 16) - 1 are written as 0.  K up to 2^30.  Serves activations (a scale for each token) and weights [N, K] (a scale for each channel) alike. */
 int adcdiff_quantize_rows(const void* x, long long ldx, int dtype, int M, int K, int8_t* q, long long ldq, float* scale, adcdiff_stream_t stream);
 
 /* out[m, n] = act(a_scale[m] * w_scale[n] * sum_k a[m, k] w[n, k] + bias[n] + residual[m, n]) on v_mfma_i32_16x16x64_i8: the sum is exact
