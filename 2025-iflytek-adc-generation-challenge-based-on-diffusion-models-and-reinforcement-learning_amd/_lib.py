@@ -189,11 +189,14 @@ def load():
     if not os.path.exists(LIB_PATH):
         raise AdcdiffError("%s is missing: run `python -c 'import __graft_entry__ as g; g.build()'` (hipcc, gfx950). "
                            "There is no CPU or PyTorch fallback for this path." % LIB_PATH)
-    lib = C.CDLL(LIB_PATH, mode=C.RTLD_GLOBAL)     # the torch binding resolves the C entry points from it
-    for name, (res, args) in SIGNATURES.items():
-        fn = getattr(lib, name)
-        fn.restype = res
-        fn.argtypes = args
+    try:
+        lib = C.CDLL(LIB_PATH, mode=C.RTLD_GLOBAL)     # the torch binding resolves the C entry points from it
+        for name, (res, args) in SIGNATURES.items():
+            fn = getattr(lib, name)
+            fn.restype = res
+            fn.argtypes = args
+    except (OSError, AttributeError) as e:
+        raise AdcdiffError("%s does not load, or is older than this package (build it again): %s" % (LIB_PATH, e)) from e
     if lib.adcdiff_abi_version() != 3:
         raise AdcdiffError("libadcdiff.so has ABI version %d, expected 3" % lib.adcdiff_abi_version())
     _lib = lib
@@ -208,7 +211,10 @@ def load_binding():
         if not os.path.exists(BINDING_PATH):
             raise AdcdiffError("%s is missing: run `python -c 'import __graft_entry__ as g; g.build()'`." % BINDING_PATH)
         import torch
-        torch.ops.load_library(BINDING_PATH)
+        try:
+            torch.ops.load_library(BINDING_PATH)
+        except OSError as e:
+            raise AdcdiffError("%s does not load with torch %s (build it again): %s" % (BINDING_PATH, torch.__version__, e)) from e
         _binding = True
 
 

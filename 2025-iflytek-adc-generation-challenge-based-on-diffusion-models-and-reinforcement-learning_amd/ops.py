@@ -318,7 +318,8 @@ def _call(name, *args):
     """torch.ops.adcdiff.<name>(*args); what the library refuses is raised as AdcdiffError."""
     op = _operators.get(name)
     if op is None:
-        _lib.load_binding()     # says so if it was not built
+        from . import torch_ops
+        torch_ops.load_binding()     # says so if it was not built
         op = _operators[name] = getattr(torch.ops.adcdiff, name).default
     try:
         return op(*args)

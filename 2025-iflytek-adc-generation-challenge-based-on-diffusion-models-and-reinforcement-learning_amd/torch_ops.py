@@ -19,7 +19,6 @@ The training loss stays a ``torch.autograd.Function`` (models/diffusion_model.py
 which an autograd formula returning one tensor per parameter could not do without a copy.
 """
 import ctypes as C
-import os
 from typing import List, Optional, Tuple
 
 import torch
@@ -284,11 +283,24 @@ _FAKES = {
     "gemm_int8": lambda a, a_scale, w, w_scale, bias, residual, act, out_dtype: a.new_empty((a.shape[0], w.shape[0]), dtype=_td(out_dtype)),
     "linear_int8": lambda x, w, w_scale, bias, residual, act, out_dtype: x.new_empty((x.shape[0], w.shape[0]), dtype=_td(out_dtype)),
 }
-if os.path.exists(_lib.LIB_PATH) and os.path.exists(_lib.BINDING_PATH):     # a tree that is not built yet still imports; ops.py says so on use
-    _lib.load_binding()
-    for _name, _fake in _FAKES.items():
-        torch.library.register_fake("adcdiff::" + _name, _fake)
-        getattr(torch.ops.adcdiff, _name)     # listed by names()
+_binding_ready = False
+
+
+def load_binding():
+    """Load the operators that csrc/torch_binding.cpp registers, with their fake-tensor rules; raises if they cannot be."""
+    global _binding_ready
+    if not _binding_ready:
+        _lib.load_binding()
+        for name, fake in _FAKES.items():
+            torch.library.register_fake("adcdiff::" + name, fake)
+            getattr(torch.ops.adcdiff, name)     # listed by names()
+        _binding_ready = True
+
+
+try:
+    load_binding()
+except _lib.AdcdiffError:     # not built yet, or for another torch: the package still imports, and ops.py says so on use
+    pass
 
 
 def names():
