@@ -82,7 +82,7 @@ __device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red, int tid)
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-// One row per team, held in registers between the maximum and the codes; bound by HBM (65536 x 2048 bfloat16 79 us, 403 MB at 5.1 TB/s; 4096 x 2048
+// One row per team, held in registers between the maximum and the codes; bound by HBM (65536 x 2048 bfloat16 74 us, 403 MB at 5.4 TB/s; 4096 x 2048
 // 7.2 us) and by latency below.  PAIRS: rows of q start on 8-byte boundaries and eight codes are one store, those behind K among them.
 template <int TPR>
 constexpr int quantize_threads() { return TPR > 64 ? TPR : threads_for<TPR>(); }
@@ -322,9 +322,10 @@ struct Finish8 {
 // instruction).  The chunk c of a row lies at position c ^ ((row >> 1) & 7), applied to the source address, so fragment reads are free of bank
 // conflicts.  STAGES - 1 tiles are under way; a stage is refilled behind the barrier that follows the last wait for its reads.  The weights are
 // the MFMA's first operand: a lane's four results are consecutive outputs of a row.
-// The loop is bound by LDS: a K tile of 128 x 128 takes 0.7 us whether one workgroup runs or all do, with the rows' lines in L2 or not
-// (a prefetch into L2 and an order of tiles that shares more rows there changed nothing), which is its 96 KiB of fragment reads and 32 KiB of DMA
-// writes at 64 bytes per cycle.  So two or three workgroups share a CU (two stages of 32 KiB, three of 16 KiB): each covers the others' barriers and
+// Bound by the waits between its steps, not by one unit (4096 x 2048 x 2048, counters): the matrix cores are busy in 43 % of the CUs' cycles and LDS reads
+// take 36 %, while the waves spend 41 % of their time behind a wait or barrier and 34 % ready for an issue slot that another wave has.  A K tile of
+// 128 x 128 takes 0.7 us whether one workgroup runs or all do, with the rows' lines in L2 or not (a prefetch into L2 and an order of tiles that shares
+// more rows there changed nothing).  So two or three workgroups share a CU (two stages of 32 KiB, three of 16 KiB): each covers the others' barriers and
 // epilogues (4096 x 2048 x 2048: 26 us, four stages and one workgroup 32 us, 256 x 128 tiles 27 us).
 template <typename Out, int BM, int BN, int STAGES>
 __global__ __launch_bounds__(512) void gemm_i8_ring_kernel(const I8Params p) {

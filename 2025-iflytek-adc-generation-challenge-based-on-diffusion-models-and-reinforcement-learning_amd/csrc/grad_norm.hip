@@ -42,7 +42,9 @@ __device__ __forceinline__ int find_entry(const GradTable& g, int chunk) {
 
 // Gradients are aligned to their element only (views into an arena); the memory system takes 16-byte accesses at any address.
 
-struct SumSquares {   // float64: any float32 gradient squares without overflow or underflow, and the sum is exact to 2^-53
+// float64: any float32 gradient squares exactly, without overflow or underflow; the sum takes one rounding of 2^-53 for each addition on an element's
+// path (32 in a thread, 6 + 4 in the workgroup, and as many again over the chunks), far below the 2^-24 of the result's own
+struct SumSquares {
     typedef double Acc;
     static __device__ __forceinline__ double zero() { return 0.0; }
     static __device__ __forceinline__ void add(double& s, float v) { s = fma((double)v, (double)v, s); }

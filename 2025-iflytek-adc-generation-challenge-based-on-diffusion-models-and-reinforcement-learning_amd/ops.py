@@ -344,8 +344,8 @@ def residual_norm(h, x, gate=None, post_norm=None, post_weight=None, post_bias=N
     h [M, D]: what the block computed; x [M, D]: the residual stream, which may have another type (float32 under bfloat16 blocks).
     post_norm / pre_norm: None, "rms" (v / sqrt(mean(v^2) + eps)) or "layer" (of v - mean(v)), each with an optional float32 weight
     and bias [D].  gate: [D] or [G, D] with G dividing M: row r reads gate row r // (M / G) (one gate for all rows, one for each
-    group of consecutive rows, one for each row).  Types float32 and bfloat16; x_new has x's type, y has h's; float32 inside, one
-    rounding per output.  Any row pitch and any D from 1 to 8192.
+    group of consecutive rows, one for each row).  Types float32 and bfloat16; x_new has x's type, y has h's; float32 inside (squares
+    of more than 1e38 in a row overflow), one rounding per output.  Any row pitch and any D from 1 to 8192.
 
     Differentiable once in every tensor, in reverse mode (a tangent raises); gradients of a shared gate and of the weights are summed in a fixed order.  Works under
     graph capture; where a backward pass is captured, no other graph of the same leaves may be alive on another stream (autograd's

@@ -348,8 +348,8 @@ int adcdiff_clip_adamw_step_noalloc(const adcdiff_opt_tensor* tensors, int n_ten
 /* The norms before and after a residual block, fused with the block's gate and the residual scale (the seam between two blocks of a
  * conditioned denoiser; no counterpart in the reference, whose blocks add h + residual bare, diffusion_model.py:907):
  *   x_new = residual_scale * x + gate . N_post(h),   y = N_pre(x_new),   N(v) = (v - [mean]) / sqrt(mean((v - [mean])^2) + eps) . weight + bias
- * norm kinds: 0 none (N(v) = v), 1 rms (no [mean]), 2 layer.  Arithmetic in float32, one rounding per output; y is formed from the
- * unrounded x_new.
+ * norm kinds: 0 none (N(v) = v), 1 rms (no [mean]), 2 layer.  Arithmetic in float32 (a row's sum of squares stays below
+ * 3e38), one rounding per output; y is formed from the unrounded x_new.
  *   h, y           [M, ld >= D] in dtype;  h NULL: x_new = x, only y = N_pre(x) is formed (no gate, no post norm, residual_scale 1)
  *   x, x_new       [M, ld >= D] in stream_dtype; x_new NULL: not written.  x_new may alias x, and y may alias h (the same rows)
  *   gate           [gate_rows, ldg] in gate_dtype, or NULL; gate_rows divides M and row r reads gate row r / (M / gate_rows); ldg = 0
