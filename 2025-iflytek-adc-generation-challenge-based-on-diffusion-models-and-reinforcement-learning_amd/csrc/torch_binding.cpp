@@ -384,13 +384,6 @@ struct Ungraded : torch::autograd::Function<Ungraded> {
     }
 };
 
-bool wants_grad(at::TensorList tensors) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor& t : tensors)
-        if (t.requires_grad()) return true;
-    return false;
-}
-
 variable_list ungraded(std::initializer_list<const Tensor*> tensors, const std::function<variable_list()>& call, const char* message) {
     variable_list inputs;
     for (const Tensor* t : tensors)
@@ -465,14 +458,10 @@ std::vector<Tensor> residual_norm_autograd(const OptTensor& h, const Tensor& x, 
     return op.call(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x, with_stats);
 }
 
-// The norm of gradients that themselves require one (create_graph) has no gradient; clipping them is not recorded, as torch.nn.utils.clip_grad_norm_ is not.
+// the norm of gradients that themselves require one (create_graph) is not differentiated
 Tensor grad_norm_autograd(at::TensorList grads, int64_t norm_type) {
     static const auto op = below_autograd("adcdiff::grad_norm", &grad_norm);
     no_tangents("grad_norm", grads);
-    if (wants_grad(grads)) {
-        const std::function<variable_list()> call = [&] { return variable_list{op.call(grads, norm_type)}; };
-        return Ungraded::apply(grads, call, std::string("grad_norm has no gradient"))[0];
-    }
     at::AutoDispatchBelowADInplaceOrView below;
     return op.call(grads, norm_type);
 }

@@ -86,17 +86,3 @@ def test_forward_mode_of_the_path_is_refused(name):
             call(forward_ad.make_dual(torch.zeros(4, 32), torch.zeros(4, 32)))
     with pytest.raises(NotImplementedError, match="forward"):
         torch.func.jvp(call, (torch.zeros(4, 32),), (torch.zeros(4, 32),))
-
-
-def test_norm_of_tensors_that_require_a_gradient():
-    """its result is part of the graph, so that backward can refuse (a detached one would be left out of a sum)"""
-    with FakeTensorMode():
-        p = _gpu(4, 32).requires_grad_()
-        for kind in (2.0, "inf"):
-            norm = ops.grad_norm([_gpu(3), p * 2.0], kind)
-            assert norm.shape == () and norm.dtype == torch.float32 and norm.requires_grad
-        with torch.no_grad():
-            assert not ops.grad_norm([p]).requires_grad
-        assert not ops.grad_norm([p.detach()]).requires_grad
-        # clipping is not recorded, as torch.nn.utils.clip_grad_norm_ is not
-        assert not ops.clip_grad_norm_([p * 2.0], 1.0).requires_grad and not ops.clip_grad_norm_([p * 2.0], 1.0, out=[_gpu(4, 32)]).requires_grad
