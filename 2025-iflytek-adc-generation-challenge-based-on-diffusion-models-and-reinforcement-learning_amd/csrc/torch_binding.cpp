@@ -458,7 +458,7 @@ std::vector<Tensor> residual_norm_autograd(const OptTensor& h, const Tensor& x, 
     return op.call(h, x, gate, post_weight, post_bias, pre_weight, pre_bias, post_norm, pre_norm, residual_scale, eps, with_x, with_stats);
 }
 
-// the norm of gradients that themselves require one (create_graph) is not differentiated
+// Gradients that themselves require one (create_graph): the norm is a constant, as torch.nn.utils' total norm is, and the clipping is not recorded
 Tensor grad_norm_autograd(at::TensorList grads, int64_t norm_type) {
     static const auto op = below_autograd("adcdiff::grad_norm", &grad_norm);
     no_tangents("grad_norm", grads);

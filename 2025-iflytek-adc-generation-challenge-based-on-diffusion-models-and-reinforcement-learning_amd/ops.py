@@ -383,7 +383,8 @@ def _as_list(tensors):
 def grad_norm(grads, norm_type=2.0):
     """The norm over all elements of all gradient tensors (float32 and bfloat16, any shapes without gaps in memory): a float32 scalar on
     their device.  norm_type 2 (squares summed in float64, so nothing overflows on the way) or inf (largest magnitude).  No
-    synchronisation, the same bits every run; NaN if any element is.  An empty list has norm 0, on the CPU."""
+    synchronisation, the same bits every run; NaN if any element is.  An empty list has norm 0, on the CPU.  The norm is a constant for
+    autograd, as the total norm of torch.nn.utils is: a penalty on it has no gradient."""
     grads, code = _as_list(grads), _norm_type(norm_type)
     return _call("grad_norm", grads, code) if grads else torch.zeros(())
 
@@ -394,7 +395,8 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, error_if_nonfinite=False, ou
     In place; with `out`, a list of tensors of the same shapes (float32 or bfloat16, such as views of an optimizer's float32 arena),
     the scaled gradients go there and `grads` stay.  Tensors that are written must not overlap one another or another gradient.
     A norm that is not finite is handled as torch.nn.utils.clip_grad_norm_ does: NaN gradients from a NaN norm, zeros (and NaN for the
-    infinite elements) from an infinite one; error_if_nonfinite raises before anything is written, at the price of a synchronisation."""
+    infinite elements) from an infinite one; error_if_nonfinite raises before anything is written, at the price of a synchronisation.  As
+    there, autograd does not record it."""
     grads, code, max_norm = _as_list(grads), _norm_type(norm_type), float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("max_norm must not be negative or NaN, got %r" % max_norm)

@@ -86,3 +86,13 @@ def test_forward_mode_of_the_path_is_refused(name):
             call(forward_ad.make_dual(torch.zeros(4, 32), torch.zeros(4, 32)))
     with pytest.raises(NotImplementedError, match="forward"):
         torch.func.jvp(call, (torch.zeros(4, 32),), (torch.zeros(4, 32),))
+
+
+def test_norms_are_constants():
+    """of tensors that require a gradient too, as the total norm of torch.nn.utils is; a compiled step may return them beside its loss"""
+    with FakeTensorMode():
+        p = _gpu(4, 32).requires_grad_()
+        for call in (lambda: ops.grad_norm([_gpu(3), p * 2.0]), lambda: ops.grad_norm([p], "inf"), lambda: ops.clip_grad_norm_([p * 2.0], 1.0),
+                     lambda: ops.clip_grad_norm_([p * 2.0], 1.0, out=[_gpu(4, 32)])):
+            norm = call()
+            assert norm.shape == () and norm.dtype == torch.float32 and not norm.requires_grad
